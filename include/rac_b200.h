@@ -1,7 +1,7 @@
 /*
  * rac_b200.h -- extensions of the RAC C API exported by librac_b200.so.
  *
- * Three groups:
+ * Four groups:
  *  1. error channel and process-wide knobs (the reference binding keeps the
  *     same knobs in rac_torch/rac_torch_bind.cpp:54-55, :205-219);
  *  2. batch forms of the _n primitives of lib/c/rac_cpu.h:110-114 and the
@@ -10,7 +10,10 @@
  *     rac_torch/rac_kernels.hip:822-909 with the same names and argument
  *     meaning, plus *_async forms of every op for callers that own device
  *     memory and a cudaStream_t (passed as void*).  These never synchronise
- *     and return a status; the PyTorch layer binds to them.
+ *     and return a status; the PyTorch layer binds to them;
+ *  4. attention over packed prompts (forward and backward), attention of new
+ *     tokens over a paged key/value cache, and the pages of that cache; no
+ *     counterpart in the reference, stream-ordered like group 3.
  *
  * Status codes follow lib/c/rac_cpu.h:54-59 and extend them.
  */
@@ -163,6 +166,84 @@ int rac_attention_async(const float *q, const float *k, const float *v, const fl
 /* Reads and clears the device's error word (bounded-loop overruns) after
  * synchronising `stream`; returns RAC_OK or RAC_ERR_DEVICE. */
 int rac_check_device_errors(void *stream);
+
+/* ── 4. packed prompts and paged caches ─────────────────────────────────── */
+/* Element types.  Sums, softmax statistics and gradients are held in 32 bits
+ * whatever the type.  head_dim is 32, 64 or 128; query head h reads key/value
+ * head h / (heads / kv_heads).  All pointers are device pointers except
+ * `strides`, a host array of element strides; bases are 16-byte aligned and
+ * strides are multiples of 16 bytes, the last axis is contiguous. */
+#define RAC_F32  0
+#define RAC_F16  1
+#define RAC_BF16 2
+
+/* softmax(scale q k^T) v within each of n_seqs sequences laid end to end:
+ * sequence i holds rows cu_seqlens[i] .. cu_seqlens[i+1]-1 (cu_seqlens[0] is
+ * 0, n_seqs+1 rising int32), lengths of 0 allowed.  q [tokens, heads,
+ * head_dim], k and v [tokens, kv_heads, head_dim]; strides = {q row, q head,
+ * k row, k head, v row, v head}.  out [tokens, heads, head_dim] contiguous;
+ * lse (optional) [heads, tokens], the natural logarithm of each row's sum.
+ * Rows behind the last sequence stay as they are, or become zeros where
+ * zero_rest is set.  workspace: rac_attention_packed_workspace() bytes,
+ * 256-byte aligned (may be NULL where that is 0). */
+long long rac_attention_packed_workspace(long long tokens, int n_seqs, int heads, int kv_heads, int head_dim,
+                                         int dtype, int backward);
+int rac_attention_packed_async(const void *q, const void *k, const void *v, const long long *strides,
+                               const int *cu_seqlens, int n_seqs, long long tokens, int heads, int kv_heads,
+                               int head_dim, int dtype, int is_causal, float scale, void *out, float *lse,
+                               int zero_rest, void *workspace, long long ws_bytes, void *stream);
+/* Gradients of the above from the forward's out and lse: dq like q, dk and dv
+ * like k (contiguous), zeros behind the last sequence.  strides = {q row, q
+ * head, k row, k head, v row, v head, dout row, dout head}.  No atomics: the
+ * same inputs give the same bits. */
+int rac_attention_packed_backward_async(const void *dout, const void *q, const void *k, const void *v,
+                                        const long long *strides, const void *out, const float *lse,
+                                        const int *cu_seqlens, int n_seqs, long long tokens, int heads,
+                                        int kv_heads, int head_dim, int dtype, int is_causal, float scale,
+                                        void *dq, void *dk, void *dv, void *workspace, long long ws_bytes,
+                                        void *stream);
+
+/* Attention of new tokens over a paged cache.  Pages hold [kv_heads,
+ * page_size, head_dim] each; cache row r of sequence b lies in page
+ * page_table[b, r / page_size] (int32 [batch, table_width]), slot r %
+ * page_size.  lengths[b] counts its rows, the new ones (the last counts[b],
+ * or `nodes` where counts is NULL; at most 64) included: they are in the
+ * cache already.  New row i sees every row before the new ones and the new
+ * rows j whose bit is set in tree[b, i] (int64 [batch, nodes]), j <= i where
+ * tree is NULL; a row that sees nothing gives zeros.  q [batch, nodes, heads,
+ * head_dim] with strides = {q batch, q node, q head, k page, k head, k row,
+ * v page, v head, v row}; out contiguous, rows from counts[b] on as they were
+ * or zeros (zero_rest).  Pages outside [0, n_pages) are not read: their rows
+ * count as hidden and rac_check_device_errors() reports RAC_ERR_DEVICE.
+ * workspace: rac_attention_cached_workspace() bytes, 256-byte aligned. */
+long long rac_attention_cached_workspace(int batch, int nodes, int heads, int kv_heads, int head_dim);
+int rac_attention_cached_async(const void *q, const void *k_pages, const void *v_pages, const long long *strides,
+                               const int *page_table, int table_width, int n_pages, int page_size,
+                               const int *lengths, const int *counts, const long long *tree, int batch, int nodes,
+                               int heads, int kv_heads, int head_dim, int dtype, float scale, void *out,
+                               int zero_rest, void *workspace, long long ws_bytes, void *stream);
+
+/* Page operations.  strides = {k layer, page, head, row, v layer, page, head,
+ * row, ...}.  Rows and pages outside the cache are skipped and reported as
+ * above. */
+/* Rows cu_seqlens[b] .. of k and v (strides[8..11] = k row, k head, v row, v
+ * head) to cache rows starts[b] .. of sequence b. */
+int rac_cache_append_async(void *k_pages, void *v_pages, const long long *strides, const void *k, const void *v,
+                           const int *page_table, int table_width, int n_pages, int page_size, const int *starts,
+                           const int *cu_seqlens, int batch, long long tokens, int kv_heads, int head_dim, int dtype,
+                           void *stream);
+/* Page src[i] to page dst[i], in every layer.  No page may be a destination
+ * twice, nor a source and a destination (the copies run at once). */
+int rac_cache_copy_pages_async(void *k_pages, void *v_pages, const long long *strides, const int *src,
+                               const int *dst, int n, int layers, int n_pages, int page_size, int kv_heads,
+                               int head_dim, int dtype, void *stream);
+/* Cache row starts[b] + accepted[b, i] to row starts[b] + i for i <
+ * n_accepted[b], in every layer; all of a sequence's rows are read before the
+ * first is written.  nodes (the width of accepted) is at most 64. */
+int rac_cache_compact_async(void *k_pages, void *v_pages, const long long *strides, const int *page_table,
+                            int table_width, int n_pages, int page_size, const int *starts, const int *accepted,
+                            const int *n_accepted, int batch, int nodes, int layers, int kv_heads, int head_dim,
+                            int dtype, void *stream);
 
 /* ── op descriptors for rac_execute ─────────────────────────────────────── */
 typedef struct { const float *A, *B; float *C; int M, N, K; } rac_matmul_desc;

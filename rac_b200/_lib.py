@@ -100,6 +100,19 @@ _SIGS = {
     "rac_rope_apply_async": (_i, [_vp, _vp, _vp, _vp, _ll, _i, _i, _i, _vp]),
     "rac_check_device_errors": (_i, [_vp]),
     "rac_attention": (None, [_vp, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i]),
+    "rac_attention_packed_workspace": (_ll, [_ll, _i, _i, _i, _i, _i, _i]),
+    "rac_attention_packed_async": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _ll, _i, _i, _i, _i, _i, _f, _vp,
+                                        _vp, _i, _vp, _ll, _vp]),
+    "rac_attention_packed_backward_async": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _ll, _i,
+                                                 _i, _i, _i, _i, _f, _vp, _vp, _vp, _vp, _ll, _vp]),
+    "rac_attention_cached_workspace": (_ll, [_i, _i, _i, _i, _i]),
+    "rac_attention_cached_async": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _vp, _vp, _i, _i, _i,
+                                        _i, _i, _i, _f, _vp, _i, _vp, _ll, _vp]),
+    "rac_cache_append_async": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _vp, _i, _ll, _i, _i,
+                                    _i, _vp]),
+    "rac_cache_copy_pages_async": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp]),
+    "rac_cache_compact_async": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i,
+                                     _i, _vp]),
     "rac_attention_async": (_i, [_vp, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, _vp]),
 }
 

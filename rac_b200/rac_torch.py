@@ -9,6 +9,10 @@ written against it runs unchanged:
     RACLlamaBlock, patch_model, unpatch_model, rac_set_precision,
     rac_get_precision, rac_set_mode, rac_get_mode, rac_info.
 
+Beyond it: rac_attention_packed (attention over packed sequences with grouped
+key/value heads, differentiable), and the n_kv_heads, cu_seqlens and cache
+arguments of RACRoPEAttention and RACLlamaBlock (see cache.py).
+
 Differences, all deliberate:
   * no CPU fallback: the reference silently runs torch ops when its
     extension is unavailable (rac_torch.py:183, :232); here a CPU tensor in
@@ -34,12 +38,13 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 
 from . import _lib, ext
 from .ext import ACT_GELU, ACT_NONE, ACT_RELU, ACT_SILU, MODE_CORDIC, MODE_FAST, MODE_SHIFTADD
 
 __all__ = [
-    "rac_matmul", "rac_linear", "RACLinear", "FusedRACLinear", "RACFusedQKV", "RACFusedFFN",
+    "rac_matmul", "rac_linear", "rac_attention_packed", "RACLinear", "FusedRACLinear", "RACFusedQKV", "RACFusedFFN",
     "RACRoPE", "RACRMSNorm", "RACLayerNorm", "RACRoPEAttention", "RACLlamaBlock",
     "patch_model", "unpatch_model", "rac_set_precision", "rac_get_precision",
     "rac_set_mode", "rac_get_mode", "rac_info", "MODE_FAST", "MODE_CORDIC", "MODE_SHIFTADD",
@@ -158,6 +163,78 @@ def _act_torch(x, act_id):
     if act_id == ACT_SILU:
         return F.silu(x)
     return x
+
+
+class RACAttentionPackedFunction(Function):
+    """Attention over packed sequences; backward from the saved output and row sums."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, cu_seqlens, is_causal, scale):
+        lse = torch.empty((q.shape[1], q.shape[0]), device=q.device, dtype=torch.float32) \
+            if any(ctx.needs_input_grad[:3]) else None
+        out = ext.attention_packed(q, k, v, cu_seqlens, is_causal, scale, lse=lse)
+        ctx.save_for_backward(q, k, v, out, lse, cu_seqlens)
+        ctx.is_causal, ctx.scale = is_causal, scale
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out):
+        q, k, v, out, lse, cu_seqlens = ctx.saved_tensors
+        return (*ext.attention_packed_backward(grad_out, q, k, v, out, lse, cu_seqlens, ctx.is_causal, ctx.scale),
+                None, None, None)
+
+
+class _RoPEFunction(Function):
+    """The pair rotation of x [..., seq, dim] by tables cos, sin [seq, dim / 2]; its
+    gradient is the rotation by the opposite angles."""
+
+    @staticmethod
+    def forward(ctx, x, cos, sin):
+        ctx.save_for_backward(cos, sin)
+        return _rope(x, cos, sin)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        cos, sin = ctx.saved_tensors
+        return _rope(g, cos, -sin), None, None
+
+
+def _rope(x, cos, sin):
+    out = x.to(torch.float32, memory_format=torch.contiguous_format, copy=True)
+    ext.rope_apply_(out, cos, sin, form=1)
+    return out if x.dtype == torch.float32 else out.to(x.dtype)
+
+
+class _RMSNormFunction(Function):
+    """RMSNorm on the row kernel with its gradient: with r = rsqrt(mean(x^2) + eps) and
+    h = g * weight, dx = r (h - x r^2 mean(h x)), dweight = sum over rows of g x r."""
+
+    @staticmethod
+    def forward(ctx, x, weight, eps):
+        ctx.save_for_backward(x, weight)
+        ctx.eps = eps
+        y = ext.rmsnorm(x.float().contiguous(), weight.float().contiguous(), eps)
+        return y if x.dtype == torch.float32 else y.to(x.dtype)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        x, weight = ctx.saved_tensors
+        xf, gf = x.float(), g.float()
+        r = torch.rsqrt(xf.square().mean(-1, keepdim=True) + ctx.eps)
+        h = gf * weight.float()
+        dx = r * (h - xf * (r * r * (h * xf).mean(-1, keepdim=True)))
+        dw = (gf * xf * r).reshape(-1, x.shape[-1]).sum(0)
+        return dx.to(x.dtype), dw.to(weight.dtype), None
+
+
+def rac_attention_packed(q, k, v, cu_seqlens, is_causal: bool = True, scale: Optional[float] = None):
+    """softmax(scale q k^T) v within each sequence of a packed batch, differentiable in q, k and v:
+    q [tokens, heads, dim], k and v [tokens, kv_heads, dim], sequence i in rows cu_seqlens[i] ..
+    cu_seqlens[i + 1] - 1.  See ext.attention_packed."""
+    return RACAttentionPackedFunction.apply(q, k, v, cu_seqlens, is_causal, scale)
 
 
 def rac_matmul(A: torch.Tensor, B: torch.Tensor) -> torch.Tensor:
@@ -393,16 +470,34 @@ class RACRoPEAttention(nn.Module):
     Q and K, softmax(QK^T * scale + mask) V, out_proj RACLinear.  In inference
     the attention core is this library's fused kernel (rac_attention, no
     [B, H, T, T] tensor); under autograd it is torch.matmul + softmax in fp32,
-    as in the reference module."""
+    as in the reference module.
+
+    Three things go beyond the reference, and run on the packed-prompt and
+    paged-cache kernels, differentiable throughout without a cache:
+
+    * n_kv_heads < n_heads: grouped key/value heads; qkv projects to
+      d_model + 2 * n_kv_heads * d_head;
+    * forward(x, cu_seqlens=...): x holds sequences of different lengths laid
+      end to end ([tokens, d] or [1, tokens, d]).  RoPE positions count from each
+      sequence's start.  Their tables hold max_seq_len rows: where x has more
+      rows than that, pass max_seqlen (the longest sequence) or positions;
+    * forward(x, cache=step, layer=i): x holds the new tokens of the sequences of
+      a RACCacheStep (cache.py) in its order; they join the cache and attend
+      over it.  No gradients."""
 
     def __init__(self, d_model: int, n_heads: int, max_seq_len: int = 4096, bias: bool = False,
-                 dropout: float = 0.0, rope_base: float = 10000.0, device=None, dtype=None):
+                 dropout: float = 0.0, rope_base: float = 10000.0, device=None, dtype=None,
+                 n_kv_heads: Optional[int] = None):
         super().__init__()
         assert d_model % n_heads == 0
         self.d_model, self.n_heads = d_model, n_heads
+        self.n_kv_heads = n_heads if n_kv_heads is None else n_kv_heads
+        if self.n_kv_heads < 1 or n_heads % self.n_kv_heads:
+            raise ValueError(f"n_heads={n_heads} must be a multiple of n_kv_heads={self.n_kv_heads}")
         self.d_head = d_model // n_heads
         self.scale = self.d_head ** -0.5
-        self.qkv = RACLinear(d_model, 3 * d_model, bias=bias, device=device, dtype=dtype)
+        self.qkv = RACLinear(d_model, d_model + 2 * self.n_kv_heads * self.d_head, bias=bias, device=device,
+                             dtype=dtype)
         self.out_proj = RACLinear(d_model, d_model, bias=bias, device=device, dtype=dtype)
         self.rope = RACRoPE(self.d_head, max_seq_len=max_seq_len, base=rope_base,
                             device=device, dtype=dtype or torch.float32)
@@ -440,11 +535,81 @@ class RACRoPEAttention(nn.Module):
         out = torch.matmul(attn, v)
         return out.transpose(1, 2).reshape(B, T, H * self.d_head)
 
-    def forward(self, x, mask=None, is_causal=False, positions=None):
+    def _rotate_rows(self, q, k, positions):
+        """RoPE of q [T, H, hd] and k [T, Hkv, hd] at positions [T]."""
+        pos = positions.to(torch.long).clamp(0, self.rope.max_seq_len - 1)
+        c = self.rope.cos_cache[pos].float().contiguous()
+        s = self.rope.sin_cache[pos].float().contiguous()
+        return tuple(_RoPEFunction.apply(t.transpose(0, 1), c, s).transpose(0, 1) for t in (q, k))
+
+    def _packed_positions(self, cu, tokens, max_seqlen):
+        longest = tokens if max_seqlen is None else max_seqlen
+        if longest > self.rope.max_seq_len:
+            raise ValueError(f"sequences of up to {longest} rows, RoPE tables of {self.rope.max_seq_len}: "
+                             "pass max_seqlen or positions")
+        tok = torch.arange(tokens, device=cu.device, dtype=torch.int32)
+        seq = torch.searchsorted(cu, tok, right=True) - 1
+        return tok - cu[seq]
+
+    def _rows_context(self, x, is_causal=False, positions=None, cu_seqlens=None, cache=None, layer=0,
+                      max_seqlen=None):
+        """Attention output before out_proj on the packed and cached kernels, in x's leading shape."""
+        if not isinstance(self.dropout, nn.Identity) and self.training:
+            raise ValueError("grouped, packed and cached attention take no dropout")
+        H, Hk, hd = self.n_heads, self.n_kv_heads, self.d_head
+        lead, T = x.shape[:-1], x.shape[:-1].numel()
+        if cache is not None:
+            if cu_seqlens is not None or positions is not None:
+                raise ValueError("a cache step brings its own cu_seqlens and positions")
+            if not is_causal:
+                raise ValueError("attention over a cache is causal: pass is_causal=True")
+            if T != cache.tokens:
+                raise ValueError(f"the cache step has {cache.tokens} new rows, x has {T}")
+            if cache.longest > self.rope.max_seq_len:
+                raise ValueError(f"sequences of {cache.longest} rows, RoPE tables of {self.rope.max_seq_len}")
+            if torch.is_grad_enabled() and (x.requires_grad or self.qkv.weight.requires_grad):
+                raise ValueError("attention over a cache has no gradient: use torch.no_grad()")
+            cu, positions = cache.cu_seqlens, cache.positions
+        elif cu_seqlens is None:
+            if x.dim() != 3:
+                raise ValueError("x must be [batch, seq, d_model]")
+            cu = torch.arange(0, T + 1, max(1, x.shape[1]), device=x.device, dtype=torch.int32)
+            if positions is not None:
+                positions = positions.to(x.device).repeat(x.shape[0])
+            else:
+                positions = torch.arange(x.shape[1], device=x.device).repeat(x.shape[0])
+            max_seqlen = x.shape[1]
+        else:
+            if x.dim() == 3 and x.shape[0] != 1:
+                raise ValueError("packed x must be [tokens, d_model] or [1, tokens, d_model]")
+            cu = cu_seqlens.to(torch.int32)
+        if positions is None:
+            positions = self._packed_positions(cu, T, max_seqlen)
+        elif tuple(positions.shape) != (T,):
+            raise ValueError(f"positions must be [{T}], got {tuple(positions.shape)}")
+        qkv = self.qkv(x).reshape(T, H + 2 * Hk, hd)
+        q, k, v = qkv[:, :H], qkv[:, H:H + Hk], qkv[:, H + Hk:]
+        q, k = self._rotate_rows(q, k, positions)
+        if cache is not None:
+            return cache.attend(layer, q, k, v, self.scale).reshape(*lead, H * hd)
+        return rac_attention_packed(q, k, v, cu, is_causal, self.scale).reshape(*lead, H * hd)
+
+    def _needs_rows(self, mask, cu_seqlens, cache):
+        if self.n_kv_heads == self.n_heads and cu_seqlens is None and cache is None:
+            return False
+        if mask is not None:
+            raise ValueError("grouped, packed and cached attention take no mask")
+        return True
+
+    def forward(self, x, mask=None, is_causal=False, positions=None, cu_seqlens=None, cache=None, layer=0,
+                max_seqlen=None):
+        if self._needs_rows(mask, cu_seqlens, cache):
+            return self.out_proj(self._rows_context(x, is_causal, positions, cu_seqlens, cache, layer, max_seqlen))
         return self.out_proj(self._context(x, mask, is_causal, positions))
 
     def extra_repr(self):
-        return f"d_model={self.d_model}, n_heads={self.n_heads}, d_head={self.d_head}"
+        kv = f", n_kv_heads={self.n_kv_heads}" if self.n_kv_heads != self.n_heads else ""
+        return f"d_model={self.d_model}, n_heads={self.n_heads}, d_head={self.d_head}{kv}"
 
 
 class RACLlamaBlock(nn.Module):
@@ -453,18 +618,22 @@ class RACLlamaBlock(nn.Module):
     Same submodule names and parameter shapes as the reference, so its
     state_dict loads unchanged.  gated=True swaps the FFN for the SwiGLU
     form (RACGatedFFN).  In inference (no grad) the two residual adds are
-    fused into the out_proj / down-projection GEMM epilogues."""
+    fused into the out_proj / down-projection GEMM epilogues.
+
+    n_kv_heads, cu_seqlens, cache, layer and max_seqlen: see RACRoPEAttention.  With
+    any of them, gradients run through the norms and RoPE as well."""
 
     def __init__(self, d_model: int, n_heads: int, ff_dim: int = None, max_seq_len: int = 4096,
                  activation: str = "silu", dropout: float = 0.0, bias: bool = False,
                  rms_eps: float = 1e-6, rope_base: float = 10000.0, gated: bool = False,
-                 device=None, dtype=None):
+                 device=None, dtype=None, n_kv_heads: Optional[int] = None):
         super().__init__()
         ff_dim = ff_dim or 4 * d_model
         self.gated = gated
         self.norm1 = RACRMSNorm(d_model, eps=rms_eps, device=device, dtype=dtype)
         self.attn = RACRoPEAttention(d_model, n_heads, max_seq_len=max_seq_len, bias=bias,
-                                     dropout=dropout, rope_base=rope_base, device=device, dtype=dtype)
+                                     dropout=dropout, rope_base=rope_base, device=device, dtype=dtype,
+                                     n_kv_heads=n_kv_heads)
         self.norm2 = RACRMSNorm(d_model, eps=rms_eps, device=device, dtype=dtype)
         if gated:
             self.ffn = RACGatedFFN(d_model, ff_dim, bias=bias, device=device, dtype=dtype)
@@ -472,7 +641,17 @@ class RACLlamaBlock(nn.Module):
             self.ffn = RACFusedFFN(d_model, ff_dim, activation=activation, bias=bias,
                                    device=device, dtype=dtype)
 
-    def forward(self, x, mask=None, is_causal=False, positions=None):
+    def forward(self, x, mask=None, is_causal=False, positions=None, cu_seqlens=None, cache=None, layer=0,
+                max_seqlen=None):
+        if self.attn._needs_rows(mask, cu_seqlens, cache):
+            kw = dict(is_causal=is_causal, positions=positions, cu_seqlens=cu_seqlens, cache=cache, layer=layer,
+                      max_seqlen=max_seqlen)
+            if torch.is_grad_enabled():
+                n1, n2 = self.norm1, self.norm2
+                x = x + self.attn(_RMSNormFunction.apply(x, n1.weight, n1.eps), **kw)
+                return x + self.ffn(_RMSNormFunction.apply(x, n2.weight, n2.eps))
+            h = self.attn.out_proj.forward_residual(self.attn._rows_context(self.norm1(x), **kw), x)
+            return self.ffn.forward_residual(self.norm2(h), h)
         if torch.is_grad_enabled():
             x = x + self.attn(self.norm1(x), mask=mask, is_causal=is_causal, positions=positions)
             return x + self.ffn(self.norm2(x))

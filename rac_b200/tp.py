@@ -50,6 +50,8 @@ class TPLlamaBlock(nn.Module):
         super().__init__()
         a = full.attn
         H, hd, d = a.n_heads, a.d_head, a.d_model
+        if a.n_kv_heads != H:
+            raise ValueError("tensor parallelism takes no grouped key/value heads")
         if H % world:
             raise ValueError(f"n_heads={H} not divisible by world={world}")
         self.world, self.rank, self.group = world, rank, group

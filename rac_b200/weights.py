@@ -9,7 +9,9 @@ RACLlamaBlock(gated=True):
 
 * q/k/v/o_proj -> attn.qkv (concatenated) and attn.out_proj;
 * grouped-query K/V heads (n_kv_heads < n_heads) are repeated per query
-  head, as the reference decoder does (bench_rac_transformer.c:402-427);
+  head, as the reference decoder does (bench_rac_transformer.c:402-427), or
+  kept as they are with repeat_kv=False (RACLlamaBlock's n_kv_heads: the cache
+  then holds only them);
 * q/k rows are permuted from the rotate-half RoPE layout of HF checkpoints to
   the interleaved pairs (x[2i], x[2i+1]) that RACRoPE rotates
   (rac_torch/rac_torch.py:1165-1181), so the block computes the checkpoint's
@@ -93,7 +95,8 @@ def rotate_half_to_interleaved(w: torch.Tensor, n_heads: int) -> torch.Tensor:
 
 def load_llama_layer(tensors_or_path, layer: int, n_heads: int, n_kv_heads: int | None = None,
                      rms_eps: float = 1e-5, rope_base: float = 10000.0, max_seq_len: int = 2048,
-                     hf_rope: bool = True, prefix: str = "model.layers", device="cuda") -> RACLlamaBlock:
+                     hf_rope: bool = True, prefix: str = "model.layers", device="cuda",
+                     repeat_kv: bool = True) -> RACLlamaBlock:
     """RACLlamaBlock(gated=True) holding layer `layer` of a Llama checkpoint."""
     p = f"{prefix}.{layer}."
     keys = ["self_attn.q_proj.weight", "self_attn.k_proj.weight", "self_attn.v_proj.weight",
@@ -129,10 +132,12 @@ def load_llama_layer(tensors_or_path, layer: int, n_heads: int, n_kv_heads: int 
         wk = rotate_half_to_interleaved(wk, n_kv)
     rep = n_heads // n_kv
     # K/V head j serves query heads j*rep .. j*rep+rep-1.
-    wk = wk.reshape(n_kv, hd, d).repeat_interleave(rep, dim=0).reshape(n_heads * hd, d)
-    wv = wv.reshape(n_kv, hd, d).repeat_interleave(rep, dim=0).reshape(n_heads * hd, d)
+    if repeat_kv:
+        wk = wk.reshape(n_kv, hd, d).repeat_interleave(rep, dim=0).reshape(n_heads * hd, d)
+        wv = wv.reshape(n_kv, hd, d).repeat_interleave(rep, dim=0).reshape(n_heads * hd, d)
     blk = RACLlamaBlock(d, n_heads, ff_dim=ff, max_seq_len=max_seq_len, bias=False,
-                        rms_eps=rms_eps, rope_base=rope_base, gated=True)
+                        rms_eps=rms_eps, rope_base=rope_base, gated=True,
+                        n_kv_heads=None if repeat_kv else n_kv)
     with torch.no_grad():
         blk.attn.qkv.weight.copy_(torch.cat([wq, wk, wv], 0))
         blk.attn.out_proj.weight.copy_(g["self_attn.o_proj.weight"])
