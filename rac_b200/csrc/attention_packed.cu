@@ -379,7 +379,7 @@ int by_type(const PackedParams& p, cudaStream_t s) {
 // 16-byte loads: aligned base, strides of whole 16-byte units.
 bool rows_ok(const Rows& r, int type) {
     const int e = elem_bytes(type);
-    return (reinterpret_cast<uintptr_t>(r.p) & 15u) == 0 && (r.row * e) % 16 == 0 && (r.head * e) % 16 == 0;
+    return (reinterpret_cast<uintptr_t>(r.p) & 15u) == 0 && (r.row * e) % 16 == 0 && (r.head * e) % 16 == 0 && r.row >= 0 && r.head >= 0;
 }
 
 int check(const PackedParams& p) {
@@ -404,6 +404,7 @@ int attention_packed(const PackedParams& p, cudaStream_t s) {
     if (p.tokens == 0) return kOk;
     if (!p.out) return kErrNullPtr;
     if (reinterpret_cast<uintptr_t>(p.out) & 15u) return kErrUnsupported;
+    if (p.type != kF32) return attention_packed_tc(p, s);
     return by_type<Fwd>(p, s);
 }
 

@@ -36,6 +36,7 @@ struct PackedParams {
 
 size_t attention_packed_workspace(long long tokens, int n_seqs, int heads, int kv_heads, int head_dim, int type,
                                   int backward);
+int attention_packed_tc(const PackedParams& p, cudaStream_t s);      // float16, bfloat16: arguments checked
 int attention_packed(const PackedParams& p, cudaStream_t s);
 int attention_packed_backward(const PackedParams& p, cudaStream_t s);
 

@@ -87,6 +87,23 @@ bool encode_tensor_2d(CUtensorMap* map, const float* base, uint64_t inner, uint6
                CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+bool encode_tensor(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* base, const uint64_t* dims,
+                   const uint64_t* strides, const uint32_t* box, int swizzle_bytes) {
+    auto enc = tensor_map_encoder();
+    if (!enc || rank < 2 || rank > 5 || (reinterpret_cast<uintptr_t>(base) & 15u)) return false;
+    cuuint64_t d[5], st[4];
+    cuuint32_t b[5], es[5];
+    for (int i = 0; i < rank; ++i) { d[i] = dims[i]; b[i] = box[i]; es[i] = 1; }
+    for (int i = 0; i + 1 < rank; ++i) {
+        if (strides[i] == 0 || (strides[i] & 15)) return false;
+        st[i] = strides[i];
+    }
+    const auto swz = swizzle_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B
+                   : swizzle_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_NONE;
+    return enc(map, type, (cuuint32_t)rank, const_cast<void*>(base), d, st, b, es, CU_TENSOR_MAP_INTERLEAVE_NONE, swz,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 static bool encode_2d(CUtensorMap* map, const float* base, uint64_t inner, uint64_t outer,
                       long long ld, uint32_t box_inner, uint32_t box_outer) {
     return encode_tensor_2d(map, base, inner, outer, ld, box_inner, box_outer, false);

@@ -64,6 +64,11 @@ bool make_tensor_maps(GemmParams& p, int layout, int BM, int BN, int BK);
 bool encode_tensor_2d(CUtensorMap* map, const float* base, uint64_t inner, uint64_t outer,
                       long long ld, uint32_t box_inner, uint32_t box_outer, bool swizzle128);
 
+// A tensor map of any rank up to 5 and type: dims and box innermost first,
+// byte strides of the outer axes, swizzle 128, 64 or 0 bytes.
+bool encode_tensor(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* base, const uint64_t* dims,
+                   const uint64_t* strides, const uint32_t* box, int swizzle_bytes);
+
 // launch_gemm without the split-K decision: launches the tile kernel for p
 // as given (p.ws == nullptr: whole K per CTA).
 int launch_gemm_into(const GemmParams& p, int layout, int mode, int variant,

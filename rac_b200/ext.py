@@ -383,10 +383,11 @@ def _same_device(*ts: torch.Tensor) -> None:
 
 
 def _fits(t: torch.Tensor) -> bool:
-    """Whether the kernels take t as it lies: contiguous last axis, 16-byte aligned base and strides."""
+    """Whether the kernels take t as it lies: contiguous last axis, 16-byte aligned base and strides, no axis
+    expanded."""
     e = t.element_size()
     return t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(
-        s * e % 16 == 0 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1)
+        s > 0 and s * e % 16 == 0 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1)
 
 
 def _lay(t: torch.Tensor) -> torch.Tensor:
