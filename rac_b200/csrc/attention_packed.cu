@@ -386,7 +386,9 @@ int check(const PackedParams& p) {
     if (p.tokens < 0 || p.n_seqs < 0 || p.heads <= 0 || p.kv_heads <= 0 || p.heads % p.kv_heads) return kErrInvalidDim;
     if (p.type < kF32 || p.type > kBF16) return kErrUnsupported;
     if (p.head_dim != 32 && p.head_dim != 64 && p.head_dim != 128) return kErrUnsupported;
-    if (p.tokens >= (1LL << 31) - (1 << 20) || p.heads > 65535) return kErrInvalidDim;
+    if (p.tokens >= (1LL << 30) || p.heads > 65535 || p.n_seqs >= (1 << 30) ||
+        packed_slots(p.tokens, p.n_seqs, kB) * p.heads >= (1LL << 31))
+        return kErrInvalidDim;
     if (p.tokens && (!p.q.p || !p.k.p || !p.v.p || (p.n_seqs && !p.cu))) return kErrNullPtr;
     if (!rows_ok(p.q, p.type) || !rows_ok(p.k, p.type) || !rows_ok(p.v, p.type)) return kErrUnsupported;
     return kOk;
@@ -394,9 +396,9 @@ int check(const PackedParams& p) {
 
 }  // namespace
 
-// Backward: D, [heads, tokens].
+// Backward: D, [heads, tokens], and two largest values.
 size_t attention_packed_workspace(long long tokens, int, int heads, int, int, int, int backward) {
-    return backward ? sizeof(float) * (size_t)tokens * heads : 0;
+    return backward ? sizeof(float) * ((size_t)tokens * heads + 2) : 0;
 }
 
 int attention_packed(const PackedParams& p, cudaStream_t s) {
@@ -417,6 +419,7 @@ int attention_packed_backward(const PackedParams& p, cudaStream_t s) {
         return kErrAlloc;
     for (const void* x : {p.out_in, (const void*)p.dq, (const void*)p.dk, (const void*)p.dv})
         if (reinterpret_cast<uintptr_t>(x) & 15u) return kErrUnsupported;
+    if (p.type != kF32) return attention_packed_backward_tc(p, s);
     return by_type<Bwd>(p, s);
 }
 

@@ -1,0 +1,644 @@
+// attention_packed_bwd_tc.cu -- gradients of attention over packed prompts on
+// the tensor cores, float16 and bfloat16.
+//
+// Two kernels, each with its sums in tensor memory and no atomics: one keeps a
+// tile of 128 queries and runs over the keys (dq), one keeps a tile of 128 keys
+// and runs over the queries of all heads of its group (dk and dv).  Both
+// compute S and dP anew: seven products where one kernel would do with five,
+// but dq would then be added up by atomics, in an order that changes.
+//
+// In the dk/dv kernel everything is transposed, so that P^T and dS^T have a key
+// a lane and feed dV += P^T dO and dK += dS^T Q from tensor memory.  The order
+//   dV(i), S(i+1), dK(i), dP(i+1), dV(i+1), ...
+// keeps the tensor core at work while the weights P(i+1) are taken from S(i+1)
+// and dS(i+1) from dP(i+1): P(i) lies in S(i)'s columns and dS(i) in dP(i)'s, so
+// that four 128-column blocks (S, dP, dK, dV) fill the 512 columns.
+//
+// float16: weights below 2^-14 and dS of small gradients would fall among the
+// subnormal numbers and lose their digits.  P carries a factor 2^10, and dS a
+// power of two taken from the largest |do| and |v| that keeps it below the
+// type's largest value: |dS| <= 2 head_dim max|do| max|v|.
+#include "attn_common.cuh"
+#include "tensor_core.cuh"
+
+namespace racb {
+namespace {
+
+using namespace tc;
+
+constexpr int kTile = 128;
+// Warps 0-3 and 4-7: columns 0-63 and 64-127 of a tile, a thread a row; 8: matrix
+// instructions; 9: loads; 10: row statistics.
+constexpr int kThreads = 384;
+constexpr int kLaunchRegs = 168, kMathRegs = 216, kOtherRegs = 72;
+static_assert(kMathRegs * 256 + kOtherRegs * 128 <= kLaunchRegs * kThreads, "register split");
+
+struct BwdArgs {
+    CUtensorMap q, k, v, g;
+    const int* cu;
+    int n_seqs, heads, kv_heads, group, causal;
+    long long tokens;
+    float c, scale;                        // scale * log2(e), scale
+    const float *lse, *delta;              // [heads, tokens]
+    const float* top;                      // float16: max |do|, max |v|
+    void *dq, *dk, *dv;
+    unsigned int* err;
+};
+
+// Power of two on dS and exponent on P.
+template <typename T>
+__device__ __forceinline__ float ds_factor(const float* top, int hd) {
+    if (!std::is_same<T, __half>::value) return 1.f;
+    const float b = 2.f * hd * top[0] * top[1];
+    if (!(b > 0.f) || b > 1e30f) return 1.f;
+    int e;
+    frexpf(b, &e);                         // b <= 2^e
+    return ldexpf(1.f, min(max(15 - e, -100), 100));
+}
+template <typename T> constexpr int p_shift() { return std::is_same<T, __half>::value ? 10 : 0; }
+
+template <int HD>
+struct Shape {
+    static constexpr int SW = HD * 2 < 128 ? HD * 2 : 128;
+    static constexpr int BOXES = HD * 2 / SW;
+    static constexpr int BOX = kTile * SW;
+    static constexpr int TILE = BOXES * BOX;
+    static constexpr int A = 3, B = 2;     // ring of Q (dk/dv) or K (dq), ring of dO or V
+    static constexpr int STAT = (2 + A + B) * TILE;
+    static constexpr int BARS = STAT + 4 * kTile * 4;
+    static constexpr int SMEM = BARS + 256;
+};
+static_assert(Shape<128>::SMEM <= 227 * 1024, "shared memory");
+
+template <int HD>
+__device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* m, int head, int row, uint64_t* bar) {
+    using Sh = Shape<HD>;
+#pragma unroll
+    for (int b = 0; b < Sh::BOXES; ++b) load_3d(dst + b * Sh::BOX, m, b * (Sh::SW / 2), head, row, bar);
+}
+
+// Rows [r0, 128) of a tile become zeros, by one warp.
+template <int HD>
+__device__ __forceinline__ void zero_rows(uint8_t* tile, int r0) {
+    using Sh = Shape<HD>;
+    const int n = (kTile - r0) * (Sh::SW / 16), lane = threadIdx.x & 31;
+    for (int e = lane; e < n * Sh::BOXES; e += 32)
+        *reinterpret_cast<uint4*>(tile + (e / n) * Sh::BOX + r0 * Sh::SW + (e % n) * 16) = make_uint4(0, 0, 0, 0);
+}
+
+// D (+)= A B^T over HD, both tiles row-major in shared memory.
+template <typename T, int HD>
+__device__ __forceinline__ void mma_rows(uint32_t d, const uint8_t* a, const uint8_t* b) {
+    using Sh = Shape<HD>;
+    constexpr uint32_t instr = instruction<T>(kTile, kTile, false);
+    for (int k = 0; k < HD; k += 16) {
+        const uint32_t off = (k * 2 / Sh::SW) * Sh::BOX + (k * 2) % Sh::SW;
+        mma_ss(d, operand<Sh::SW>(smem(a) + off, 16, 8 * Sh::SW), operand<Sh::SW>(smem(b) + off, 16, 8 * Sh::SW), instr,
+               k > 0);
+    }
+}
+// D (+)= W B, W [128, 128] packed in tensor memory (columns 0-31 and 64-95 of its
+// block), B's rows summed over.
+template <typename T, int HD>
+__device__ __forceinline__ void mma_weights(uint32_t d, uint32_t w, const uint8_t* b, bool add) {
+    using Sh = Shape<HD>;
+    constexpr uint32_t instr = instruction<T>(kTile, HD, true);
+    for (int k = 0; k < kTile; k += 16)
+        mma_ts(d, w + (k < 64 ? k / 2 : 64 + (k - 64) / 2), operand<Sh::SW>(smem(b) + k * Sh::SW, Sh::BOX, 8 * Sh::SW),
+               instr, add || k > 0);
+}
+
+// A row of HD sums, times f, to global memory.
+template <typename T, int HD>
+__device__ __forceinline__ void store_row(uint32_t t, float f, T* dst, bool live, int b0 = 0, int step = 1) {
+#pragma unroll
+    for (int b = 0; b < HD / 32; ++b) {
+        if (b % step != b0) continue;
+        uint32_t o[32];
+        ld32(o, t + 32 * b);
+        wait_ld();
+        if (!live) continue;
+#pragma unroll
+        for (int i = 0; i < 32; i += 8) {
+            uint4 u;
+            u.x = pack2<T>(__uint_as_float(o[i]) * f, __uint_as_float(o[i + 1]) * f);
+            u.y = pack2<T>(__uint_as_float(o[i + 2]) * f, __uint_as_float(o[i + 3]) * f);
+            u.z = pack2<T>(__uint_as_float(o[i + 4]) * f, __uint_as_float(o[i + 5]) * f);
+            u.w = pack2<T>(__uint_as_float(o[i + 6]) * f, __uint_as_float(o[i + 7]) * f);
+            *reinterpret_cast<uint4*>(dst + 32 * b + i) = u;
+        }
+    }
+}
+
+// Rows behind the last sequence: zeros.
+template <typename T, int HD>
+__device__ __forceinline__ void zero_out(T* dst, long long row, int row0, int len) {
+    const int n = min(kTile, len - row0) * (HD / 8);
+    for (int e = threadIdx.x; e < n; e += kThreads)
+        *reinterpret_cast<uint4*>(dst + (row0 + e / (HD / 8)) * row + (e % (HD / 8)) * 8) = make_uint4(0, 0, 0, 0);
+}
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// ── dk, dv ────────────────────────────────────────────────────────────────
+template <typename T, int HD>
+__global__ void __launch_bounds__(kThreads, 1) k_packed_dkv_tc(const __grid_constant__ BwdArgs a) {
+    using Sh = Shape<HD>;
+    constexpr int NA = Sh::A, NB = Sh::B;
+    extern __shared__ __align__(1024) uint8_t sm[];
+    uint8_t *ks = sm, *vs = sm + Sh::TILE, *qr = sm + 2 * Sh::TILE, *gr = qr + NA * Sh::TILE;
+    float* st_lse = reinterpret_cast<float*>(sm + Sh::STAT);       // [2][128]
+    float* st_d = st_lse + 2 * kTile;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(sm + Sh::BARS);
+    uint64_t *kv_full = bars, *q_full = bars + 1, *q_empty = q_full + NA, *g_full = q_empty + NA, *g_empty = g_full + NB,
+             *stat_full = g_empty + NB, *stat_empty = stat_full + 2, *s_ready = stat_empty + 2, *dp_ready = s_ready + 1,
+             *p_ready = dp_ready + 1, *ds_ready = p_ready + 1, *done = ds_ready + 1, *fixed = done + 1;
+    uint32_t* tmem_base = reinterpret_cast<uint32_t*>(fixed + NB);
+    volatile int* gone = reinterpret_cast<volatile int*>(tmem_base + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    const int kvh = blockIdx.x % a.kv_heads;
+    const PackedTile t = packed_tile(a.cu, a.n_seqs, a.tokens, kTile, blockIdx.x / a.kv_heads);
+    if (t.row0 >= t.len) return;
+    const long long out_row = (long long)a.kv_heads * HD;
+    T* dk = static_cast<T*>(a.dk) + (t.start * a.kv_heads + kvh) * HD;
+    T* dv = static_cast<T*>(a.dv) + (t.start * a.kv_heads + kvh) * HD;
+    if (t.seq == a.n_seqs) {
+        zero_out<T, HD>(dk, out_row, t.row0, t.len);
+        zero_out<T, HD>(dv, out_row, t.row0, t.len);
+        return;
+    }
+    const int first = a.causal ? t.row0 / kTile : 0;               // query tiles that see this one
+    const int nq = (t.len + kTile - 1) / kTile - first;
+    const int n = nq * a.group;
+    const bool ragged = t.len % kTile != 0;                        // the last query tile of each head
+
+    if (threadIdx.x == 0) {
+        *gone = 0;
+        bar_init(kv_full, 1);
+        for (int i = 0; i < NA; ++i) { bar_init(q_full + i, 1); bar_init(q_empty + i, 1); }
+        for (int i = 0; i < NB; ++i) { bar_init(g_full + i, 1); bar_init(g_empty + i, 1); }
+        for (int i = 0; i < 2; ++i) { bar_init(stat_full + i, 1); bar_init(stat_empty + i, 256); }
+        bar_init(s_ready, 1); bar_init(dp_ready, 1); bar_init(p_ready, 256); bar_init(ds_ready, 256);
+        bar_init(done, 1);
+        for (int i = 0; i < NB; ++i) bar_init(fixed + i, 1);
+        bar_init_done();
+    }
+    if (warp == 8) tmem_alloc(tmem_base, 512);
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tm = *tmem_base, tS = tm, tP = tm + 128, tV = tm + 256, tK = tm + 384;
+
+    if (warp >= 8) {
+        fewer_registers<kOtherRegs>();
+        if (warp == 9) {
+            auto head_of = [&](int i) { return kvh * a.group + i / nq; };
+            auto row_of = [&](int i) { return (int)t.start + (first + i % nq) * kTile; };
+            if (lane == 0) {
+                bar_expect(kv_full, 2 * Sh::TILE);
+                load_tile<HD>(ks, &a.k, kvh, (int)t.start + t.row0, kv_full);
+                load_tile<HD>(vs, &a.v, kvh, (int)t.start + t.row0, kv_full);
+            }
+            bool ok = true;
+            // Entry i is loaded as soon as its places are free; in a sequence's last
+            // tile the rows behind it are cleared once they have landed: the weights
+            // there are 0, and 0 times another sequence's NaN would not be.
+            for (int i = 0; ok && i < n; ++i) {
+                const int sa = i % NA, sb = i % NB;
+                if (i >= NA) ok = bar_wait(q_empty + sa, (i / NA - 1) & 1, gone);
+                if (ok && i >= NB) ok = bar_wait(g_empty + sb, (i / NB - 1) & 1, gone);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                if (lane == 0) {
+                    bar_expect(q_full + sa, Sh::TILE);
+                    load_tile<HD>(qr + sa * Sh::TILE, &a.q, head_of(i), row_of(i), q_full + sa);
+                    bar_expect(g_full + sb, Sh::TILE);
+                    load_tile<HD>(gr + sb * Sh::TILE, &a.g, head_of(i), row_of(i), g_full + sb);
+                }
+                __syncwarp();
+                if (ragged && i % nq == nq - 1) {
+                    ok = bar_wait(q_full + sa, (i / NA) & 1, gone) && bar_wait(g_full + sb, (i / NB) & 1, gone);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    zero_rows<HD>(qr + sa * Sh::TILE, t.len % kTile);
+                    zero_rows<HD>(gr + sb * Sh::TILE, t.len % kTile);
+                    fence_async_smem();
+                    __syncwarp();
+                }
+                if (lane == 0) bar_arrive(fixed + sb);
+            }
+        } else if (warp == 8) {
+            if (lane == 0) {
+                auto ready = [&](int i) { return bar_wait(fixed + i % NB, (i / NB) & 1, gone); };
+                bool ok = bar_wait(kv_full, 0, gone) && bar_wait(q_full, 0, gone) && ready(0);
+                if (ok) {
+                    mma_rows<T, HD>(tS, ks, qr);
+                    commit(s_ready);
+                    ok = bar_wait(g_full, 0, gone);
+                }
+                if (ok) {
+                    mma_rows<T, HD>(tP, vs, gr);
+                    commit(dp_ready);
+                }
+                for (int i = 0; ok && i < n; ++i) {
+                    const bool more = i + 1 < n;
+                    const int sa = i % NA, sb = i % NB, na = (i + 1) % NA, nb = (i + 1) % NB;
+                    ok = bar_wait(p_ready, i & 1, gone);
+                    if (!ok) break;
+                    fence_after();
+                    mma_weights<T, HD>(tV, tS, gr + sb * Sh::TILE, i > 0);
+                    commit(g_empty + sb);
+                    if (more) {
+                        ok = bar_wait(q_full + na, ((i + 1) / NA) & 1, gone) && ready(i + 1);
+                        if (!ok) break;
+                        mma_rows<T, HD>(tS, ks, qr + na * Sh::TILE);
+                        commit(s_ready);
+                    }
+                    ok = bar_wait(ds_ready, i & 1, gone);
+                    if (!ok) break;
+                    fence_after();
+                    mma_weights<T, HD>(tK, tP, qr + sa * Sh::TILE, i > 0);
+                    commit(q_empty + sa);
+                    if (more) {
+                        ok = bar_wait(g_full + nb, ((i + 1) / NB) & 1, gone);
+                        if (!ok) break;
+                        mma_rows<T, HD>(tP, vs, gr + nb * Sh::TILE);
+                        commit(dp_ready);
+                    }
+                }
+                if (ok) commit(done);
+            }
+            __syncwarp();
+        } else if (warp == 10) {
+            // Row statistics of each query tile; a row behind the sequence has weight exp2(-inf).
+            const float gf = ds_factor<T>(a.top, HD) * (1.f / (1 << p_shift<T>()));
+            for (int i = 0; i < n; ++i) {
+                const int sl = i & 1;
+                const bool ok = i < 2 || bar_wait(stat_empty + sl, (i / 2 - 1) & 1, gone);
+                if (!__all_sync(0xffffffffu, ok)) break;
+                const long long at = (long long)(kvh * a.group + i / nq) * a.tokens + t.start;
+                for (int r = lane; r < kTile; r += 32) {
+                    const int row = (first + i % nq) * kTile + r;
+                    float x = INFINITY, d = 0.f;
+                    if (row < t.len) {
+                        x = a.lse[at + row];
+                        x = x == -INFINITY ? INFINITY : x * kLog2e - p_shift<T>();
+                        d = a.delta[at + row] * gf;
+                    }
+                    st_lse[sl * kTile + r] = x;
+                    st_d[sl * kTile + r] = d;
+                }
+                __syncwarp();
+                if (lane == 0) bar_arrive(stat_full + sl);
+            }
+        }
+    } else {
+        more_registers<kMathRegs>();
+        const int half = warp >> 2, row = t.row0 + (warp & 3) * 32 + lane;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t s0 = tS + lanes + 64 * half, p0 = tP + lanes + 64 * half;
+        const float gf = ds_factor<T>(a.top, HD) * (1.f / (1 << p_shift<T>()));
+        bool ok = true;
+        for (int i = 0; i < n; ++i) {
+            const int sl = i & 1;
+            ok = bar_wait(stat_full + sl, (i / 2) & 1, gone) && bar_wait(s_ready, i & 1, gone);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            fence_after();
+            const bool diag = a.causal && i % nq == 0;
+            const int see = diag ? row - t.row0 - 64 * half : -1;          // columns from here on see this key
+            const float* lse = st_lse + sl * kTile + 64 * half;
+            const float* dd = st_d + sl * kTile + 64 * half;
+            float p[64];
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                uint32_t s[32], w[16];
+                ld32(s, s0 + 32 * b);
+                wait_ld();
+#pragma unroll
+                for (int x = 0; x < 32; x += 4) {
+                    const float4 m = *reinterpret_cast<const float4*>(lse + 32 * b + x);
+                    p[32 * b + x] = exp2_fast(fmaf(__uint_as_float(s[x]), a.c, -m.x));
+                    p[32 * b + x + 1] = exp2_fast(fmaf(__uint_as_float(s[x + 1]), a.c, -m.y));
+                    p[32 * b + x + 2] = exp2_fast(fmaf(__uint_as_float(s[x + 2]), a.c, -m.z));
+                    p[32 * b + x + 3] = exp2_fast(fmaf(__uint_as_float(s[x + 3]), a.c, -m.w));
+                }
+                if (diag) {
+#pragma unroll
+                    for (int x = 0; x < 32; ++x)
+                        if (32 * b + x < see) p[32 * b + x] = 0.f;
+                }
+#pragma unroll
+                for (int x = 0; x < 16; ++x) w[x] = pack2<T>(p[32 * b + 2 * x], p[32 * b + 2 * x + 1]);
+                st16(s0 + 16 * b, w);
+            }
+            wait_st();
+            fence_before();
+            bar_arrive(p_ready);
+            ok = bar_wait(dp_ready, i & 1, gone);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            fence_after();
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                uint32_t s[32], w[16];
+                ld32(s, p0 + 32 * b);
+                wait_ld();
+#pragma unroll
+                for (int x = 0; x < 32; x += 4) {
+                    const float4 m = *reinterpret_cast<const float4*>(dd + 32 * b + x);
+                    float e[4] = {fmaf(__uint_as_float(s[x]), gf, -m.x), fmaf(__uint_as_float(s[x + 1]), gf, -m.y),
+                                  fmaf(__uint_as_float(s[x + 2]), gf, -m.z), fmaf(__uint_as_float(s[x + 3]), gf, -m.w)};
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) e[y] = 32 * b + x + y < see ? 0.f : e[y] * p[32 * b + x + y];
+                    w[x / 2] = pack2<T>(e[0], e[1]);
+                    w[x / 2 + 1] = pack2<T>(e[2], e[3]);
+                }
+                st16(p0 + 16 * b, w);
+            }
+            wait_st();
+            fence_before();
+            bar_arrive(ds_ready);
+            bar_arrive(stat_empty + sl);
+        }
+        if (ok) ok = bar_wait(done, 0, gone);
+        if (__all_sync(0xffffffffu, ok)) {
+            fence_after();
+            const bool live = row < t.len;
+            if (half == 0) store_row<T, HD>(tV + lanes, 1.f / (1 << p_shift<T>()), dv + row * out_row, live);
+            else store_row<T, HD>(tK + lanes, a.scale / ds_factor<T>(a.top, HD), dk + row * out_row, live);
+        }
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    if (warp == 8) tmem_free(tm, 512);
+    if (threadIdx.x == 0 && *gone) atomicOr(a.err, kErrTcWait);
+}
+
+// ── dq ────────────────────────────────────────────────────────────────────
+// S has two blocks of columns, so that S(j+2) can follow dQ(j), whose weights
+// dS(j) lie in S(j)'s; the order is dP(j+1), dQ(j), S(j+2).
+template <typename T, int HD>
+__global__ void __launch_bounds__(kThreads, 1) k_packed_dq_tc(const __grid_constant__ BwdArgs a) {
+    using Sh = Shape<HD>;
+    constexpr int NA = Sh::A, NB = Sh::B;
+    extern __shared__ __align__(1024) uint8_t sm[];
+    uint8_t *qs = sm, *gs = sm + Sh::TILE, *kr = sm + 2 * Sh::TILE, *vr = kr + NA * Sh::TILE;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(sm + Sh::BARS);
+    uint64_t *qg_full = bars, *k_full = bars + 1, *k_empty = k_full + NA, *v_full = k_empty + NA, *v_empty = v_full + NB,
+             *s_ready = v_empty + NB, *dp_ready = s_ready + 2, *ds_ready = dp_ready + 1, *done = ds_ready + 1,
+             *fixed = done + 1;
+    uint32_t* tmem_base = reinterpret_cast<uint32_t*>(fixed + 1);
+    volatile int* gone = reinterpret_cast<volatile int*>(tmem_base + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    const int head = blockIdx.x % a.heads, kvh = head / a.group;
+    const PackedTile t = packed_tile(a.cu, a.n_seqs, a.tokens, kTile, (gridDim.x - 1 - blockIdx.x) / a.heads);
+    if (t.row0 >= t.len) return;
+    const long long out_row = (long long)a.heads * HD;
+    T* dq = static_cast<T*>(a.dq) + (t.start * a.heads + head) * HD;
+    if (t.seq == a.n_seqs) {
+        zero_out<T, HD>(dq, out_row, t.row0, t.len);
+        return;
+    }
+    const int last = a.causal ? min(t.row0 + kTile, t.len) : t.len;
+    const int n = (last + kTile - 1) / kTile;
+    const bool ragged = n * kTile > t.len;
+
+    if (threadIdx.x == 0) {
+        *gone = 0;
+        bar_init(qg_full, 1);
+        for (int i = 0; i < NA; ++i) { bar_init(k_full + i, 1); bar_init(k_empty + i, 1); }
+        for (int i = 0; i < NB; ++i) { bar_init(v_full + i, 1); bar_init(v_empty + i, 1); }
+        bar_init(s_ready, 1); bar_init(s_ready + 1, 1); bar_init(dp_ready, 1); bar_init(ds_ready, 256);
+        bar_init(done, 1); bar_init(fixed, 1);
+        bar_init_done();
+    }
+    if (warp == 8) tmem_alloc(tmem_base, 512);
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tm = *tmem_base, tS = tm, tP = tm + 256, tQ = tm + 384;
+
+    if (warp >= 8) {
+        fewer_registers<kOtherRegs>();
+        if (warp == 9) {
+            if (lane == 0) {
+                const int r0 = (int)t.start;
+                bar_expect(qg_full, 2 * Sh::TILE);
+                load_tile<HD>(qs, &a.q, head, r0 + t.row0, qg_full);
+                load_tile<HD>(gs, &a.g, head, r0 + t.row0, qg_full);
+                for (int j = 0; j < n; ++j) {
+                    const int sa = j % NA, sb = j % NB;
+                    if (j >= NA && !bar_wait(k_empty + sa, (j / NA - 1) & 1, gone)) break;
+                    bar_expect(k_full + sa, Sh::TILE);
+                    load_tile<HD>(kr + sa * Sh::TILE, &a.k, kvh, r0 + j * kTile, k_full + sa);
+                    if (j >= NB && !bar_wait(v_empty + sb, (j / NB - 1) & 1, gone)) break;
+                    bar_expect(v_full + sb, Sh::TILE);
+                    load_tile<HD>(vr + sb * Sh::TILE, &a.v, kvh, r0 + j * kTile, v_full + sb);
+                }
+            }
+            __syncwarp();
+            if (ragged) {                   // keys behind the sequence: their dS is 0, 0 times NaN would not be
+                const int j = n - 1;
+                if (bar_wait(k_full + j % NA, (j / NA) & 1, gone)) {
+                    zero_rows<HD>(kr + (j % NA) * Sh::TILE, t.len - j * kTile);
+                    fence_async_smem();
+                }
+                __syncwarp();
+                if (lane == 0) bar_arrive(fixed);
+            }
+        } else if (warp == 8) {
+            if (lane == 0) {
+                auto scores = [&](int j) {
+                    if (!bar_wait(k_full + j % NA, (j / NA) & 1, gone)) return false;
+                    if (ragged && j == n - 1 && !bar_wait(fixed, 0, gone)) return false;
+                    mma_rows<T, HD>(tS + 128 * (j & 1), qs, kr + (j % NA) * Sh::TILE);
+                    commit(s_ready + (j & 1));
+                    return true;
+                };
+                auto dps = [&](int j) {
+                    if (!bar_wait(v_full + j % NB, (j / NB) & 1, gone)) return false;
+                    mma_rows<T, HD>(tP, gs, vr + (j % NB) * Sh::TILE);
+                    commit(dp_ready);
+                    commit(v_empty + j % NB);
+                    return true;
+                };
+                bool ok = bar_wait(qg_full, 0, gone) && scores(0) && dps(0);
+                if (ok && n > 1) ok = scores(1);
+                for (int j = 0; ok && j < n; ++j) {
+                    ok = bar_wait(ds_ready, j & 1, gone);
+                    if (!ok) break;
+                    fence_after();
+                    if (j + 1 < n) ok = dps(j + 1);
+                    if (!ok) break;
+                    mma_weights<T, HD>(tQ, tS + 128 * (j & 1), kr + (j % NA) * Sh::TILE, j > 0);
+                    commit(k_empty + j % NA);
+                    if (j + 2 < n) ok = scores(j + 2);
+                }
+                if (ok) commit(done);
+            }
+            __syncwarp();
+        }
+    } else {
+        more_registers<kMathRegs>();
+        const int half = warp >> 2, row = t.row0 + (warp & 3) * 32 + lane;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t p0 = tP + lanes + 64 * half;
+        const float gf = ds_factor<T>(a.top, HD);
+        float lse = INFINITY, d = 0.f;
+        if (row < t.len) {
+            const long long at = (long long)head * a.tokens + t.start + row;
+            lse = a.lse[at];
+            lse = lse == -INFINITY ? INFINITY : lse * kLog2e;
+            d = a.delta[at] * gf;
+        }
+        bool ok = true;
+        for (int j = 0; j < n; ++j) {
+            const uint32_t s0 = tS + lanes + 128 * (j & 1) + 64 * half;
+            ok = bar_wait(s_ready + (j & 1), (j / 2) & 1, gone);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            fence_after();
+            const int lim = min(t.len, a.causal ? row + 1 : t.len) - j * kTile - 64 * half;   // columns below are seen
+            float p[64];
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                uint32_t s[32];
+                ld32(s, s0 + 32 * b);
+                wait_ld();
+#pragma unroll
+                for (int x = 0; x < 32; ++x) p[32 * b + x] = exp2_fast(fmaf(__uint_as_float(s[x]), a.c, -lse));
+            }
+            ok = bar_wait(dp_ready, j & 1, gone);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            fence_after();
+            const bool part = __any_sync(0xffffffffu, lim < 64);
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                uint32_t s[32], w[16];
+                ld32(s, p0 + 32 * b);
+                wait_ld();
+#pragma unroll
+                for (int x = 0; x < 32; ++x) p[32 * b + x] *= fmaf(__uint_as_float(s[x]), gf, -d);
+                if (part) {
+#pragma unroll
+                    for (int x = 0; x < 32; ++x)
+                        if (32 * b + x >= lim) p[32 * b + x] = 0.f;
+                }
+#pragma unroll
+                for (int x = 0; x < 16; ++x) w[x] = pack2<T>(p[32 * b + 2 * x], p[32 * b + 2 * x + 1]);
+                st16(s0 + 16 * b, w);
+            }
+            wait_st();
+            fence_before();
+            bar_arrive(ds_ready);
+        }
+        if (ok) ok = bar_wait(done, 0, gone);
+        if (__all_sync(0xffffffffu, ok)) {
+            fence_after();
+            store_row<T, HD>(tQ + lanes, a.scale / gf, dq + row * out_row, row < t.len, half, 2);
+        }
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    if (warp == 8) tmem_free(tm, 512);
+    if (threadIdx.x == 0 && *gone) atomicOr(a.err, kErrTcWait);
+}
+
+// D = do . o of each (token, head), HD / 8 lanes a row; float16: the largest |do|
+// and |v| of the sequences' rows (blocks of y = 1 read v).
+template <typename T, int HD>
+__global__ void __launch_bounds__(256) k_packed_delta16(const PackedParams p, float* __restrict__ delta,
+                                                        float* __restrict__ top) {
+    constexpr int L = HD / 8;
+    const bool is_v = blockIdx.y;
+    const int heads = is_v ? p.kv_heads : p.heads;
+    const long long r = ((long long)blockIdx.x * 256 + threadIdx.x) / L;
+    const int lane = threadIdx.x % L;
+    float m = 0.f, s = 0.f;
+    const long long used = packed_cu(p.cu, p.n_seqs, p.tokens);
+    const bool live = r < used * heads;
+    if (live) {
+        const Rows& x = is_v ? p.v : p.dout;
+        const T* row = static_cast<const T*>(x.p) + (r / heads) * x.row + (r % heads) * x.head;
+        const uint4 gu = *reinterpret_cast<const uint4*>(row + lane * 8);
+        const T* ge = reinterpret_cast<const T*>(&gu);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(to_f32(ge[i])));
+        if (!is_v) {
+            const uint4 ou = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.out_in) + r * HD + lane * 8);
+            const T* oe = reinterpret_cast<const T*>(&ou);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s = fmaf(to_f32(ge[i]), to_f32(oe[i]), s);
+        }
+    }
+#pragma unroll
+    for (int off = L / 2; off; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+    if (live && !is_v && lane == 0) delta[(r % heads) * p.tokens + r / heads] = s;
+    if (std::is_same<T, __half>::value) {
+#pragma unroll
+        for (int off = 16; off; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+        if ((threadIdx.x & 31) == 0 && m > 0.f) atomicMax(reinterpret_cast<int*>(top + is_v), __float_as_int(m));
+    }
+}
+
+template <typename T, int HD>
+int launch_bwd(const BwdArgs& a, const PackedParams& p, cudaStream_t s) {
+    using Sh = Shape<HD>;
+    const bool f16 = std::is_same<T, __half>::value;
+    float* top = const_cast<float*>(a.top);
+    if (f16 && cudaMemsetAsync(top, 0, 2 * sizeof(float), s) != cudaSuccess) return kErrCuda;
+    const long long lanes = a.tokens * a.heads * (HD / 8);
+    k_packed_delta16<T, HD><<<dim3((unsigned)((lanes + 255) / 256), f16 ? 2 : 1), 256, 0, s>>>(
+        p, const_cast<float*>(a.delta), top);
+    if (cudaGetLastError() != cudaSuccess) return kErrCuda;
+    const unsigned slots = (unsigned)packed_slots(a.tokens, a.n_seqs, kTile);
+    if (cudaFuncSetAttribute(k_packed_dkv_tc<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::SMEM) != cudaSuccess ||
+        cudaFuncSetAttribute(k_packed_dq_tc<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::SMEM) != cudaSuccess)
+        return kErrCuda;
+    k_packed_dkv_tc<T, HD><<<slots * a.kv_heads, kThreads, Sh::SMEM, s>>>(a);
+    if (cudaGetLastError() != cudaSuccess) return kErrCuda;
+    k_packed_dq_tc<T, HD><<<slots * a.heads, kThreads, Sh::SMEM, s>>>(a);
+    return cudaGetLastError() == cudaSuccess ? kOk : kErrCuda;
+}
+
+template <typename T>
+int bwd_by_dim(const BwdArgs& a, const PackedParams& p, cudaStream_t s) {
+    switch (p.head_dim) {
+        case 32: return launch_bwd<T, 32>(a, p, s);
+        case 64: return launch_bwd<T, 64>(a, p, s);
+        default: return launch_bwd<T, 128>(a, p, s);
+    }
+}
+
+}  // namespace
+
+// Workspace: D [heads, tokens], then the two largest values.
+int attention_packed_backward_tc(const PackedParams& p, cudaStream_t s) {
+    BwdArgs a{};
+    if (!rows_map(&a.q, p.q, p.type, p.tokens, p.heads, p.head_dim) ||
+        !rows_map(&a.k, p.k, p.type, p.tokens, p.kv_heads, p.head_dim) ||
+        !rows_map(&a.v, p.v, p.type, p.tokens, p.kv_heads, p.head_dim) ||
+        !rows_map(&a.g, p.dout, p.type, p.tokens, p.heads, p.head_dim))
+        return kErrUnsupported;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) { cudaGetLastError(); return kErrCuda; }
+    a.cu = p.cu; a.n_seqs = p.n_seqs; a.heads = p.heads; a.kv_heads = p.kv_heads; a.group = p.heads / p.kv_heads;
+    a.causal = p.causal; a.tokens = p.tokens;
+    a.c = p.scale == 0.f ? 1e-30f : p.scale * kLog2e;
+    a.scale = p.scale;
+    a.lse = p.lse_in;
+    a.delta = static_cast<float*>(p.ws);
+    a.top = a.delta + p.tokens * p.heads;
+    a.dq = p.dq; a.dk = p.dk; a.dv = p.dv;
+    a.err = device_error_word(dev);
+    if (!a.err) return kErrCuda;
+    return p.type == kBF16 ? bwd_by_dim<__nv_bfloat16>(a, p, s) : bwd_by_dim<__half>(a, p, s);
+}
+
+}  // namespace racb

@@ -52,8 +52,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_packed_fwd_tc(const __grid_cons
     uint8_t* ring = base + 2 * Sh::TILE;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-    const int head = blockIdx.x, kvh = head / a.group;
-    const PackedTile t = packed_tile(a.cu, a.n_seqs, a.tokens, 2 * kRows, (long long)gridDim.y - 1 - blockIdx.y);
+    const int head = blockIdx.x % a.heads, kvh = head / a.group;
+    const PackedTile t = packed_tile(a.cu, a.n_seqs, a.tokens, 2 * kRows, (gridDim.x - 1 - blockIdx.x) / a.heads);
     if (t.row0 >= t.len) return;
     T* out = static_cast<T*>(a.out) + (t.start * a.heads + head) * HD;
     const long long out_row = (long long)a.heads * HD;
@@ -284,23 +284,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_packed_fwd_tc(const __grid_cons
     if (threadIdx.x == 0 && gone) atomicOr(a.err, kErrTcWait);
 }
 
-// Rows of heads as a [tokens, heads, head_dim] tensor map with boxes of 128 rows of one head.
-bool rows_map(CUtensorMap* m, const Rows& r, int type, long long tokens, int heads, int hd) {
-    const int e = elem_bytes(type), sw = hd * e < 128 ? hd * e : 128;
-    const uint64_t dims[3] = {(uint64_t)hd, (uint64_t)heads, (uint64_t)tokens};
-    // An axis of one place is never stepped along.
-    const uint64_t strides[2] = {(uint64_t)(heads > 1 ? r.head : hd) * e, (uint64_t)(tokens > 1 ? r.row : (long long)heads * hd) * e};
-    const uint32_t box[3] = {(uint32_t)(sw / e), 1, (uint32_t)kRows};
-    return encode_tensor(m, type == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, r.p,
-                         dims, strides, box, sw);
-}
-
 template <typename T, int HD>
 int launch_fwd(const FwdArgs& a, cudaStream_t s) {
     if (cudaFuncSetAttribute(k_packed_fwd_tc<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<HD>::SMEM) !=
         cudaSuccess)
         return kErrCuda;
-    const dim3 grid(a.heads, (unsigned)packed_slots(a.tokens, a.n_seqs, 2 * kRows));
+    const unsigned grid = (unsigned)(packed_slots(a.tokens, a.n_seqs, 2 * kRows) * a.heads);
     k_packed_fwd_tc<T, HD><<<grid, kThreads, Shape<HD>::SMEM, s>>>(a);
     return cudaGetLastError() == cudaSuccess ? kOk : kErrCuda;
 }
@@ -315,6 +304,17 @@ int fwd_by_dim(const FwdArgs& a, int hd, cudaStream_t s) {
 }
 
 }  // namespace
+
+// Rows of heads as a [tokens, heads, head_dim] tensor map with boxes of 128 rows of one head.
+bool rows_map(CUtensorMap* m, const Rows& r, int type, long long tokens, int heads, int hd) {
+    const int e = elem_bytes(type), sw = hd * e < 128 ? hd * e : 128;
+    const uint64_t dims[3] = {(uint64_t)hd, (uint64_t)heads, (uint64_t)tokens};
+    // An axis of one place is never stepped along.
+    const uint64_t strides[2] = {(uint64_t)(heads > 1 ? r.head : hd) * e, (uint64_t)(tokens > 1 ? r.row : (long long)heads * hd) * e};
+    const uint32_t box[3] = {(uint32_t)(sw / e), 1, (uint32_t)kRows};
+    return encode_tensor(m, type == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, r.p,
+                         dims, strides, box, sw);
+}
 
 int attention_packed_tc(const PackedParams& p, cudaStream_t s) {
     FwdArgs a{};

@@ -2,6 +2,7 @@
 // attention and of the cache's page operations.  All take device pointers,
 // enqueue on `s`, never synchronise and return a racb::Status.
 #pragma once
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 namespace racb {
@@ -36,7 +37,10 @@ struct PackedParams {
 
 size_t attention_packed_workspace(long long tokens, int n_seqs, int heads, int kv_heads, int head_dim, int type,
                                   int backward);
-int attention_packed_tc(const PackedParams& p, cudaStream_t s);      // float16, bfloat16: arguments checked
+// float16 and bfloat16, arguments checked.
+int attention_packed_tc(const PackedParams& p, cudaStream_t s);
+int attention_packed_backward_tc(const PackedParams& p, cudaStream_t s);
+bool rows_map(CUtensorMap* m, const Rows& r, int type, long long tokens, int heads, int hd);
 int attention_packed(const PackedParams& p, cudaStream_t s);
 int attention_packed_backward(const PackedParams& p, cudaStream_t s);
 

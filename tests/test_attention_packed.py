@@ -192,6 +192,17 @@ def test_differentiable(cuda):
 
 
 @gpu
+@pytest.mark.parametrize("dt", [F32, F16, BF16])
+def test_backward_from_autograd(cuda, dt):
+    """The engine calls the backward from a thread of its own, which may have used no GPU before."""
+    q, k, v, go, cu = make([140, 33], 8, 2, 128, dt, cuda, seed=9)
+    leaves = [x.detach().requires_grad_(True) for x in (q, k, v)]
+    got = torch.autograd.grad(R.rac_attention_packed(*leaves, cu, True, 0.1), leaves, go)
+    want = run_all(q, k, v, go, cu, True, 0.1)
+    assert all(torch.equal(a, want[n]) for a, n in zip(got, ("dq", "dk", "dv")))
+
+
+@gpu
 def test_capture_and_another_stream(cuda):
     """Captured forward and backward replay on new inputs, two graphs that were captured one after the other
     do not disturb each other; a side stream gives the same bits."""
