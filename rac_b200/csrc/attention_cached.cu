@@ -89,7 +89,22 @@ int by_dim(const CachedParams& p, unsigned int* err, cudaStream_t s) {
 
 }  // namespace
 
-size_t attention_cached_workspace(int, int, int, int, int) { return 0; }
+// Blocks of the tensor-core kernel: one an SM.
+static int block_count() {
+    static int per_dev[64] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { cudaGetLastError(); return 0; }
+    if (per_dev[dev] == 0) {
+        int n = 0;
+        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) { cudaGetLastError(); return 0; }
+        per_dev[dev] = n;
+    }
+    return per_dev[dev];
+}
+
+size_t attention_cached_workspace(int, int nodes, int heads, int kv_heads, int head_dim) {
+    return attention_cached_tc_workspace(block_count(), nodes, heads, kv_heads, head_dim);
+}
 
 int attention_cached(const CachedParams& p, cudaStream_t s) {
     if (p.batch < 0 || p.nodes < 0 || p.heads <= 0 || p.kv_heads <= 0 || p.heads % p.kv_heads || p.nodes > 64 ||
@@ -104,14 +119,20 @@ int attention_cached(const CachedParams& p, cudaStream_t s) {
         if (st * e % 16) return kErrUnsupported;
     for (const void* x : {p.q, (const void*)p.k.p, (const void*)p.v.p, (const void*)p.out})
         if (reinterpret_cast<uintptr_t>(x) & 15u) return kErrUnsupported;
+    if ((long long)p.batch * p.kv_heads * ((long long)p.nodes * (p.heads / p.kv_heads)) >= (1LL << 31)) return kErrInvalidDim;
+    if (p.type != kF32) {
+        const int blocks = block_count();
+        if (blocks == 0) return kErrCuda;
+        if (!p.ws || p.ws_bytes < attention_cached_tc_workspace(blocks, p.nodes, p.heads, p.kv_heads, p.head_dim))
+            return kErrAlloc;
+        return attention_cached_tc(p, blocks, s);
+    }
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) { cudaGetLastError(); return kErrCuda; }
     unsigned int* err = device_error_word(dev);
     if (!err) return kErrCuda;
     switch (p.type) {
         case kF32: return by_dim<float>(p, err, s);
-        case kF16: return by_dim<__half>(p, err, s);
-        case kBF16: return by_dim<__nv_bfloat16>(p, err, s);
         default: return kErrUnsupported;
     }
 }

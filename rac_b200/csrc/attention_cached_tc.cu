@@ -1,0 +1,680 @@
+// attention_cached_tc.cu -- attention of new tokens over a paged cache on the
+// tensor cores, float16 and bfloat16.
+//
+// The rows of one product are the new rows of a sequence times the query heads
+// of one key/value head: 4 for a single token with a group of 4, up to 256 for
+// a tree, in one or two tiles of 128 (rows that do not exist cost matrix time,
+// but the cache's bytes bound this kernel: 128 keys are 64 KB at dim 128, some
+// 2800 cycles of an SM's share of HBM, against 1024 of a tile's two products).
+// Up to 32 (64) rows stand in the tile four times (twice), and each copy weighs
+// a quarter (half) of a tile's keys: the four warps that read a tile's lanes
+// share its softmax, which one warp alone would take 3000 cycles for.
+// Keys and values come through the page table by 16-byte asynchronous copies,
+// four warps of them, into a ring; hidden rows and bad pages become zeros on
+// the way, and their scores are masked by bits that the loading warps note.
+//
+// Work is split by keys, not by sequences: all tiles of all (sequence, head)
+// units stand in one line, cut into as many equal pieces as there are blocks,
+// so that caches of any lengths keep every SM busy.  Each block reads the
+// lengths and finds its piece; the host need not know them.  A unit that lies
+// in one piece is finished there; of one that is cut each piece leaves its
+// normalised sum and the logarithm of its weight, and a second kernel joins
+// them (its launch overlaps the first).
+#include "attn_common.cuh"
+#include "tensor_core.cuh"
+
+namespace racb {
+namespace {
+
+using namespace tc;
+
+constexpr int kKeys = 128;                 // keys of a tile
+constexpr int kRowTile = 128, kUnitRows = 256;
+// Warps 0-3, 4-7: softmax of row tile 0, 1; 8-11: loads; 12: matrix instructions; 13-15 fill the warpgroup.
+constexpr int kThreads = 512;
+constexpr int kLaunchRegs = 128, kMathRegs = 160, kLoadRegs = 104, kOtherRegs = 88;
+static_assert(kMathRegs * 256 + kLoadRegs * 128 + kOtherRegs * 128 <= kLaunchRegs * kThreads, "register split");
+constexpr int kInfo = 8;                   // tiles of key masks in flight
+
+struct Args {
+    CachedParams p;
+    float c;                               // scale * log2(e)
+    int rows, row_units, unit_rows;        // rows of a (sequence, kv head); units they make; rows of a unit
+    int copies;                            // of the rows in a tile: 4 up to 32 rows, 2 up to 64, 1
+    float *part, *part_lse;                // [2 * blocks, unit_rows, dim], [2 * blocks, unit_rows]
+    unsigned int* err;
+};
+
+template <int HD>
+struct Shape {
+    static constexpr int SW = HD * 2 < 128 ? HD * 2 : 128;
+    static constexpr int BOXES = HD * 2 / SW;
+    static constexpr int BOX = kKeys * SW;
+    static constexpr int TILE = BOXES * BOX;
+    static constexpr int STAGES = HD == 128 ? 4 : HD == 64 ? 8 : 12;
+    static constexpr int RING = 2 * TILE, OFFS = RING + STAGES * TILE;
+    static constexpr int OKS = OFFS + 2 * 2 * kKeys * 8, BARS = OKS + kInfo * 16;
+    static constexpr int WALK = BARS + 512, JOIN = WALK + 128;      // JOIN: [128][33] floats, then [128] float2
+    static constexpr int SMEM = JOIN + kRowTile * 33 * 4 + kRowTile * 8;
+    static constexpr int CH = HD / 8;                               // 16-byte units of a row
+};
+static_assert(Shape<128>::SMEM <= 227 * 1024, "shared memory");
+
+// Byte offset of 16-byte unit c of row r in a swizzled tile.
+template <int HD>
+__device__ __forceinline__ uint32_t place(int r, int c) {
+    using Sh = Shape<HD>;
+    constexpr int U = Sh::SW / 16;
+    const int sw = U == 8 ? r & 7 : (r >> 1) & 3;
+    return (c / U) * Sh::BOX + r * Sh::SW + (((c % U) ^ sw) << 4);
+}
+
+__device__ __forceinline__ int rows_in_cache(const CachedParams& p, int b) {
+    const long long cap = min((long long)p.table_width * p.page_size, 0x7fff0000LL);
+    const long long n = p.lengths[b];
+    return (int)(n < 0 ? 0 : (n > cap ? cap : n));
+}
+__device__ __forceinline__ int new_rows(const CachedParams& p, int b) {
+    return p.counts ? max(0, min(p.counts[b], p.nodes)) : p.nodes;
+}
+// Key tiles of a sequence: one at least, which writes the zeros of an empty one.
+__device__ __forceinline__ int tiles_of(const CachedParams& p, int b) {
+    return max(1, (rows_in_cache(p, b) + kKeys - 1) / kKeys);
+}
+
+// The piece of the line of tiles that a block works on, as segments of one unit each.
+struct Walk {
+    long long pos, end, at;                // at: position of sequence b's first tile
+    int b;
+};
+struct Segment {
+    int b, kvh, unit, tiles, j0, j1;       // key tiles [j0, j1) of `tiles`
+    long long pos;
+};
+__device__ __forceinline__ bool next(const Args& a, Walk& w, Segment& s) {
+    if (w.pos >= w.end) return false;
+    const long long per = (long long)a.p.kv_heads * a.row_units;
+    int n = tiles_of(a.p, w.b);
+    while (w.pos >= w.at + n * per) {
+        w.at += n * per;
+        ++w.b;
+        n = tiles_of(a.p, w.b);
+    }
+    const long long rel = w.pos - w.at, u = rel / n;
+    s.b = w.b;
+    s.kvh = (int)(u / a.row_units);
+    s.unit = (int)(u % a.row_units);
+    s.tiles = n;
+    s.j0 = (int)(rel % n);
+    s.j1 = (int)min((long long)n, s.j0 + w.end - w.pos);
+    s.pos = w.pos;
+    w.pos += s.j1 - s.j0;
+    return true;
+}
+
+// Sum over b < limit of the key tiles, by one warp.
+__device__ __forceinline__ long long tiles_before(const CachedParams& p, int limit) {
+    long long n = 0;
+    for (int b = threadIdx.x & 31; b < limit; b += 32) n += tiles_of(p, b);
+#pragma unroll
+    for (int off = 16; off; off >>= 1) n += __shfl_xor_sync(0xffffffffu, n, off);
+    return n;
+}
+
+// Block `blk` of n works on positions [total blk / n, total (blk + 1) / n), n the
+// blocks launched or, where that is less, the tiles there are: no piece is empty.
+__device__ __forceinline__ Walk piece(const Args& a, int blk, int blocks) {
+    const long long per = (long long)a.p.kv_heads * a.row_units, total = tiles_before(a.p, a.p.batch) * per;
+    const long long n_pieces = min((long long)blocks, total);
+    Walk w;
+    w.pos = blk < n_pieces ? total * blk / n_pieces : total;
+    w.end = blk < n_pieces ? total * (blk + 1) / n_pieces : total;
+    w.at = 0;
+    w.b = 0;
+    const int lane = threadIdx.x & 31;
+    for (int b0 = 0; b0 < a.p.batch && w.pos < w.end; b0 += 32) {
+        long long n = b0 + lane < a.p.batch ? tiles_of(a.p, b0 + lane) * per : 0;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const long long x = __shfl_up_sync(0xffffffffu, n, off);
+            if (lane >= off) n += x;
+        }
+        // n: end of sequence b0 + lane, counted from w.at
+        const unsigned past = __ballot_sync(0xffffffffu, w.at + n > w.pos);
+        if (past) {
+            const int l = __ffs(past) - 1;
+            const long long before = __shfl_sync(0xffffffffu, n, l ? l - 1 : 0);
+            w.at += l ? before : 0;
+            w.b = b0 + l;
+            break;
+        }
+        w.at += __shfl_sync(0xffffffffu, n, 31);
+    }
+    return w;
+}
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool live) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+// The barrier gets this thread's arrival once its copies so far have landed.
+__device__ __forceinline__ void copies_arrive(uint64_t* bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" :: "r"(smem(bar)) : "memory");
+}
+// A barrier of 128 threads that gives up like every other wait.
+__device__ __forceinline__ bool group_sync(uint64_t* bar, uint32_t& phase, volatile int* gone) {
+    bar_arrive(bar);
+    const bool ok = bar_wait(bar, phase & 1, gone);
+    ++phase;
+    return __all_sync(0xffffffffu, ok);
+}
+
+// Scores of 32 keys (columns at ts + 32 b of the thread's row); `see`: which are visible.
+__device__ __forceinline__ void load_scores(uint32_t (&v)[32], uint32_t ts, int b, bool part, uint32_t see, bool neg) {
+    ld32(v, ts + 32 * b);
+    wait_ld();
+    if (part) {
+        const uint32_t hide = neg ? 0x7f800000u : 0xff800000u;
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+            if (!(see >> i & 1)) v[i] = hide;
+    }
+}
+// The largest score times c, whatever c's sign.
+__device__ __forceinline__ float largest(const uint32_t (&v)[32], bool neg) {
+    float z[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) z[i] = __uint_as_float(v[i]);
+    if (neg) {
+#pragma unroll
+        for (int i = 4; i < 32; ++i) z[i & 3] = fminf(z[i & 3], __uint_as_float(v[i]));
+        return fminf(fminf(z[0], z[1]), fminf(z[2], z[3]));
+    }
+#pragma unroll
+    for (int i = 4; i < 32; ++i) z[i & 3] = fmaxf(z[i & 3], __uint_as_float(v[i]));
+    return fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3]));
+}
+// Weights exp2(c s - ref) of 32 keys, packed to ts + 16 b; returns their sum.
+template <typename T>
+__device__ __forceinline__ float put_weights(const uint32_t (&v)[32], uint32_t ts, int b, float c, float ref) {
+    uint32_t q[16];
+    float add[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const float e0 = exp2_fast(fmaf(__uint_as_float(v[2 * i]), c, -ref));
+        const float e1 = exp2_fast(fmaf(__uint_as_float(v[2 * i + 1]), c, -ref));
+        add[i & 3] += e0 + e1;
+        q[i] = pack2<T>(e0, e1);
+    }
+    st16(ts + 16 * b, q);
+    return (add[0] + add[1]) + (add[2] + add[3]);
+}
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(kThreads, 1) k_cached_tc(const __grid_constant__ Args a) {
+    using Sh = Shape<HD>;
+    constexpr int ST = Sh::STAGES;
+    extern __shared__ __align__(1024) uint8_t sm[];
+    uint8_t *qs = sm, *ring = sm + Sh::RING;
+    long long* offs = reinterpret_cast<long long*>(sm + Sh::OFFS);         // [2][k, v][128]
+    uint32_t* oks = reinterpret_cast<uint32_t*>(sm + Sh::OKS);             // [kInfo][4]
+    uint64_t* bars = reinterpret_cast<uint64_t*>(sm + Sh::BARS);
+    uint64_t *full = bars, *empty = full + ST, *info = empty + ST, *q_full = info + kInfo, *q_empty = q_full + 2,
+             *s_ready = q_empty + 2, *p_ready = s_ready + 2, *o_ready = p_ready + 2, *pv_done = o_ready + 2,
+             *load_sync = pv_done + 1, *math_sync = load_sync + 1;
+    uint32_t* tmem_base = reinterpret_cast<uint32_t*>(math_sync + 1);
+    volatile int* gone = reinterpret_cast<volatile int*>(tmem_base + 1);
+    Walk* walk = reinterpret_cast<Walk*>(sm + Sh::WALK);
+    float* join = reinterpret_cast<float*>(sm + Sh::JOIN);
+    float2* join_ml = reinterpret_cast<float2*>(join + kRowTile * 33);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const CachedParams& p = a.p;
+
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (threadIdx.x == 0) {
+        *gone = 0;
+        for (int i = 0; i < ST; ++i) { bar_init(full + i, 128); bar_init(empty + i, 1); }
+        for (int i = 0; i < kInfo; ++i) bar_init(info + i, 4);
+        for (int i = 0; i < 2; ++i) {
+            bar_init(q_full + i, 128); bar_init(q_empty + i, 1); bar_init(s_ready + i, 1); bar_init(p_ready + i, 128);
+            bar_init(o_ready + i, 1);
+        }
+        bar_init(pv_done, 1);
+        bar_init(load_sync, 128);
+        bar_init(math_sync, 128);
+        bar_init_done();
+    }
+    if (warp == 12) tmem_alloc(tmem_base, 512);
+    if (warp == 8) {
+        const Walk w = piece(a, blockIdx.x, gridDim.x);
+        if (lane == 0) *walk = w;
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tm = *tmem_base, tS = tm, tO = tm + 256;
+    Walk w = *walk;
+    Segment s;
+    // Two row tiles: each has a block of S columns and they take turns.  One: it
+    // has both blocks, and tile g's scores lie in block g & 1.
+    const int nw = a.unit_rows > kRowTile ? 2 : 1;
+
+    if (warp >= 12) {
+        fewer_registers<kOtherRegs>();
+        if (warp == 12 && lane == 0) {
+            constexpr uint32_t iqk = instruction<T>(kRowTile, kKeys, false), ipv = instruction<T>(kRowTile, HD, true);
+            int g = 0, seg = 0;            // tiles and segments so far
+            bool ok = true;
+            while (ok && next(a, w, s)) {
+                const int n = s.j1 - s.j0, qslot = nw == 1 ? seg & 1 : 0;
+                auto scores = [&](int x, int j) {              // row tile x, key tile j of the segment
+                    const int e = 2 * (g + j), buf = nw == 2 ? x : (g + j) & 1;
+                    if (!bar_wait(full + e % ST, (e / ST) & 1, gone)) return false;
+                    fence_async_smem();        // the copies' writes, for the matrix instructions
+                    product_ss<HD / 16, Sh::SW>(tS + buf * kKeys, smem(qs + (nw == 1 ? qslot : x) * Sh::TILE),
+                                                smem(ring + (e % ST) * Sh::TILE), Sh::BOX, iqk);
+                    commit(s_ready + buf);
+                    if (x == nw - 1) {
+                        commit(empty + e % ST);
+                        if (j == n - 1) commit(q_empty + qslot);
+                    }
+                    return true;
+                };
+                ok = bar_wait(q_full + qslot, (nw == 1 ? seg >> 1 : seg) & 1, gone);
+                if (!ok) break;
+                for (int x = 0; ok && x < nw; ++x) ok = scores(x, 0);
+                if (ok && nw == 1 && n > 1) ok = scores(0, 1);
+                for (int j = 0; ok && j < n; ++j) {
+                    const int e = 2 * (g + j) + 1;
+                    ok = bar_wait(full + e % ST, (e / ST) & 1, gone);
+                    fence_async_smem();
+                    for (int x = 0; ok && x < nw; ++x) {
+                        // Weights of two tiles may be ready before the values of the first have
+                        // landed: a barrier for each block of S columns.
+                        const int buf = nw == 2 ? x : (g + j) & 1;
+                        ok = bar_wait(p_ready + buf, (nw == 2 ? g + j : (g + j) >> 1) & 1, gone);
+                        if (!ok) break;
+                        fence_after();
+                        const uint64_t vb = operand<Sh::SW>(smem(ring + (e % ST) * Sh::TILE), Sh::BOX, 8 * Sh::SW);
+                        const uint32_t pw = tS + buf * kKeys;
+#pragma unroll
+                        for (int k = 0; k < kKeys; k += 16)
+                            mma_ts(tO + x * 128, pw + k / 2, vb + (k * Sh::SW >> 4), ipv, j > 0 || k > 0);
+                        if (nw == 1) commit(pv_done);
+                        if (x == nw - 1) commit(empty + e % ST);
+                        if (j == n - 1) commit(o_ready + x);
+                        else if (nw == 2) ok = scores(x, j + 1);
+                        else if (j + 2 < n) ok = scores(0, j + 2);
+                    }
+                }
+                g += n;
+                ++seg;
+            }
+        }
+        __syncwarp();
+    } else if (warp >= 8) {
+        fewer_registers<kLoadRegs>();
+        const int tid = threadIdx.x - 256;
+        const char *kp = static_cast<const char*>(p.k.p), *vp = static_cast<const char*>(p.v.p);
+        // A thread copies unit c of rows row0, row0 + STEP, ...; STEP is a multiple of 8,
+        // so that the swizzle is the same for all of them.
+        constexpr int STEP = 128 / Sh::CH, N = kKeys / STEP;
+        static_assert(STEP % 8 == 0, "swizzle");
+        const int c = tid % Sh::CH, row0 = tid / Sh::CH;
+        const uint32_t dst0 = smem(ring) + place<HD>(row0, c);
+        const int group = p.heads / p.kv_heads, span = kRowTile / a.copies;
+        int e = 0, g = 0, seg = 0;                             // ring entries, tiles, segments so far
+        uint32_t syncs = 0;
+        bool ok = true;
+        while (ok && next(a, w, s)) {
+            const int len = rows_in_cache(p, s.b), qslot = nw == 1 ? seg & 1 : 0, use = nw == 1 ? seg >> 1 : seg;
+            if (use > 0) ok = bar_wait(q_empty + qslot, (use - 1) & 1, gone);
+            if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+            const int* table = p.table + (long long)s.b * p.table_width;
+            auto page_of = [&](int j) {
+                const int r = j * kKeys + tid;
+                return r < len ? table[r / p.page_size] : -1;
+            };
+            int page = page_of(s.j0);
+            // Queries: row r of the unit is new row r / group, head r % group of the group.
+            const int r0 = s.unit * kUnitRows;
+#pragma unroll 4
+            for (int x = tid; x < nw * kRowTile * Sh::CH; x += 128) {
+                const int place_row = x / Sh::CH, qc = x % Sh::CH, r = nw == 2 ? place_row : place_row % span;
+                uint4 u = make_uint4(0, 0, 0, 0);
+                if (r < a.unit_rows && r0 + r < a.rows) {
+                    const int node = (r0 + r) / group, h = s.kvh * group + (r0 + r) % group;
+                    u = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + s.b * p.q_batch + node * p.q_node +
+                                                        h * p.q_head + qc * 8);
+                }
+                *reinterpret_cast<uint4*>(qs + ((nw == 1 ? qslot : 0) + place_row / kRowTile) * Sh::TILE +
+                                          place<HD>(place_row % kRowTile, qc)) = u;
+            }
+            fence_async_smem();
+            bar_arrive(q_full + qslot);
+            for (int j = s.j0; j < s.j1; ++j, ++g) {
+                const int r = j * kKeys + tid;
+                const bool live = page >= 0 && page < p.pages;
+                if (!live && r < len) atomicOr(a.err, kErrBadPage);
+                const int slot = r % p.page_size;
+                long long* o = offs + (g & 1) * 2 * kKeys;
+                o[tid] = live ? (page * p.k.page + s.kvh * p.k.head + slot * p.k.row) * (long long)sizeof(T) : -1;
+                o[kKeys + tid] = live ? (page * p.v.page + s.kvh * p.v.head + slot * p.v.row) * (long long)sizeof(T) : -1;
+                const uint32_t bits = __ballot_sync(0xffffffffu, live);
+                if (lane == 0) {
+                    oks[(g % kInfo) * 4 + warp - 8] = bits;
+                    bar_arrive(info + g % kInfo);
+                }
+                if (j + 1 < s.j1) page = page_of(j + 1);
+                ok = group_sync(load_sync, syncs, gone);
+                for (int kv = 0; kv < 2; ++kv, ++e) {
+                    if (e >= ST && ok) ok = bar_wait(empty + e % ST, (e / ST - 1) & 1, gone);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    const uint32_t dst = dst0 + (e % ST) * Sh::TILE;
+                    const char* src = (kv ? vp : kp) + c * 16;
+                    const long long* at = o + kv * kKeys + row0;
+#pragma unroll
+                    for (int i0 = 0; i0 < N; i0 += 8) {
+                        long long x[8];
+#pragma unroll
+                        for (int i = 0; i < 8 && i0 + i < N; ++i) x[i] = at[(i0 + i) * STEP];
+#pragma unroll
+                        for (int i = 0; i < 8 && i0 + i < N; ++i)
+                            copy16(dst + (i0 + i) * STEP * Sh::SW, x[i] < 0 ? static_cast<const char*>(p.q) : src + x[i],
+                                   x[i] >= 0);
+                    }
+                    copies_arrive(full + e % ST);
+                }
+                if (!ok) break;
+            }
+            ++seg;
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+    } else {
+        more_registers<kMathRegs>();
+        const int x = warp >> 2, group = p.heads / p.kv_heads, span = kRowTile / a.copies;
+        const int lane_row = (warp & 3) * 32 + lane, copy = lane_row / span;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, to = tm + lanes + 256 + x * 128;
+        const bool neg = a.c < 0.f;
+        int g = 0, seg = 0;
+        uint32_t syncs = 0;
+        bool ok = true;
+        while (x < nw && ok && next(a, w, s)) {
+            const int n = s.j1 - s.j0;
+            const int ur = x * kRowTile + lane_row % span, r = s.unit * kUnitRows + ur;   // row of the unit, of the head
+            const bool mine = ur < a.unit_rows && r < a.rows;
+            const int cnt = new_rows(p, s.b), len = rows_in_cache(p, s.b), node = r / group;
+            const bool busy = __any_sync(0xffffffffu, mine);                              // else nothing to weigh
+            const int prefix = max(0, len - cnt);
+            unsigned long long sees = 0;
+            if (mine) sees = p.tree ? (unsigned long long)p.tree[(long long)s.b * p.nodes + node] : ~0ull >> (63 - node);
+            if (len - prefix < 64) sees &= (1ull << (len - prefix)) - 1;
+            float m = -INFINITY, l = 0.f;
+            for (int j = 0; j < n; ++j) {
+                const int t = g + j, buf = nw == 2 ? x : t & 1;
+                ok = bar_wait(s_ready + buf, (nw == 2 ? t : t >> 1) & 1, gone) &&
+                     bar_wait(info + t % kInfo, (t / kInfo) & 1, gone);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                fence_after();
+                if (busy) {
+                    const uint32_t ts = tm + lanes + buf * kKeys;
+                    const uint32_t* in = oks + (t % kInfo) * 4;
+                    const int pre = prefix - (s.j0 + j) * kKeys;       // keys of the prefix in this tile
+                    const bool part = pre < kKeys || (in[0] & in[1] & in[2] & in[3]) != 0xffffffffu;
+                    // Visible: keys below pre, then the row's own mask, whose bit 0 stands at `at`.
+                    auto visible = [&](int b) {
+                        const int at = pre - 32 * b;
+                        uint32_t see = 0;
+                        if (at >= 32) see = 0xffffffffu;
+                        else if (at >= 0) see = (uint32_t)(sees << at) | ((1u << at) - 1);
+                        else if (at > -64) see = (uint32_t)(sees >> -at);
+                        return see & in[b];
+                    };
+                    // The reference point moves only when a weight would pass 2^8.
+                    auto move = [&](float top) {
+                        if (j == 0) {
+                            m = top;
+                        } else if (__any_sync(0xffffffffu, top > m + 8.f)) {
+                            const float up = top > m + 8.f ? exp2_fast(m - top) : 1.f;
+                            if (top > m + 8.f) m = top;
+                            l *= up;
+                            if (nw == 1) { // the last product may still run; with two tiles S has waited for it
+                                ok = __all_sync(0xffffffffu, bar_wait(pv_done, (t - 1) & 1, gone));
+                                fence_after();
+                            }
+#pragma unroll
+                            for (int b = 0; b < HD / 32; ++b) {
+                                uint32_t o[32];
+                                ld32(o, to + 32 * b);
+                                wait_ld();
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * up);
+                                st32(to + 32 * b, o);
+                            }
+                        }
+                        return m == -INFINITY ? 0.f : m;
+                    };
+                    const uint32_t none[16] = {};
+                    if (a.copies == 4) {               // this copy's 32 keys; the others weigh the rest
+                        uint32_t v[32];
+                        load_scores(v, ts, copy, part, visible(copy), neg);
+                        const float ref = move(largest(v, neg) * a.c);
+#pragma unroll
+                        for (int b = 0; b < 4; ++b)
+                            if (b != copy) st16(ts + 16 * b, none);
+                        l += put_weights<T>(v, ts, copy, a.c, ref);
+                    } else if (a.copies == 2) {
+                        uint32_t v[2][32];
+                        const int b0 = 2 * copy;
+                        load_scores(v[0], ts, b0, part, visible(b0), neg);
+                        load_scores(v[1], ts, b0 + 1, part, visible(b0 + 1), neg);
+                        const float y0 = largest(v[0], neg), y1 = largest(v[1], neg);
+                        const float ref = move((neg ? fminf(y0, y1) : fmaxf(y0, y1)) * a.c);
+                        st16(ts + 32 - 16 * b0, none);
+                        st16(ts + 48 - 16 * b0, none);
+                        l += put_weights<T>(v[0], ts, b0, a.c, ref);
+                        l += put_weights<T>(v[1], ts, b0 + 1, a.c, ref);
+                    } else {
+                        // Read twice rather than held: the registers of 128 would not fit.
+                        float y = neg ? INFINITY : -INFINITY;
+#pragma unroll
+                        for (int b = 0; b < 4; ++b) {
+                            uint32_t v[32];
+                            load_scores(v, ts, b, part, visible(b), neg);
+                            const float z = largest(v, neg);
+                            y = neg ? fminf(y, z) : fmaxf(y, z);
+                        }
+                        const float ref = move(y * a.c);
+#pragma unroll
+                        for (int b = 0; b < 4; ++b) {
+                            uint32_t v[32];
+                            load_scores(v, ts, b, part, visible(b), neg);
+                            l += put_weights<T>(v, ts, b, a.c, ref);     // over scores that have been read
+                        }
+                    }
+                    if (!ok) break;
+                    wait_st();
+                }
+                fence_before();
+                bar_arrive(p_ready + buf);
+            }
+            if (ok) ok = __all_sync(0xffffffffu, bar_wait(o_ready + x, seg & 1, gone));
+            if (!ok) break;
+            fence_after();
+            const bool whole = n == s.tiles, live = mine && node < cnt;
+            const long long piece_at = 2LL * blockIdx.x + (s.pos == walk->pos ? 0 : 1);
+            T* out = static_cast<T*>(p.out) +
+                     (((long long)s.b * p.nodes + node) * p.heads + s.kvh * group + r % group) * HD;
+            float* part = a.part + (piece_at * a.unit_rows + ur) * HD;
+            // Eight sums of the row, normalised: to the output where the unit is whole.
+            auto store8 = [&](int at, const float (&f)[8]) {
+                if (whole) {
+                    uint4 u;
+                    uint32_t* uu = reinterpret_cast<uint32_t*>(&u);
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) uu[y] = live ? pack2<T>(f[2 * y], f[2 * y + 1]) : 0u;
+                    if (mine && (live || p.zero_rest)) *reinterpret_cast<uint4*>(out + at) = u;
+                } else if (live) {
+                    *reinterpret_cast<float4*>(part + at) = make_float4(f[0], f[1], f[2], f[3]);
+                    *reinterpret_cast<float4*>(part + at + 4) = make_float4(f[4], f[5], f[6], f[7]);
+                }
+            };
+            if (a.copies > 1) {
+                // The copies' sums of a row become one: each with its own reference point.
+                join_ml[lane_row] = make_float2(m, l);
+                ok = group_sync(math_sync, syncs, gone);
+                float M = -INFINITY, L = 0.f;
+                for (int i = 0; i < a.copies; ++i) M = fmaxf(M, join_ml[i * span + lane_row % span].x);
+                for (int i = 0; i < a.copies; ++i) {
+                    const float2 y = join_ml[i * span + lane_row % span];
+                    L += y.x == -INFINITY ? 0.f : y.y * exp2_fast(y.x - M);
+                }
+                const float f = m == -INFINITY ? 0.f : exp2_fast(m - M), inv = L == 0.f ? 0.f : 1.f / L;
+                for (int b = 0; ok && b < HD / 32; ++b) {
+                    uint32_t o[32];
+                    ld32(o, to + 32 * b);
+                    wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) join[lane_row * 33 + i] = f == 0.f ? 0.f : __uint_as_float(o[i]) * f;
+                    ok = group_sync(math_sync, syncs, gone);
+                    if (!ok) break;
+                    for (int i0 = copy * (32 / a.copies); i0 < (copy + 1) * (32 / a.copies); i0 += 8) {
+                        float y[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            y[i] = 0.f;
+                            for (int k = 0; k < a.copies; ++k) y[i] += join[(k * span + lane_row % span) * 33 + i0 + i];
+                            y[i] *= inv;
+                        }
+                        store8(32 * b + i0, y);
+                    }
+                    ok = group_sync(math_sync, syncs, gone);
+                }
+                if (!ok) break;
+                if (!whole && live && copy == 0)
+                    a.part_lse[piece_at * a.unit_rows + ur] = L == 0.f ? -INFINITY : M + log2f(L);
+            } else if (busy) {
+                const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+                for (int b = 0; b < HD / 32; ++b) {
+                    uint32_t o[32];
+                    ld32(o, to + 32 * b);
+                    wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8) {
+                        float y[8];
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) y[k] = inv == 0.f ? 0.f : __uint_as_float(o[i + k]) * inv;
+                        store8(32 * b + i, y);
+                    }
+                }
+                if (!whole && live) a.part_lse[piece_at * a.unit_rows + ur] = l == 0.f ? -INFINITY : m + log2f(l);
+            }
+            g += n;
+            ++seg;
+        }
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    if (warp == 12) tmem_free(tm, 512);
+    if (threadIdx.x == 0 && *gone) atomicOr(a.err, kErrTcWait);
+}
+
+// Joins the pieces of cut units: a block a unit, a warp a row.
+template <typename T, int HD>
+__global__ void __launch_bounds__(256) k_cached_join(const __grid_constant__ Args a, int launched) {
+    const CachedParams& p = a.p;
+    const long long per = (long long)p.kv_heads * a.row_units;
+    const int b = (int)(blockIdx.x / per), u = (int)(blockIdx.x % per);
+    const int kvh = u / a.row_units, unit = u % a.row_units, group = p.heads / p.kv_heads;
+    const long long total = tiles_before(p, p.batch) * per;
+    const int n = tiles_of(p, b);
+    const long long blocks = min((long long)launched, total);
+    const long long t0 = tiles_before(p, b) * per + (long long)u * n;
+    const long long c0 = ((t0 + 1) * blocks - 1) / total, c1 = ((t0 + n) * blocks - 1) / total;
+    const int cnt = new_rows(p, b), lane = threadIdx.x & 31;
+    const long long s0 = 2 * c0 + (total * c0 / blocks == t0 ? 0 : 1);     // the first piece's place
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (c0 == c1) return;
+    for (int ur = threadIdx.x >> 5; ur < a.unit_rows; ur += 8) {
+        const int r = unit * kUnitRows + ur, node = r / group;
+        if (r >= a.rows || (node >= cnt && !p.zero_rest)) continue;
+        float acc[HD / 32], w = 0.f;
+#pragma unroll
+        for (int i = 0; i < HD / 32; ++i) acc[i] = 0.f;
+        if (node < cnt) {
+            float m = -INFINITY;
+            for (long long c = c0; c <= c1; ++c)
+                m = fmaxf(m, a.part_lse[(c == c0 ? s0 : 2 * c) * a.unit_rows + ur]);
+            if (m != -INFINITY)
+                for (long long c = c0; c <= c1; ++c) {
+                    const long long at = (c == c0 ? s0 : 2 * c) * a.unit_rows + ur;
+                    const float f = exp2_fast(a.part_lse[at] - m);
+                    w += f;
+#pragma unroll
+                    for (int i = 0; i < HD / 32; ++i) acc[i] = fmaf(f, a.part[at * HD + i * 32 + lane], acc[i]);
+                }
+        }
+        T* out = static_cast<T*>(p.out) + (((long long)b * p.nodes + node) * p.heads + kvh * group + r % group) * HD;
+        const float f = w == 0.f ? 0.f : 1.f / w;
+#pragma unroll
+        for (int i = 0; i < HD / 32; ++i) out[i * 32 + lane] = from_f32<T>(acc[i] * f);
+    }
+}
+
+template <typename T, int HD>
+int launch(const Args& a, int blocks, cudaStream_t s) {
+    if (cudaFuncSetAttribute(k_cached_tc<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<HD>::SMEM) != cudaSuccess)
+        return kErrCuda;
+    k_cached_tc<T, HD><<<blocks, kThreads, Shape<HD>::SMEM, s>>>(a);
+    if (cudaGetLastError() != cudaSuccess) return kErrCuda;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)((long long)a.p.batch * a.p.kv_heads * a.row_units));
+    cfg.blockDim = dim3(256);
+    cfg.stream = s;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, k_cached_join<T, HD>, a, blocks) == cudaSuccess ? kOk : kErrCuda;
+}
+
+template <typename T>
+int by_dim(const Args& a, int blocks, cudaStream_t s) {
+    switch (a.p.head_dim) {
+        case 32: return launch<T, 32>(a, blocks, s);
+        case 64: return launch<T, 64>(a, blocks, s);
+        default: return launch<T, 128>(a, blocks, s);
+    }
+}
+
+}  // namespace
+
+// Two pieces a block.
+size_t attention_cached_tc_workspace(int blocks, int nodes, int heads, int kv_heads, int head_dim) {
+    const long long rows = (long long)nodes * (heads / kv_heads);
+    return (size_t)2 * blocks * (rows < kUnitRows ? rows : kUnitRows) * (head_dim + 1) * sizeof(float);
+}
+
+int attention_cached_tc(const CachedParams& p, int blocks, cudaStream_t s) {
+    Args a{};
+    a.p = p;
+    // 0 would turn a hidden score's infinity into NaN; 1e-30 weighs the rest alike.
+    a.c = p.scale == 0.f ? 1e-30f : p.scale * 1.4426950408889634f;
+    a.rows = p.nodes * (p.heads / p.kv_heads);
+    a.row_units = (a.rows + kUnitRows - 1) / kUnitRows;
+    a.unit_rows = a.rows < kUnitRows ? a.rows : kUnitRows;
+    a.copies = a.unit_rows <= 32 ? 4 : a.unit_rows <= 64 ? 2 : 1;
+    a.part = static_cast<float*>(p.ws);
+    a.part_lse = a.part + (size_t)2 * blocks * a.unit_rows * p.head_dim;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) { cudaGetLastError(); return kErrCuda; }
+    a.err = device_error_word(dev);
+    if (!a.err) return kErrCuda;
+    return p.type == kBF16 ? by_dim<__nv_bfloat16>(a, blocks, s) : by_dim<__half>(a, blocks, s);
+}
+
+}  // namespace racb

@@ -69,6 +69,9 @@ struct CachedParams {
 };
 
 size_t attention_cached_workspace(int batch, int nodes, int heads, int kv_heads, int head_dim);
+// float16 and bfloat16 on `blocks` blocks, arguments checked.
+size_t attention_cached_tc_workspace(int blocks, int nodes, int heads, int kv_heads, int head_dim);
+int attention_cached_tc(const CachedParams& p, int blocks, cudaStream_t s);
 int attention_cached(const CachedParams& p, cudaStream_t s);
 
 struct AppendParams {

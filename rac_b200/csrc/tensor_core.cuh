@@ -152,6 +152,20 @@ __device__ __forceinline__ void commit(uint64_t* bar) {
 template <int N> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(N)); }
 template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(N)); }
 
+// Sums over a contiguous axis: D (+)= A B^T over 16 * STEPS summed values, both
+// operands K-major in boxes of rows of SW bytes (box: bytes of one).  The
+// addresses of the steps are constants apart, so that one thread issues a step
+// in a few cycles.
+template <int STEPS, int SW>
+__device__ __forceinline__ void product_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t box, uint32_t instr) {
+    const uint64_t da = operand<SW>(a, 16, 8 * SW), db = operand<SW>(b, 16, 8 * SW);
+#pragma unroll
+    for (int k = 0; k < STEPS; ++k) {
+        const uint32_t off = ((k * 32 / SW) * box + (k * 32) % SW) >> 4;
+        mma_ss(d, da + off, db + off, instr, k > 0);
+    }
+}
+
 // ── values ────────────────────────────────────────────────────────────────
 template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
 template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {

@@ -51,7 +51,7 @@ SHAPES = [  # lengths, nodes, heads, kv_heads, dim, page
     ([1], 1, 1, 1, 64, 16), ([300], 1, 32, 32, 128, 16), ([17, 0, 513, 64], 1, 8, 2, 128, 64),
     ([100, 7], 7, 4, 1, 32, 24), ([13, 200, 64, 1000], 13, 6, 2, 64, 8), ([64, 400], 64, 8, 2, 128, 64),
     ([65, 129, 511], 33, 4, 4, 64, 1), ([2000], 1, 16, 1, 128, 128), ([1500, 3], 3, 12, 4, 128, 100),
-    ([5] * 50, 1, 4, 2, 64, 16), ([4096], 48, 4, 1, 64, 256)]
+    ([5] * 50, 1, 4, 2, 64, 16), ([4096], 48, 4, 1, 64, 256), ([3000 + 700 * i for i in range(6)], 1, 16, 8, 32, 48)]
 
 
 @gpu
