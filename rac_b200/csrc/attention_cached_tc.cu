@@ -54,8 +54,8 @@ struct Shape {
     static constexpr int STAGES = HD == 128 ? 4 : HD == 64 ? 8 : 12;
     static constexpr int RING = 2 * TILE, OFFS = RING + STAGES * TILE;
     static constexpr int OKS = OFFS + 2 * 2 * kKeys * 8, BARS = OKS + kInfo * 16;
-    static constexpr int WALK = BARS + 512, JOIN = WALK + 128;      // JOIN: [128][33] floats, then [128] float2
-    static constexpr int SMEM = JOIN + kRowTile * 33 * 4 + kRowTile * 8;
+    static constexpr int WALK = BARS + 512, JOIN = WALK + 128;      // JOIN, twice: [128][17] floats, [128] float2
+    static constexpr int JOIN1 = kRowTile * 17 * 4 + kRowTile * 8, SMEM = JOIN + 2 * JOIN1;
     static constexpr int CH = HD / 8;                               // 16-byte units of a row
 };
 static_assert(Shape<128>::SMEM <= 227 * 1024, "shared memory");
@@ -220,12 +220,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_cached_tc(const __grid_constant
     uint64_t* bars = reinterpret_cast<uint64_t*>(sm + Sh::BARS);
     uint64_t *full = bars, *empty = full + ST, *info = empty + ST, *q_full = info + kInfo, *q_empty = q_full + 2,
              *s_ready = q_empty + 2, *p_ready = s_ready + 2, *o_ready = p_ready + 2, *pv_done = o_ready + 2,
-             *load_sync = pv_done + 1, *math_sync = load_sync + 1;
-    uint32_t* tmem_base = reinterpret_cast<uint32_t*>(math_sync + 1);
+             *load_sync = pv_done + 1, *math_sync = load_sync + 1;   // math_sync: two
+    uint32_t* tmem_base = reinterpret_cast<uint32_t*>(math_sync + 2);
     volatile int* gone = reinterpret_cast<volatile int*>(tmem_base + 1);
     Walk* walk = reinterpret_cast<Walk*>(sm + Sh::WALK);
-    float* join = reinterpret_cast<float*>(sm + Sh::JOIN);
-    float2* join_ml = reinterpret_cast<float2*>(join + kRowTile * 33);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const CachedParams& p = a.p;
 
@@ -241,6 +239,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_cached_tc(const __grid_constant
         bar_init(pv_done, 1);
         bar_init(load_sync, 128);
         bar_init(math_sync, 128);
+        bar_init(math_sync + 1, 128);
         bar_init_done();
     }
     if (warp == 12) tmem_alloc(tmem_base, 512);
@@ -263,8 +262,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_cached_tc(const __grid_constant
         if (warp == 12 && lane == 0) {
             constexpr uint32_t iqk = instruction<T>(kRowTile, kKeys, false), ipv = instruction<T>(kRowTile, HD, true);
             int g = 0, seg = 0;            // tiles and segments so far
-            bool ok = true;
-            while (ok && next(a, w, s)) {
+            bool ok = true, more = next(a, w, s);
+            Segment later = s;
+            while (ok && more) {
                 const int n = s.j1 - s.j0, qslot = nw == 1 ? seg & 1 : 0;
                 auto scores = [&](int x, int j) {              // row tile x, key tile j of the segment
                     const int e = 2 * (g + j), buf = nw == 2 ? x : (g + j) & 1;
@@ -298,16 +298,18 @@ __global__ void __launch_bounds__(kThreads, 1) k_cached_tc(const __grid_constant
                         const uint32_t pw = tS + buf * kKeys;
 #pragma unroll
                         for (int k = 0; k < kKeys; k += 16)
-                            mma_ts(tO + x * 128, pw + k / 2, vb + (k * Sh::SW >> 4), ipv, j > 0 || k > 0);
+                            mma_ts(tO + (nw == 2 ? x : seg & 1) * 128, pw + k / 2, vb + (k * Sh::SW >> 4), ipv, j > 0 || k > 0);
                         if (nw == 1) commit(pv_done);
                         if (x == nw - 1) commit(empty + e % ST);
-                        if (j == n - 1) commit(o_ready + x);
+                        if (j == n - 1) commit(o_ready + (nw == 2 ? x : seg & 1));
                         else if (nw == 2) ok = scores(x, j + 1);
                         else if (j + 2 < n) ok = scores(0, j + 2);
                     }
+                    if (j == 0) more = next(a, w, later);
                 }
                 g += n;
                 ++seg;
+                s = later;
             }
         }
         __syncwarp();
@@ -322,35 +324,39 @@ __global__ void __launch_bounds__(kThreads, 1) k_cached_tc(const __grid_constant
         const int c = tid % Sh::CH, row0 = tid / Sh::CH;
         const uint32_t dst0 = smem(ring) + place<HD>(row0, c);
         const int group = p.heads / p.kv_heads, span = kRowTile / a.copies;
+        const float per_group = 1.f / group;
         int e = 0, g = 0, seg = 0;                             // ring entries, tiles, segments so far
         uint32_t syncs = 0;
-        bool ok = true;
-        while (ok && next(a, w, s)) {
+        bool ok = true, more = next(a, w, s);
+        // The next segment and its first page are looked up while the first tile of
+        // this one is under way: each lookup is a trip to memory that is busy.
+        Segment later = s;
+        int later_page = -1;
+        auto page_of = [&](const Segment& x, int j) {
+            const int r = j * kKeys + tid;
+            return r < rows_in_cache(p, x.b) ? p.table[(long long)x.b * p.table_width + r / p.page_size] : -1;
+        };
+        int page = more ? page_of(s, s.j0) : -1;
+        while (ok && more) {
             const int len = rows_in_cache(p, s.b), qslot = nw == 1 ? seg & 1 : 0, use = nw == 1 ? seg >> 1 : seg;
             if (use > 0) ok = bar_wait(q_empty + qslot, (use - 1) & 1, gone);
             if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-            const int* table = p.table + (long long)s.b * p.table_width;
-            auto page_of = [&](int j) {
-                const int r = j * kKeys + tid;
-                return r < len ? table[r / p.page_size] : -1;
-            };
-            int page = page_of(s.j0);
             // Queries: row r of the unit is new row r / group, head r % group of the group.
             const int r0 = s.unit * kUnitRows;
+            const uint32_t qdst = smem(qs) + (nw == 1 ? qslot : 0) * Sh::TILE + place<HD>(row0, c);
+            const T* q = static_cast<const T*>(p.q) + s.b * p.q_batch + s.kvh * group * p.q_head + c * 8;
+            for (int x = 0; x < nw; ++x) {
 #pragma unroll 4
-            for (int x = tid; x < nw * kRowTile * Sh::CH; x += 128) {
-                const int place_row = x / Sh::CH, qc = x % Sh::CH, r = nw == 2 ? place_row : place_row % span;
-                uint4 u = make_uint4(0, 0, 0, 0);
-                if (r < a.unit_rows && r0 + r < a.rows) {
-                    const int node = (r0 + r) / group, h = s.kvh * group + (r0 + r) % group;
-                    u = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + s.b * p.q_batch + node * p.q_node +
-                                                        h * p.q_head + qc * 8);
+                for (int i = 0; i < N; ++i) {
+                    const int pr = row0 + i * STEP, r = nw == 2 ? x * kRowTile + pr : pr & (span - 1);
+                    const bool live = r < a.unit_rows && r0 + r < a.rows;
+                    // (r0 + r) / group: a half is further from every quotient than float rounding reaches.
+                    const int node = (int)((r0 + r + 0.5f) * per_group), h = (r0 + r) - node * group;
+                    copy16(qdst + x * Sh::TILE + i * STEP * Sh::SW, live ? q + node * p.q_node + h * p.q_head : static_cast<const T*>(p.q),
+                           live);
                 }
-                *reinterpret_cast<uint4*>(qs + ((nw == 1 ? qslot : 0) + place_row / kRowTile) * Sh::TILE +
-                                          place<HD>(place_row % kRowTile, qc)) = u;
             }
-            fence_async_smem();
-            bar_arrive(q_full + qslot);
+            copies_arrive(q_full + qslot);
             for (int j = s.j0; j < s.j1; ++j, ++g) {
                 const int r = j * kKeys + tid;
                 const bool live = page >= 0 && page < p.pages;
@@ -364,7 +370,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_cached_tc(const __grid_constant
                     oks[(g % kInfo) * 4 + warp - 8] = bits;
                     bar_arrive(info + g % kInfo);
                 }
-                if (j + 1 < s.j1) page = page_of(j + 1);
+                if (j + 1 < s.j1) page = page_of(s, j + 1);
                 ok = group_sync(load_sync, syncs, gone);
                 for (int kv = 0; kv < 2; ++kv, ++e) {
                     if (e >= ST && ok) ok = bar_wait(empty + e % ST, (e / ST - 1) & 1, gone);
@@ -386,22 +392,39 @@ __global__ void __launch_bounds__(kThreads, 1) k_cached_tc(const __grid_constant
                     copies_arrive(full + e % ST);
                 }
                 if (!ok) break;
+                if (j == s.j0) {
+                    more = next(a, w, later);
+                    if (more) later_page = page_of(later, later.j0);
+                }
             }
+            s = later;
+            page = later_page;
             ++seg;
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
     } else {
         more_registers<kMathRegs>();
         const int x = warp >> 2, group = p.heads / p.kv_heads, span = kRowTile / a.copies;
-        const int lane_row = (warp & 3) * 32 + lane, copy = lane_row / span;
-        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, to = tm + lanes + 256 + x * 128;
+        const int lane_row = (warp & 3) * 32 + lane, copy = lane_row / span, row = lane_row & (span - 1);
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        float* join = reinterpret_cast<float*>(sm + Sh::JOIN + x * Sh::JOIN1);
+        float2* join_ml = reinterpret_cast<float2*>(join + kRowTile * 17);
         const bool neg = a.c < 0.f;
         int g = 0, seg = 0;
         uint32_t syncs = 0;
         bool ok = true;
-        while (x < nw && ok && next(a, w, s)) {
+        while (ok && next(a, w, s)) {
             const int n = s.j1 - s.j0;
-            const int ur = x * kRowTile + lane_row % span, r = s.unit * kUnitRows + ur;   // row of the unit, of the head
+            if (nw == 1) {
+                // One row tile: the warpgroups take turns by segment, and one stores its
+                // sums while the other weighs the next segment's scores.
+                if ((seg & 1) != x) { g += n; ++seg; continue; }
+                // Up to here the barriers below have been another's to wait for.
+                if (seg) ok = __all_sync(0xffffffffu, bar_wait(o_ready + ((seg - 1) & 1), ((seg - 1) >> 1) & 1, gone));
+                if (!ok) break;
+            }
+            const uint32_t to = tm + lanes + 256 + x * 128;
+            const int ur = (nw == 2 ? x * kRowTile : 0) + row, r = s.unit * kUnitRows + ur;   // row of the unit, of the head
             const bool mine = ur < a.unit_rows && r < a.rows;
             const int cnt = new_rows(p, s.b), len = rows_in_cache(p, s.b), node = r / group;
             const bool busy = __any_sync(0xffffffffu, mine);                              // else nothing to weigh
@@ -443,7 +466,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_cached_tc(const __grid_constant
                                 ok = __all_sync(0xffffffffu, bar_wait(pv_done, (t - 1) & 1, gone));
                                 fence_after();
                             }
-#pragma unroll
+#pragma unroll 1
                             for (int b = 0; b < HD / 32; ++b) {
                                 uint32_t o[32];
                                 ld32(o, to + 32 * b);
@@ -478,7 +501,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_cached_tc(const __grid_constant
                     } else {
                         // Read twice rather than held: the registers of 128 would not fit.
                         float y = neg ? INFINITY : -INFINITY;
-#pragma unroll
+#pragma unroll 1
                         for (int b = 0; b < 4; ++b) {
                             uint32_t v[32];
                             load_scores(v, ts, b, part, visible(b), neg);
@@ -486,7 +509,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_cached_tc(const __grid_constant
                             y = neg ? fminf(y, z) : fmaxf(y, z);
                         }
                         const float ref = move(y * a.c);
-#pragma unroll
+#pragma unroll 1
                         for (int b = 0; b < 4; ++b) {
                             uint32_t v[32];
                             load_scores(v, ts, b, part, visible(b), neg);
@@ -499,7 +522,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_cached_tc(const __grid_constant
                 fence_before();
                 bar_arrive(p_ready + buf);
             }
-            if (ok) ok = __all_sync(0xffffffffu, bar_wait(o_ready + x, seg & 1, gone));
+            if (ok) ok = __all_sync(0xffffffffu, bar_wait(o_ready + x, (nw == 2 ? seg : seg >> 1) & 1, gone));
             if (!ok) break;
             fence_after();
             const bool whole = n == s.tiles, live = mine && node < cnt;
@@ -507,66 +530,67 @@ __global__ void __launch_bounds__(kThreads, 1) k_cached_tc(const __grid_constant
             T* out = static_cast<T*>(p.out) +
                      (((long long)s.b * p.nodes + node) * p.heads + s.kvh * group + r % group) * HD;
             float* part = a.part + (piece_at * a.unit_rows + ur) * HD;
-            // Eight sums of the row, normalised: to the output where the unit is whole.
-            auto store8 = [&](int at, const float (&f)[8]) {
+            // Four sums of the row, normalised: to the output where the unit is whole.
+            auto store4 = [&](int at, const float (&f)[4]) {
                 if (whole) {
-                    uint4 u;
-                    uint32_t* uu = reinterpret_cast<uint32_t*>(&u);
-#pragma unroll
-                    for (int y = 0; y < 4; ++y) uu[y] = live ? pack2<T>(f[2 * y], f[2 * y + 1]) : 0u;
-                    if (mine && (live || p.zero_rest)) *reinterpret_cast<uint4*>(out + at) = u;
+                    if (mine && (live || p.zero_rest))
+                        *reinterpret_cast<uint2*>(out + at) =
+                            live ? make_uint2(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3])) : make_uint2(0u, 0u);
                 } else if (live) {
                     *reinterpret_cast<float4*>(part + at) = make_float4(f[0], f[1], f[2], f[3]);
-                    *reinterpret_cast<float4*>(part + at + 4) = make_float4(f[4], f[5], f[6], f[7]);
                 }
             };
             if (a.copies > 1) {
                 // The copies' sums of a row become one: each with its own reference point.
                 join_ml[lane_row] = make_float2(m, l);
-                ok = group_sync(math_sync, syncs, gone);
+                ok = group_sync(math_sync + x, syncs, gone);
                 float M = -INFINITY, L = 0.f;
-                for (int i = 0; i < a.copies; ++i) M = fmaxf(M, join_ml[i * span + lane_row % span].x);
-                for (int i = 0; i < a.copies; ++i) {
-                    const float2 y = join_ml[i * span + lane_row % span];
+                for (int i = row; i < kRowTile; i += span) M = fmaxf(M, join_ml[i].x);
+                for (int i = row; i < kRowTile; i += span) {
+                    const float2 y = join_ml[i];
                     L += y.x == -INFINITY ? 0.f : y.y * exp2_fast(y.x - M);
                 }
                 const float f = m == -INFINITY ? 0.f : exp2_fast(m - M), inv = L == 0.f ? 0.f : 1.f / L;
-                for (int b = 0; ok && b < HD / 32; ++b) {
-                    uint32_t o[32];
-                    ld32(o, to + 32 * b);
+                const int most = 16 / a.copies;        // columns that a thread adds up: 4 or 8
+#pragma unroll 1
+                for (int b = 0; b < HD / 16; ++b) {
+                    uint32_t o[16];
+                    ld16(o, to + 16 * b);
                     wait_ld();
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) join[lane_row * 33 + i] = f == 0.f ? 0.f : __uint_as_float(o[i]) * f;
-                    ok = group_sync(math_sync, syncs, gone);
+                    for (int i = 0; i < 16; ++i) join[lane_row * 17 + i] = f == 0.f ? 0.f : __uint_as_float(o[i]) * f;
+                    ok = group_sync(math_sync + x, syncs, gone);
                     if (!ok) break;
-                    for (int i0 = copy * (32 / a.copies); i0 < (copy + 1) * (32 / a.copies); i0 += 8) {
-                        float y[8];
+#pragma unroll 1
+                    for (int i0 = copy * most; i0 < (copy + 1) * most; i0 += 4) {
+                        float y[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+                        for (int k = row; k < kRowTile; k += span)
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            y[i] = 0.f;
-                            for (int k = 0; k < a.copies; ++k) y[i] += join[(k * span + lane_row % span) * 33 + i0 + i];
-                            y[i] *= inv;
-                        }
-                        store8(32 * b + i0, y);
+                            for (int i = 0; i < 4; ++i) y[i] += join[k * 17 + i0 + i];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) y[i] *= inv;
+                        store4(16 * b + i0, y);
                     }
-                    ok = group_sync(math_sync, syncs, gone);
+                    ok = group_sync(math_sync + x, syncs, gone);
+                    if (!ok) break;
                 }
                 if (!ok) break;
                 if (!whole && live && copy == 0)
                     a.part_lse[piece_at * a.unit_rows + ur] = L == 0.f ? -INFINITY : M + log2f(L);
             } else if (busy) {
                 const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
+#pragma unroll 1
                 for (int b = 0; b < HD / 32; ++b) {
                     uint32_t o[32];
                     ld32(o, to + 32 * b);
                     wait_ld();
 #pragma unroll
-                    for (int i = 0; i < 32; i += 8) {
-                        float y[8];
+                    for (int i = 0; i < 32; i += 4) {
+                        float y[4];
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) y[k] = inv == 0.f ? 0.f : __uint_as_float(o[i + k]) * inv;
-                        store8(32 * b + i, y);
+                        for (int k = 0; k < 4; ++k) y[k] = inv == 0.f ? 0.f : __uint_as_float(o[i + k]) * inv;
+                        store4(32 * b + i, y);
                     }
                 }
                 if (!whole && live) a.part_lse[piece_at * a.unit_rows + ur] = l == 0.f ? -INFINITY : m + log2f(l);
@@ -582,12 +606,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_cached_tc(const __grid_constant
     if (threadIdx.x == 0 && *gone) atomicOr(a.err, kErrTcWait);
 }
 
-// Joins the pieces of cut units: a block a unit, a warp a row.
+// Joins the pieces of cut units: a warp a row, eight rows of one unit a block.
 template <typename T, int HD>
 __global__ void __launch_bounds__(256) k_cached_join(const __grid_constant__ Args a, int launched) {
     const CachedParams& p = a.p;
     const long long per = (long long)p.kv_heads * a.row_units;
-    const int b = (int)(blockIdx.x / per), u = (int)(blockIdx.x % per);
+    const int parts = (a.unit_rows + 7) / 8, ur = (int)(blockIdx.x % parts) * 8 + (threadIdx.x >> 5);
+    const long long bu = blockIdx.x / parts;
+    const int b = (int)(bu / per), u = (int)(bu % per);
     const int kvh = u / a.row_units, unit = u % a.row_units, group = p.heads / p.kv_heads;
     const long long total = tiles_before(p, p.batch) * per;
     const int n = tiles_of(p, b);
@@ -598,30 +624,28 @@ __global__ void __launch_bounds__(256) k_cached_join(const __grid_constant__ Arg
     const long long s0 = 2 * c0 + (total * c0 / blocks == t0 ? 0 : 1);     // the first piece's place
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (c0 == c1) return;
-    for (int ur = threadIdx.x >> 5; ur < a.unit_rows; ur += 8) {
-        const int r = unit * kUnitRows + ur, node = r / group;
-        if (r >= a.rows || (node >= cnt && !p.zero_rest)) continue;
-        float acc[HD / 32], w = 0.f;
+    const int r = unit * kUnitRows + ur, node = r / group;
+    if (ur >= a.unit_rows || r >= a.rows || (node >= cnt && !p.zero_rest)) return;
+    float acc[HD / 32], w = 0.f, m = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < HD / 32; ++i) acc[i] = 0.f;
-        if (node < cnt) {
-            float m = -INFINITY;
-            for (long long c = c0; c <= c1; ++c)
-                m = fmaxf(m, a.part_lse[(c == c0 ? s0 : 2 * c) * a.unit_rows + ur]);
-            if (m != -INFINITY)
-                for (long long c = c0; c <= c1; ++c) {
-                    const long long at = (c == c0 ? s0 : 2 * c) * a.unit_rows + ur;
-                    const float f = exp2_fast(a.part_lse[at] - m);
-                    w += f;
+    for (int i = 0; i < HD / 32; ++i) acc[i] = 0.f;
+    if (node < cnt) {
+        // A running reference point: the pieces are read once.
+#pragma unroll 4
+        for (long long c = c0; c <= c1; ++c) {
+            const long long at = (c == c0 ? s0 : 2 * c) * a.unit_rows + ur;
+            const float x = a.part_lse[at], top = fmaxf(m, x), ref = top == -INFINITY ? 0.f : top;
+            const float keep = exp2_fast(m - ref), f = exp2_fast(x - ref);
+            m = top;
+            w = fmaf(w, keep, f);
 #pragma unroll
-                    for (int i = 0; i < HD / 32; ++i) acc[i] = fmaf(f, a.part[at * HD + i * 32 + lane], acc[i]);
-                }
+            for (int i = 0; i < HD / 32; ++i) acc[i] = fmaf(f, a.part[at * HD + i * 32 + lane], acc[i] * keep);
         }
-        T* out = static_cast<T*>(p.out) + (((long long)b * p.nodes + node) * p.heads + kvh * group + r % group) * HD;
-        const float f = w == 0.f ? 0.f : 1.f / w;
-#pragma unroll
-        for (int i = 0; i < HD / 32; ++i) out[i * 32 + lane] = from_f32<T>(acc[i] * f);
     }
+    T* out = static_cast<T*>(p.out) + (((long long)b * p.nodes + node) * p.heads + kvh * group + r % group) * HD;
+    const float f = w == 0.f ? 0.f : 1.f / w;
+#pragma unroll
+    for (int i = 0; i < HD / 32; ++i) out[i * 32 + lane] = from_f32<T>(acc[i] * f);
 }
 
 template <typename T, int HD>
@@ -634,7 +658,7 @@ int launch(const Args& a, int blocks, cudaStream_t s) {
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)((long long)a.p.batch * a.p.kv_heads * a.row_units));
+    cfg.gridDim = dim3((unsigned)((long long)a.p.batch * a.p.kv_heads * a.row_units * ((a.unit_rows + 7) / 8)));
     cfg.blockDim = dim3(256);
     cfg.stream = s;
     cfg.attrs = &attr;
