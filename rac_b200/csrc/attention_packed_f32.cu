@@ -1,0 +1,983 @@
+// attention_packed_f32.cu -- attention over packed prompts in float32, forward
+// and backward, on the float16 tensor cores.
+//
+// A float32 value x is kept as two float16 parts, hi = f16(x f) and lo =
+// f16(x f - hi), 22 bits together; f is a power of two for each head of each
+// tile of 128 rows that puts the tile's largest value between 2^13 and 2^14,
+// so that the error is 2^-22 of a value or 2^-39 of its tile's largest.  A
+// product of two such matrices is lo hi + hi lo + hi hi (lo lo lies below the
+// last bit): three float16 products, a rate of 1647 / 3 = 549 TFLOP/s against
+// the FP32 pipe's 74.
+//
+// The tensor core adds into its 32-bit sums by cutting off (measured: 1e-7 of
+// the sum for each instruction of 16 summed values, all in one direction, so
+// that 1024 of them lose 1e-4).  So a sum in tensor memory is never carried on
+// from one tile of 64 to the next: it is added to 32-bit registers, rounded to
+// nearest, where the tile's factor is applied as well.  Within a product the
+// small parts come first.
+#include "attn_common.cuh"
+#include "tensor_core.cuh"
+
+namespace racb {
+namespace {
+
+using namespace tc;
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kSplit = 128;                // rows that share a factor
+constexpr int kWide = 128, kNarrow = 64;   // rows of the tile that stays and of those that pass by
+
+// ── parts ─────────────────────────────────────────────────────────────────
+struct SplitArgs {
+    Rows in[4];                            // q, k, v, dout
+    int heads[4], first[5];                // heads of each; prefix sums
+    __half* parts[4];                      // [tokens, 2 heads, dim]: hi of each head, then lo
+    float* factors[4];                     // [slots, heads]: 1 / f
+    const float* out;                      // with dout: the forward's output, for D = do . o
+    float* delta;                          // [heads, tokens]
+    const int* cu;
+    int n_seqs;
+    long long tokens;
+};
+
+template <int HD>
+__global__ void __launch_bounds__(256) k_split(const SplitArgs a) {
+    constexpr int L = HD / 4, STEP = 256 / L, N = kSplit / STEP;
+    __shared__ float red[8];
+    int h = blockIdx.x % a.first[4], w = 0;
+    const int slot = blockIdx.x / a.first[4];
+    while (h >= a.first[w + 1]) ++w;
+    h -= a.first[w];
+    const PackedTile t = packed_tile(a.cu, a.n_seqs, a.tokens, kSplit, slot);
+    if (t.row0 >= t.len || t.seq == a.n_seqs) return;
+    const int lane = threadIdx.x % L, row0 = t.row0 + threadIdx.x / L;
+    const float* in = static_cast<const float*>(a.in[w].p) + t.start * a.in[w].row + h * a.in[w].head + lane * 4;
+    float4 x[N];
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int r = row0 + i * STEP;
+        x[i] = r < t.len ? *reinterpret_cast<const float4*>(in + r * a.in[w].row) : make_float4(0.f, 0.f, 0.f, 0.f);
+        const float y[4] = {fabsf(x[i].x), fabsf(x[i].y), fabsf(x[i].z), fabsf(x[i].w)};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) m = y[k] < INFINITY ? fmaxf(m, y[k]) : m;    // infinities and NaN keep to themselves
+    }
+    if (w == 3) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int r = row0 + i * STEP;
+            float s = 0.f;
+            if (r < t.len) {
+                const float4 o = *reinterpret_cast<const float4*>(a.out + ((t.start + r) * a.heads[3] + h) * HD + lane * 4);
+                s = fmaf(x[i].x, o.x, fmaf(x[i].y, o.y, fmaf(x[i].z, o.z, x[i].w * o.w)));
+            }
+#pragma unroll
+            for (int off = L / 2; off; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+            if (lane == 0 && r < t.len) a.delta[h * a.tokens + t.start + r] = s;
+        }
+    }
+#pragma unroll
+    for (int off = 16; off; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
+    __syncthreads();
+    m = red[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) m = fmaxf(m, red[i]);
+    int e = 14;
+    if (m > 0.f) frexpf(m, &e);            // m < 2^e
+    e = max(14 - e, -112);
+    e = min(e, 120);
+    const float f = ldexpf(1.f, e);
+    if (threadIdx.x == 0) a.factors[w][(long long)slot * a.heads[w] + h] = ldexpf(1.f, -e);
+    __half* p = a.parts[w] + (t.start * 2 * a.heads[w] + h) * HD + lane * 4;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int r = row0 + i * STEP;
+        if (r >= t.len) continue;
+        const float y[4] = {x[i].x * f, x[i].y * f, x[i].z * f, x[i].w * f};
+        __half hi[4], lo[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            hi[k] = __float2half_rn(y[k]);
+            lo[k] = __float2half_rn(y[k] - __half2float(hi[k]));
+        }
+        __half* row = p + (long long)r * 2 * a.heads[w] * HD;
+        *reinterpret_cast<uint2*>(row) = *reinterpret_cast<uint2*>(hi);
+        *reinterpret_cast<uint2*>(row + (long long)a.heads[w] * HD) = *reinterpret_cast<uint2*>(lo);
+    }
+}
+
+// ── tiles and products ────────────────────────────────────────────────────
+struct Args {
+    CUtensorMap q, k, v, g;                // boxes of 64 rows of one part of one head
+    const int* cu;
+    int n_seqs, heads, kv_heads, group, causal, zero_rest;
+    long long tokens;
+    float c, scale;                        // scale * log2(e), scale
+    const float *fq, *fk, *fv, *fg;        // factors
+    const float *lse_in, *delta;
+    float *out, *lse, *dq, *dk, *dv;
+    unsigned int* err;
+};
+
+template <int HD>
+struct Shape {
+    static constexpr int SW = HD * 2 < 128 ? HD * 2 : 128;
+    static constexpr int BOXES = HD * 2 / SW;
+    // A part of a tile: its boxes of all rows; the other part behind it.
+    static constexpr int PART64 = kNarrow * HD * 2, PART128 = kWide * HD * 2;
+    static constexpr int TILE64 = 2 * PART64, TILE128 = 2 * PART128;
+};
+
+// One part-pair of a tile of ROWS rows (64 or 128): boxes [rows, SW] one after another.
+template <int HD, int ROWS>
+__device__ __forceinline__ void load_parts(uint8_t* dst, const CUtensorMap* m, int head, int heads, int row, uint64_t* bar) {
+    using Sh = Shape<HD>;
+#pragma unroll
+    for (int part = 0; part < 2; ++part)
+#pragma unroll
+        for (int b = 0; b < Sh::BOXES; ++b)
+#pragma unroll
+            for (int r = 0; r < ROWS; r += kNarrow)
+                load_3d(dst + part * ROWS * HD * 2 + (b * ROWS + r) * Sh::SW, m, b * (Sh::SW / 2), part * heads + head,
+                        row + r, bar);
+}
+
+// Rows [r0, 64) of both parts become zeros, by one warp.
+template <int HD>
+__device__ __forceinline__ void zero_parts(uint8_t* tile, int r0) {
+    using Sh = Shape<HD>;
+    const int n = (kNarrow - r0) * (Sh::SW / 16), lane = threadIdx.x & 31;
+    for (int e = lane; e < n * Sh::BOXES * 2; e += 32)
+        *reinterpret_cast<uint4*>(tile + (e / n) * kNarrow * Sh::SW + r0 * Sh::SW + (e % n) * 16) = make_uint4(0, 0, 0, 0);
+}
+
+// D = A B^T over HD: A 128 rows, B 64 rows, both in parts.
+template <int HD>
+__device__ __forceinline__ void parts_rows(uint32_t d, uint32_t a, uint32_t b) {
+    using Sh = Shape<HD>;
+    constexpr uint32_t instr = instruction<__half>(kWide, kNarrow, false);
+#pragma unroll
+    for (int t = 0; t < 3; ++t) {          // lo hi, hi lo, hi hi
+        const uint64_t da = operand<Sh::SW>(a + (t == 0 ? Sh::PART128 : 0), 16, 8 * Sh::SW);
+        const uint64_t db = operand<Sh::SW>(b + (t == 1 ? Sh::PART64 : 0), 16, 8 * Sh::SW);
+#pragma unroll
+        for (int k = 0; k < HD; k += 16)
+            mma_ss(d, da + (((k * 2 / Sh::SW) * kWide * Sh::SW + (k * 2) % Sh::SW) >> 4),
+                   db + (((k * 2 / Sh::SW) * kNarrow * Sh::SW + (k * 2) % Sh::SW) >> 4), instr, t > 0 || k > 0);
+    }
+}
+// D = W B: W [128, 64] in tensor memory, for each 32 columns 16 of hi and 16 of
+// lo; B 64 rows in parts, summed over.
+template <int HD>
+__device__ __forceinline__ void parts_weights(uint32_t d, uint32_t w, uint32_t b) {
+    using Sh = Shape<HD>;
+    constexpr uint32_t instr = instruction<__half>(kWide, HD, true);
+#pragma unroll
+    for (int t = 0; t < 3; ++t) {
+        const uint64_t db = operand<Sh::SW>(b + (t == 1 ? Sh::PART64 : 0), kNarrow * Sh::SW, 8 * Sh::SW);
+#pragma unroll
+        for (int k = 0; k < kNarrow; k += 16)
+            mma_ts(d, w + (k / 32) * 32 + (k % 32) / 2 + (t == 0 ? 16 : 0), db + (k * Sh::SW >> 4), instr, t > 0 || k > 0);
+    }
+}
+// 32 weights of a row as parts, to the columns that parts_weights reads.
+__device__ __forceinline__ void put_parts(uint32_t addr, const float (&p)[32]) {
+    uint32_t hi[16], lo[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        hi[i] = pack2<__half>(p[2 * i], p[2 * i + 1]);
+        const __half2 h = *reinterpret_cast<const __half2*>(&hi[i]);
+        lo[i] = pack2<__half>(p[2 * i] - __low2float(h), p[2 * i + 1] - __high2float(h));
+    }
+    st16(addr, hi);
+    st16(addr + 16, lo);
+}
+// acc += f * 32 columns.
+__device__ __forceinline__ void take32(float* acc, uint32_t addr, float f) {
+    uint32_t o[32];
+    ld32(o, addr);
+    wait_ld();
+#pragma unroll
+    for (int i = 0; i < 32; ++i) acc[i] = fmaf(__uint_as_float(o[i]), f, acc[i]);
+}
+__device__ __forceinline__ void store32(float* dst, const float* v, float f) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 4)
+        *reinterpret_cast<float4*>(dst + i) = make_float4(v[i] * f, v[i + 1] * f, v[i + 2] * f, v[i + 3] * f);
+}
+__device__ __forceinline__ void zero_rows_out(float* dst, long long row_stride, int hd, int row0, int len) {
+    const int n = min(kWide, len - row0) * (hd / 4);
+    for (int e = threadIdx.x; e < n; e += blockDim.x)
+        *reinterpret_cast<float4*>(dst + (row0 + e / (hd / 4)) * row_stride + (e % (hd / 4)) * 4) =
+            make_float4(0.f, 0.f, 0.f, 0.f);
+}
+
+// Warps 0-3, 4-7: mathematics; 8: matrix instructions; 9: loads; 10: row statistics.
+constexpr int kThreads = 384;
+constexpr int kLaunchRegs = 168, kMathRegs = 200, kOtherRegs = 104;
+static_assert(kMathRegs * 256 + kOtherRegs * 128 <= kLaunchRegs * kThreads, "register split");
+
+// Slot (of 128 rows) of a row of a sequence.
+__device__ __forceinline__ long long slot_of(const PackedTile& t, int row) { return t.start / kSplit + t.seq + row / kSplit; }
+
+// ── forward ───────────────────────────────────────────────────────────────
+// The warpgroups take the key tiles in turn, each with its own scores, its own
+// reference point and its own sum in registers; the two join at the end.
+template <int HD>
+struct FwdShape {
+    using Sh = Shape<HD>;
+    static constexpr int STAGES = HD == 128 ? 4 : HD == 64 ? 8 : 12;
+    static constexpr int BARS = Sh::TILE128 + STAGES * Sh::TILE64, SMEM = BARS + 512;
+    static_assert(STAGES * Sh::TILE64 >= kWide * (HD + 1) * 4 + kWide * 8, "room to join");
+    static_assert(SMEM <= 227 * 1024, "shared memory");
+};
+
+template <int HD>
+__global__ void __launch_bounds__(kThreads, 1) k_f32_fwd(const __grid_constant__ Args a) {
+    using Sh = Shape<HD>;
+    using Fs = FwdShape<HD>;
+    constexpr int ST = Fs::STAGES;
+    extern __shared__ __align__(1024) uint8_t sm[];
+    uint8_t *qs = sm, *ring = sm + Sh::TILE128;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(sm + Fs::BARS);
+    uint64_t *full = bars, *empty = full + ST, *q_full = empty + ST, *fixed = q_full + 1, *s_ready = fixed + 1,
+             *p_ready = s_ready + 2, *o_ready = p_ready + 2, *joined = o_ready + 2;
+    uint32_t* tmem_base = reinterpret_cast<uint32_t*>(joined + 1);
+    volatile int* gone = reinterpret_cast<volatile int*>(tmem_base + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    const int head = blockIdx.x % a.heads, kvh = head / a.group;
+    const PackedTile t = packed_tile(a.cu, a.n_seqs, a.tokens, kWide, (gridDim.x - 1 - blockIdx.x) / a.heads);
+    if (t.row0 >= t.len) return;
+    float* out = a.out + (t.start * a.heads + head) * HD;
+    const long long out_row = (long long)a.heads * HD;
+    if (t.seq == a.n_seqs) {
+        if (a.zero_rest) zero_rows_out(out, out_row, HD, t.row0, t.len);
+        return;
+    }
+    const int last = a.causal ? min(t.row0 + kWide, t.len) : t.len;
+    const int n = (last + kNarrow - 1) / kNarrow;
+    const bool ragged = n * kNarrow > t.len;
+
+    if (threadIdx.x == 0) {
+        *gone = 0;
+        for (int i = 0; i < ST; ++i) { bar_init(full + i, 1); bar_init(empty + i, 1); }
+        bar_init(q_full, 1); bar_init(fixed, 1); bar_init(joined, 128);
+        for (int w = 0; w < 2; ++w) { bar_init(s_ready + w, 1); bar_init(p_ready + w, 128); bar_init(o_ready + w, 1); }
+        bar_init_done();
+    }
+    if (warp == 8) tmem_alloc(tmem_base, 512);
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tm = *tmem_base, tS = tm, tO = tm + 256;    // S: 64 columns each, O: 128 each
+
+    // The ring holds K0, K1, V0, K2, V1, K3, ...: entry of K_j, of V_j.
+    auto k_entry = [](int j) { return j < 2 ? j : 2 * j - 1; };
+    auto v_entry = [&](int j) { return n == 1 ? 1 : j + 2 < n + 1 ? 2 * j + 2 : n + j; };
+
+    if (warp >= 8) {
+        fewer_registers<kOtherRegs>();
+        if (warp == 9) {
+            if (lane == 0) {
+                const int r0 = (int)t.start;
+                bar_expect(q_full, Sh::TILE128);
+                load_parts<HD, kWide>(qs, &a.q, head, a.heads, r0 + t.row0, q_full);
+                int e = 0;
+                bool ok = true;
+                auto load = [&](const CUtensorMap* m, int j) {
+                    const int st = e % ST;
+                    if (e >= ST) ok = bar_wait(empty + st, (e / ST - 1) & 1, gone);
+                    if (!ok) return;
+                    bar_expect(full + st, Sh::TILE64);
+                    load_parts<HD, kNarrow>(ring + st * Sh::TILE64, m, kvh, a.kv_heads, r0 + j * kNarrow, full + st);
+                    ++e;
+                };
+                load(&a.k, 0);
+                if (ok && n > 1) load(&a.k, 1);
+                for (int j = 0; ok && j < n; ++j) {
+                    load(&a.v, j);
+                    if (ok && j + 2 < n) load(&a.k, j + 2);
+                }
+            }
+            __syncwarp();
+            if (ragged) {
+                const int e = v_entry(n - 1), st = e % ST;
+                if (bar_wait(full + st, (e / ST) & 1, gone)) {
+                    zero_parts<HD>(ring + st * Sh::TILE64, t.len - (n - 1) * kNarrow);
+                    fence_async_smem();
+                }
+                __syncwarp();
+                if (lane == 0) bar_arrive(fixed);
+            }
+        } else if (warp == 8) {
+            if (lane == 0) {
+                auto scores = [&](int j) {
+                    const int e = k_entry(j), st = e % ST;
+                    if (!bar_wait(full + st, (e / ST) & 1, gone)) return false;
+                    parts_rows<HD>(tS + 64 * (j & 1), smem(qs), smem(ring + st * Sh::TILE64));
+                    commit(s_ready + (j & 1));
+                    commit(empty + st);
+                    return true;
+                };
+                bool ok = bar_wait(q_full, 0, gone) && scores(0);
+                if (ok && n > 1) ok = scores(1);
+                for (int j = 0; ok && j < n; ++j) {
+                    const int e = v_entry(j), st = e % ST, w = j & 1;
+                    ok = bar_wait(full + st, (e / ST) & 1, gone) && (!(ragged && j == n - 1) || bar_wait(fixed, 0, gone)) &&
+                         bar_wait(p_ready + w, (j >> 1) & 1, gone);
+                    if (!ok) break;
+                    fence_after();
+                    parts_weights<HD>(tO + 128 * w, tS + 64 * w, smem(ring + st * Sh::TILE64));
+                    commit(o_ready + w);
+                    commit(empty + st);
+                    if (j + 2 < n) ok = scores(j + 2);
+                }
+            }
+            __syncwarp();
+        }
+    } else {
+        more_registers<kMathRegs>();
+        const int w = warp >> 2, lr = (warp & 3) * 32 + lane, row = t.row0 + lr;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, ts = tS + lanes + 64 * w, to = tO + lanes + 128 * w;
+        const float cq = a.c * a.fq[slot_of(t, t.row0) * a.heads + head];
+        const bool neg = a.c < 0.f;
+        float o[HD], m = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int i = 0; i < HD; ++i) o[i] = 0.f;
+        bool ok = true;
+        for (int j = w; j < n; j += 2) {
+            const long long ks = slot_of(t, j * kNarrow) * a.kv_heads + kvh;
+            const float c = cq * a.fk[ks], fv = a.fv[ks];
+            ok = __all_sync(0xffffffffu, bar_wait(s_ready + w, (j >> 1) & 1, gone));
+            if (!ok) break;
+            fence_after();
+            const int lim = min(t.len, a.causal ? row + 1 : t.len) - j * kNarrow;     // keys below are seen
+            const bool part = lim < kNarrow;
+            const float hide = neg ? INFINITY : -INFINITY;
+            float y = hide;
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                uint32_t s[32];
+                ld32(s, ts + 32 * b);
+                wait_ld();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    const float x = part && 32 * b + i >= lim ? hide : __uint_as_float(s[i]);
+                    y = neg ? fminf(y, x) : fmaxf(y, x);
+                }
+            }
+            const float top = y * c;
+            // The reference point moves only when a weight would pass 2^8.
+            if (top > m + 8.f) {
+                const float up = exp2_fast(m - top);
+                m = top;
+                l *= up;
+#pragma unroll
+                for (int i = 0; i < HD; ++i) o[i] *= up;
+            }
+            // Weights carry 2^6, which keeps their second parts above the smallest half.
+            const float ref = m == -INFINITY ? 0.f : m - 6.f;
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                uint32_t s[32];
+                float p[32], add[4] = {0.f, 0.f, 0.f, 0.f};
+                ld32(s, ts + 32 * b);
+                wait_ld();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    p[i] = part && 32 * b + i >= lim ? 0.f : exp2_fast(fmaf(__uint_as_float(s[i]), c, -ref));
+                    add[i & 3] += p[i];
+                }
+                l += (add[0] + add[1]) + (add[2] + add[3]);
+                put_parts(ts + 32 * b, p);
+            }
+            wait_st();
+            fence_before();
+            bar_arrive(p_ready + w);
+            ok = __all_sync(0xffffffffu, bar_wait(o_ready + w, (j >> 1) & 1, gone));
+            if (!ok) break;
+            fence_after();
+#pragma unroll
+            for (int b = 0; b < HD / 32; ++b) take32(o + 32 * b, to + 32 * b, fv);
+        }
+        // All products are done when both warpgroups are through: the ring is free.
+        float* jo = reinterpret_cast<float*>(ring);
+        float2* jm = reinterpret_cast<float2*>(jo + kWide * (HD + 1));
+        if (w == 1) {
+            if (ok && n > 1) {
+                // The last product of the other warpgroup may still read the ring.
+                ok = __all_sync(0xffffffffu, bar_wait(o_ready, ((n - 1) >> 1) & 1, gone));
+                if (ok) {
+                    jm[lr] = make_float2(m, l);
+#pragma unroll
+                    for (int i = 0; i < HD; ++i) jo[lr * (HD + 1) + i] = o[i];
+                }
+                bar_arrive(joined);
+            }
+        } else if (ok) {
+            if (n > 1) {
+                ok = __all_sync(0xffffffffu, bar_wait(joined, 0, gone));
+                const float2 z = jm[lr];
+                const float M = fmaxf(m, z.x), f0 = m == -INFINITY ? 0.f : exp2_fast(m - M),
+                            f1 = z.x == -INFINITY ? 0.f : exp2_fast(z.x - M);
+                l = l * f0 + z.y * f1;
+                m = M;
+#pragma unroll
+                for (int i = 0; i < HD; ++i) o[i] = o[i] * f0 + jo[lr * (HD + 1) + i] * f1;
+            }
+            if (ok && row < t.len) {
+                const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+                for (int b = 0; b < HD / 32; ++b) store32(out + row * out_row + 32 * b, o + 32 * b, inv);
+                if (a.lse)
+                    a.lse[(long long)head * a.tokens + t.start + row] =
+                        l == 0.f ? -INFINITY : (m - 6.f) * 0.69314718055994531f + logf(l);
+            }
+        }
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    if (warp == 8) tmem_free(tm, 512);
+    if (threadIdx.x == 0 && *gone) atomicOr(a.err, kErrTcWait);
+}
+
+// ── backward ──────────────────────────────────────────────────────────────
+// Parts of a tile's largest value reach 2^14, so that with the factors f of dO
+// and V  |dS| <= 2 dim 2^28 f f'.  dS goes into parts times g = 2^15 / that, and
+// P times 2^12: dS' = P' (acc 2^-26 / dim - D g 2^-12), acc the sum of dO V^T's parts.
+constexpr float kPUp = 12.f, kPDown = 1.f / 4096.f;
+template <int HD> constexpr float acc_factor() { return 1.f / (67108864.f * HD); }
+template <int HD> __device__ __forceinline__ float ds_up(float fg, float fv) { return 1.f / (16384.f * HD) / fg / fv; }
+
+template <int HD>
+struct BwdShape {
+    using Sh = Shape<HD>;
+    // Places of Q (dk/dv) or K (dq), which a later product reads again, and of dO or V.
+    static constexpr int A = HD == 128 ? 2 : 3, B = HD == 128 ? 1 : 3;
+    static constexpr int RING = 2 * Sh::TILE128, STAT = RING + (A + B) * Sh::TILE64, BARS = STAT + 2 * 2 * kNarrow * 4;
+    static constexpr int SMEM = BARS + 512;
+    static_assert(SMEM <= 227 * 1024, "shared memory");
+};
+
+// dk and dv of 128 keys: query tiles of 64 pass by, of all heads of the group.
+// The order is dV(i), S(i+1), dK(i), dP(i+1); P(i) lies in S(i)'s columns, dS(i) in dP(i)'s.
+template <int HD>
+__global__ void __launch_bounds__(kThreads, 1) k_f32_dkv(const __grid_constant__ Args a) {
+    using Sh = Shape<HD>;
+    using Bs = BwdShape<HD>;
+    constexpr int NA = Bs::A, NB = Bs::B;
+    extern __shared__ __align__(1024) uint8_t sm[];
+    uint8_t *ks = sm, *vs = sm + Sh::TILE128, *qr = sm + Bs::RING, *gr = qr + NA * Sh::TILE64;
+    float* st_lse = reinterpret_cast<float*>(sm + Bs::STAT);       // [2][64]
+    float* st_d = st_lse + 2 * kNarrow;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(sm + Bs::BARS);
+    uint64_t *q_full = bars, *q_empty = q_full + NA, *q_fixed = q_empty + NA, *g_full = q_fixed + NA, *g_empty = g_full + NB,
+             *g_fixed = g_empty + NB, *kv_full = g_fixed + NB, *stat_full = kv_full + 1,
+             *stat_empty = stat_full + 2, *s_ready = stat_empty + 2, *dp_ready = s_ready + 1, *p_ready = dp_ready + 1,
+             *ds_ready = p_ready + 1, *dv_done = ds_ready + 1, *dk_done = dv_done + 1;
+    uint32_t* tmem_base = reinterpret_cast<uint32_t*>(dk_done + 1);
+    volatile int* gone = reinterpret_cast<volatile int*>(tmem_base + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    const int kvh = blockIdx.x % a.kv_heads;
+    const PackedTile t = packed_tile(a.cu, a.n_seqs, a.tokens, kWide, blockIdx.x / a.kv_heads);
+    if (t.row0 >= t.len) return;
+    const long long out_row = (long long)a.kv_heads * HD;
+    float* dk = a.dk + (t.start * a.kv_heads + kvh) * HD;
+    float* dv = a.dv + (t.start * a.kv_heads + kvh) * HD;
+    if (t.seq == a.n_seqs) {
+        zero_rows_out(dk, out_row, HD, t.row0, t.len);
+        zero_rows_out(dv, out_row, HD, t.row0, t.len);
+        return;
+    }
+    const int first = a.causal ? t.row0 / kNarrow : 0;             // query tiles that see these keys
+    const int nq = (t.len + kNarrow - 1) / kNarrow - first;
+    const int n = nq * a.group;
+    const bool ragged = t.len % kNarrow != 0;                      // the last query tile of each head
+
+    if (threadIdx.x == 0) {
+        *gone = 0;
+        for (int i = 0; i < NA; ++i) { bar_init(q_full + i, 1); bar_init(q_empty + i, 1); bar_init(q_fixed + i, 1); }
+        for (int i = 0; i < NB; ++i) { bar_init(g_full + i, 1); bar_init(g_empty + i, 1); bar_init(g_fixed + i, 1); }
+        bar_init(kv_full, 1);
+        for (int i = 0; i < 2; ++i) { bar_init(stat_full + i, 1); bar_init(stat_empty + i, 256); }
+        bar_init(s_ready, 1); bar_init(dp_ready, 1); bar_init(p_ready, 256); bar_init(ds_ready, 256);
+        bar_init(dv_done, 1); bar_init(dk_done, 1);
+        bar_init_done();
+    }
+    if (warp == 8) tmem_alloc(tmem_base, 512);
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tm = *tmem_base, tS = tm, tP = tm + 64, tV = tm + 128, tK = tm + 256;
+    auto head_of = [&](int i) { return kvh * a.group + i / nq; };
+    auto row_of = [&](int i) { return (first + i % nq) * kNarrow; };
+
+    if (warp >= 8) {
+        fewer_registers<kOtherRegs>();
+        if (warp == 9) {
+            // `fixed` tells that the rows behind the sequence are cleared (their weights
+            // are 0, 0 times another sequence's NaN is not).
+            if (lane == 0) {
+                bar_expect(kv_full, 2 * Sh::TILE128);
+                load_parts<HD, kWide>(ks, &a.k, kvh, a.kv_heads, (int)t.start + t.row0, kv_full);
+                load_parts<HD, kWide>(vs, &a.v, kvh, a.kv_heads, (int)t.start + t.row0, kv_full);
+            }
+            auto load = [&](const CUtensorMap* m, int i, uint8_t* r, uint64_t* full, uint64_t* empty, uint64_t* fixed, int n_places) {
+                const int st = i % n_places;
+                uint8_t* dst = r + st * Sh::TILE64;
+                if (!__all_sync(0xffffffffu, i < n_places || bar_wait(empty + st, (i / n_places - 1) & 1, gone))) return false;
+                if (lane == 0) {
+                    bar_expect(full + st, Sh::TILE64);
+                    load_parts<HD, kNarrow>(dst, m, head_of(i), a.heads, (int)t.start + row_of(i), full + st);
+                }
+                __syncwarp();
+                if (ragged && i % nq == nq - 1) {
+                    if (!__all_sync(0xffffffffu, bar_wait(full + st, (i / n_places) & 1, gone))) return false;
+                    zero_parts<HD>(dst, t.len % kNarrow);
+                    fence_async_smem();
+                    __syncwarp();
+                }
+                if (lane == 0) bar_arrive(fixed + st);
+                return true;
+            };
+            for (int i = 0; i < n; ++i)
+                if (!load(&a.q, i, qr, q_full, q_empty, q_fixed, NA) || !load(&a.g, i, gr, g_full, g_empty, g_fixed, NB)) break;
+        } else if (warp == 8) {
+            if (lane == 0) {
+                auto scores = [&](int i) {
+                    const int st = i % NA;
+                    if (!bar_wait(q_full + st, (i / NA) & 1, gone) || !bar_wait(q_fixed + st, (i / NA) & 1, gone)) return false;
+                    parts_rows<HD>(tS, smem(ks), smem(qr + st * Sh::TILE64));
+                    commit(s_ready);
+                    return true;
+                };
+                auto dps = [&](int i) {
+                    const int st = i % NB;
+                    if (!bar_wait(g_full + st, (i / NB) & 1, gone) || !bar_wait(g_fixed + st, (i / NB) & 1, gone)) return false;
+                    parts_rows<HD>(tP, smem(vs), smem(gr + st * Sh::TILE64));
+                    commit(dp_ready);
+                    return true;
+                };
+                bool ok = bar_wait(kv_full, 0, gone) && scores(0) && dps(0);
+                for (int i = 0; ok && i < n; ++i) {
+                    const bool more = i + 1 < n;
+                    ok = bar_wait(p_ready, i & 1, gone);
+                    if (!ok) break;
+                    fence_after();
+                    parts_weights<HD>(tV, tS, smem(gr + (i % NB) * Sh::TILE64));
+                    commit(dv_done);
+                    commit(g_empty + i % NB);
+                    ok = (!more || scores(i + 1)) && bar_wait(ds_ready, i & 1, gone);
+                    if (!ok) break;
+                    fence_after();
+                    parts_weights<HD>(tK, tP, smem(qr + (i % NA) * Sh::TILE64));
+                    commit(dk_done);
+                    commit(q_empty + i % NA);
+                    ok = !more || dps(i + 1);
+                }
+            }
+            __syncwarp();
+        } else if (warp == 10) {
+            const float fv = a.fv[slot_of(t, t.row0) * a.kv_heads + kvh];
+            for (int i = 0; i < n; ++i) {
+                const int sl = i & 1, h = head_of(i);
+                const bool ok = i < 2 || bar_wait(stat_empty + sl, (i / 2 - 1) & 1, gone);
+                if (!__all_sync(0xffffffffu, ok)) break;
+                const float up = ds_up<HD>(a.fg[slot_of(t, row_of(i)) * a.heads + h], fv) * kPDown;
+                for (int r = lane; r < kNarrow; r += 32) {
+                    const int row = row_of(i) + r;
+                    float x = INFINITY, d = 0.f;
+                    if (row < t.len) {
+                        x = a.lse_in[(long long)h * a.tokens + t.start + row];
+                        x = x == -INFINITY ? INFINITY : x * kLog2e - kPUp;
+                        d = a.delta[(long long)h * a.tokens + t.start + row] * up;
+                    }
+                    st_lse[sl * kNarrow + r] = x;
+                    st_d[sl * kNarrow + r] = d;
+                }
+                __syncwarp();
+                if (lane == 0) bar_arrive(stat_full + sl);
+            }
+        }
+    } else {
+        more_registers<kMathRegs>();
+        const int half = warp >> 2, row = t.row0 + (warp & 3) * 32 + lane;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t s0 = tS + lanes + 32 * half, p0 = tP + lanes + 32 * half;
+        // Half the columns of dv and dk each (dim 32: one warpgroup has dv, the other dk).
+        constexpr int W = HD == 32 ? 32 : HD / 2;
+        const uint32_t v0 = tV + lanes + (HD == 32 ? 0 : W * half), k0 = tK + lanes + (HD == 32 ? 0 : W * half);
+        const long long ks = slot_of(t, t.row0) * a.kv_heads + kvh;
+        const float fk = a.fk[ks], fv = a.fv[ks];
+        float av[W], ak[HD == 32 ? 1 : W];
+#pragma unroll
+        for (int i = 0; i < W; ++i) av[i] = 0.f;
+        if (HD != 32) {
+#pragma unroll
+            for (int i = 0; i < W; ++i) ak[i % (HD == 32 ? 1 : W)] = 0.f;
+        }
+        bool ok = true;
+        float take_k = 0.f;                // factor of the dK tile that has not been taken yet
+        auto add_k = [&](int i) {
+            ok = __all_sync(0xffffffffu, bar_wait(dk_done, i & 1, gone));
+            if (!ok) return;
+            fence_after();
+            if (HD == 32) {
+                if (half == 1) take32(av, k0, take_k);
+            } else {
+#pragma unroll
+                for (int b = 0; b < W / 32; ++b) take32(ak + 32 * b, k0 + 32 * b, take_k);
+            }
+            fence_before();
+        };
+        for (int i = 0; i < n; ++i) {
+            const int sl = i & 1, q0 = row_of(i);
+            const long long qs = slot_of(t, q0) * a.heads + head_of(i);
+            const float fq = a.fq[qs], fg = a.fg[qs], c = a.c * fq * fk;
+            ok = bar_wait(stat_full + sl, (i / 2) & 1, gone) && bar_wait(s_ready, i & 1, gone);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            fence_after();
+            const int see = a.causal ? row - q0 - 32 * half : -1;          // columns from here on see this key
+            const float* lse = st_lse + sl * kNarrow + 32 * half;
+            const float* dd = st_d + sl * kNarrow + 32 * half;
+            float p[32];
+            {
+                uint32_t s[32];
+                ld32(s, s0);
+                wait_ld();
+#pragma unroll
+                for (int x = 0; x < 32; ++x)
+                    p[x] = x < see ? 0.f : exp2_fast(fmaf(__uint_as_float(s[x]), c, -lse[x]));
+                put_parts(s0, p);
+            }
+            wait_st();
+            fence_before();
+            bar_arrive(p_ready);
+            if (i) add_k(i - 1);
+            if (!ok) break;
+            take_k = fq / ds_up<HD>(fg, fv);
+            ok = __all_sync(0xffffffffu, bar_wait(dp_ready, i & 1, gone));
+            if (!ok) break;
+            fence_after();
+            {
+                uint32_t s[32];
+                ld32(s, p0);
+                wait_ld();
+#pragma unroll
+                for (int x = 0; x < 32; ++x)
+                    p[x] = x < see ? 0.f : p[x] * fmaf(__uint_as_float(s[x]), acc_factor<HD>(), -dd[x]);
+                put_parts(p0, p);
+            }
+            wait_st();
+            fence_before();
+            bar_arrive(ds_ready);
+            bar_arrive(stat_empty + sl);
+            ok = __all_sync(0xffffffffu, bar_wait(dv_done, i & 1, gone));
+            if (!ok) break;
+            fence_after();
+            if (HD != 32 || half == 0) {
+#pragma unroll
+                for (int b = 0; b < W / 32; ++b) take32(av + 32 * b, v0 + 32 * b, fg * kPDown);
+            }
+            fence_before();
+        }
+        if (ok) add_k(n - 1);
+        if (ok && row < t.len) {
+            if (HD == 32) {
+                store32((half ? dk : dv) + row * out_row, av, half ? a.scale : 1.f);
+            } else {
+#pragma unroll
+                for (int b = 0; b < W / 32; ++b) {
+                    store32(dv + row * out_row + W * half + 32 * b, av + 32 * b, 1.f);
+                    store32(dk + row * out_row + W * half + 32 * b, ak + 32 * b, a.scale);
+                }
+            }
+        }
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    if (warp == 8) tmem_free(tm, 512);
+    if (threadIdx.x == 0 && *gone) atomicOr(a.err, kErrTcWait);
+}
+
+// dq of 128 queries: key tiles of 64 pass by.  S has two blocks of columns, dS(j)
+// lies in S(j)'s; the order is dP(j+1), dQ(j), S(j+2).
+template <int HD>
+__global__ void __launch_bounds__(kThreads, 1) k_f32_dq(const __grid_constant__ Args a) {
+    using Sh = Shape<HD>;
+    using Bs = BwdShape<HD>;
+    constexpr int NA = Bs::A, NB = Bs::B;
+    extern __shared__ __align__(1024) uint8_t sm[];
+    uint8_t *qs = sm, *gs = sm + Sh::TILE128, *kr = sm + Bs::RING, *vr = kr + NA * Sh::TILE64;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(sm + Bs::BARS);
+    uint64_t *k_full = bars, *k_empty = k_full + NA, *v_full = k_empty + NA, *v_empty = v_full + NB, *fixed = v_empty + NB,
+             *qg_full = fixed + 1, *s_ready = qg_full + 1,
+             *dp_ready = s_ready + 2, *ds_ready = dp_ready + 1, *dq_done = ds_ready + 1;
+    uint32_t* tmem_base = reinterpret_cast<uint32_t*>(dq_done + 1);
+    volatile int* gone = reinterpret_cast<volatile int*>(tmem_base + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    const int head = blockIdx.x % a.heads, kvh = head / a.group;
+    const PackedTile t = packed_tile(a.cu, a.n_seqs, a.tokens, kWide, (gridDim.x - 1 - blockIdx.x) / a.heads);
+    if (t.row0 >= t.len) return;
+    const long long out_row = (long long)a.heads * HD;
+    float* dq = a.dq + (t.start * a.heads + head) * HD;
+    if (t.seq == a.n_seqs) {
+        zero_rows_out(dq, out_row, HD, t.row0, t.len);
+        return;
+    }
+    const int last = a.causal ? min(t.row0 + kWide, t.len) : t.len;
+    const int n = (last + kNarrow - 1) / kNarrow;
+    const bool ragged = n * kNarrow > t.len;
+
+    if (threadIdx.x == 0) {
+        *gone = 0;
+        for (int i = 0; i < NA; ++i) { bar_init(k_full + i, 1); bar_init(k_empty + i, 1); }
+        for (int i = 0; i < NB; ++i) { bar_init(v_full + i, 1); bar_init(v_empty + i, 1); }
+        bar_init(fixed, 1); bar_init(qg_full, 1); bar_init(s_ready, 1); bar_init(s_ready + 1, 1);
+        bar_init(dp_ready, 1); bar_init(ds_ready, 256); bar_init(dq_done, 1);
+        bar_init_done();
+    }
+    if (warp == 8) tmem_alloc(tmem_base, 512);
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tm = *tmem_base, tS = tm, tP = tm + 128, tQ = tm + 256;
+
+    if (warp >= 8) {
+        fewer_registers<kOtherRegs>();
+        if (warp == 9) {
+            if (lane == 0) {
+                const int r0 = (int)t.start;
+                bar_expect(qg_full, 2 * Sh::TILE128);
+                load_parts<HD, kWide>(qs, &a.q, head, a.heads, r0 + t.row0, qg_full);
+                load_parts<HD, kWide>(gs, &a.g, head, a.heads, r0 + t.row0, qg_full);
+                for (int j = 0; j < n; ++j) {
+                    const int sa = j % NA, sb = j % NB;
+                    if (j >= NA && !bar_wait(k_empty + sa, (j / NA - 1) & 1, gone)) break;
+                    bar_expect(k_full + sa, Sh::TILE64);
+                    load_parts<HD, kNarrow>(kr + sa * Sh::TILE64, &a.k, kvh, a.kv_heads, r0 + j * kNarrow, k_full + sa);
+                    if (j >= NB && !bar_wait(v_empty + sb, (j / NB - 1) & 1, gone)) break;
+                    bar_expect(v_full + sb, Sh::TILE64);
+                    load_parts<HD, kNarrow>(vr + sb * Sh::TILE64, &a.v, kvh, a.kv_heads, r0 + j * kNarrow, v_full + sb);
+                }
+            }
+            __syncwarp();
+            if (ragged) {                   // keys behind the sequence: their dS is 0, 0 times NaN would not be
+                const int st = (n - 1) % NA;
+                if (bar_wait(k_full + st, ((n - 1) / NA) & 1, gone)) {
+                    zero_parts<HD>(kr + st * Sh::TILE64, t.len - (n - 1) * kNarrow);
+                    fence_async_smem();
+                }
+                __syncwarp();
+                if (lane == 0) bar_arrive(fixed);
+            }
+        } else if (warp == 8) {
+            if (lane == 0) {
+                auto scores = [&](int j) {
+                    if (!bar_wait(k_full + j % NA, (j / NA) & 1, gone)) return false;
+                    parts_rows<HD>(tS + 64 * (j & 1), smem(qs), smem(kr + (j % NA) * Sh::TILE64));
+                    commit(s_ready + (j & 1));
+                    return true;
+                };
+                auto dps = [&](int j) {
+                    if (!bar_wait(v_full + j % NB, (j / NB) & 1, gone)) return false;
+                    parts_rows<HD>(tP, smem(gs), smem(vr + (j % NB) * Sh::TILE64));
+                    commit(dp_ready);
+                    commit(v_empty + j % NB);
+                    return true;
+                };
+                bool ok = bar_wait(qg_full, 0, gone) && scores(0) && dps(0);
+                if (ok && n > 1) ok = scores(1);
+                for (int j = 0; ok && j < n; ++j) {
+                    ok = bar_wait(ds_ready, j & 1, gone);
+                    if (!ok) break;
+                    fence_after();
+                    if (j + 1 < n) ok = dps(j + 1);
+                    if (ok && ragged && j == n - 1) ok = bar_wait(fixed, 0, gone);
+                    if (!ok) break;
+                    parts_weights<HD>(tQ, tS + 64 * (j & 1), smem(kr + (j % NA) * Sh::TILE64));
+                    commit(dq_done);
+                    commit(k_empty + j % NA);
+                    if (j + 2 < n) ok = scores(j + 2);
+                }
+            }
+            __syncwarp();
+        }
+    } else {
+        more_registers<kMathRegs>();
+        const int half = warp >> 2, row = t.row0 + (warp & 3) * 32 + lane;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        constexpr int W = HD == 32 ? 32 : HD / 2;
+        const uint32_t q0 = tQ + lanes + (HD == 32 ? 0 : W * half), p0 = tP + lanes + 32 * half;
+        const long long qslot = slot_of(t, t.row0) * a.heads + head;
+        const float fq = a.fq[qslot], fg = a.fg[qslot];
+        float lse = INFINITY, d = 0.f, acc[W];
+#pragma unroll
+        for (int i = 0; i < W; ++i) acc[i] = 0.f;
+        if (row < t.len) {
+            const long long at = (long long)head * a.tokens + t.start + row;
+            lse = a.lse_in[at];
+            lse = lse == -INFINITY ? INFINITY : lse * kLog2e - kPUp;
+            d = a.delta[at];
+        }
+        bool ok = true;
+        float take_f = 0.f;
+        auto add_q = [&](int j) {
+            ok = __all_sync(0xffffffffu, bar_wait(dq_done, j & 1, gone));
+            if (!ok) return;
+            fence_after();
+            if (HD != 32 || half == 0) {
+#pragma unroll
+                for (int b = 0; b < W / 32; ++b) take32(acc + 32 * b, q0 + 32 * b, take_f);
+            }
+            fence_before();
+        };
+        for (int j = 0; j < n; ++j) {
+            const uint32_t s0 = tS + lanes + 64 * (j & 1) + 32 * half;
+            const long long ks = slot_of(t, j * kNarrow) * a.kv_heads + kvh;
+            const float fk = a.fk[ks], fv = a.fv[ks], c = a.c * fq * fk;
+            ok = __all_sync(0xffffffffu, bar_wait(s_ready + (j & 1), (j >> 1) & 1, gone));
+            if (!ok) break;
+            fence_after();
+            const int lim = min(t.len, a.causal ? row + 1 : t.len) - j * kNarrow - 32 * half;
+            float p[32];
+            uint32_t s[32];
+            ld32(s, s0);
+            wait_ld();
+#pragma unroll
+            for (int x = 0; x < 32; ++x) p[x] = exp2_fast(fmaf(__uint_as_float(s[x]), c, -lse));
+            if (j) add_q(j - 1);
+            if (!ok) break;
+            const float up = ds_up<HD>(fg, fv), du = d * up * kPDown;
+            take_f = fk / up;
+            ok = __all_sync(0xffffffffu, bar_wait(dp_ready, j & 1, gone));
+            if (!ok) break;
+            fence_after();
+            ld32(s, p0);
+            wait_ld();
+#pragma unroll
+            for (int x = 0; x < 32; ++x)
+                p[x] = x >= lim ? 0.f : p[x] * fmaf(__uint_as_float(s[x]), acc_factor<HD>(), -du);
+            put_parts(s0, p);
+            wait_st();
+            fence_before();
+            bar_arrive(ds_ready);
+        }
+        if (ok) add_q(n - 1);
+        if (ok && row < t.len && (HD != 32 || half == 0)) {
+#pragma unroll
+            for (int b = 0; b < W / 32; ++b)
+                store32(dq + row * out_row + (HD == 32 ? 0 : W * half) + 32 * b, acc + 32 * b, a.scale);
+        }
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    if (warp == 8) tmem_free(tm, 512);
+    if (threadIdx.x == 0 && *gone) atomicOr(a.err, kErrTcWait);
+}
+
+// ── launches ──────────────────────────────────────────────────────────────
+size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+
+// Workspace: parts of q, k, v (and dO), their factors, and D.
+struct Room {
+    __half* parts[4];
+    float* factors[4];
+    float* delta;
+    size_t bytes;
+};
+Room room(void* ws, long long tokens, int n_seqs, int heads, int kv_heads, int hd, int backward) {
+    const long long slots = packed_slots(tokens, n_seqs, kSplit);
+    const int h[4] = {heads, kv_heads, kv_heads, backward ? heads : 0};
+    Room r{};
+    char* p = static_cast<char*>(ws);
+    size_t at = 0;
+    for (int i = 0; i < 4; ++i) {
+        r.parts[i] = reinterpret_cast<__half*>(p + at);
+        at += up256((size_t)tokens * 2 * h[i] * hd * sizeof(__half));
+    }
+    for (int i = 0; i < 4; ++i) {
+        r.factors[i] = reinterpret_cast<float*>(p + at);
+        at += up256((size_t)slots * h[i] * sizeof(float));
+    }
+    r.delta = reinterpret_cast<float*>(p + at);
+    if (backward) at += up256((size_t)tokens * heads * sizeof(float));
+    r.bytes = at;
+    return r;
+}
+
+bool parts_map(CUtensorMap* m, const __half* p, long long tokens, int heads, int hd) {
+    const int sw = hd * 2 < 128 ? hd * 2 : 128;
+    const uint64_t dims[3] = {(uint64_t)hd, (uint64_t)2 * heads, (uint64_t)tokens};
+    const uint64_t strides[2] = {(uint64_t)hd * 2, (uint64_t)2 * heads * hd * 2};
+    const uint32_t box[3] = {(uint32_t)(sw / 2), 1, (uint32_t)kNarrow};
+    return encode_tensor(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, p, dims, strides, box, sw);
+}
+
+template <int HD>
+int launch(const PackedParams& p, const Room& r, Args& a, bool backward, cudaStream_t s) {
+    SplitArgs sp{};
+    const Rows in[4] = {p.q, p.k, p.v, p.dout};
+    const int h[4] = {p.heads, p.kv_heads, p.kv_heads, backward ? p.heads : 0};
+    for (int i = 0; i < 4; ++i) {
+        sp.in[i] = in[i]; sp.heads[i] = h[i]; sp.first[i + 1] = sp.first[i] + h[i];
+        sp.parts[i] = r.parts[i]; sp.factors[i] = r.factors[i];
+    }
+    sp.out = static_cast<const float*>(p.out_in); sp.delta = r.delta;
+    sp.cu = p.cu; sp.n_seqs = p.n_seqs; sp.tokens = p.tokens;
+    const unsigned slots = (unsigned)packed_slots(p.tokens, p.n_seqs, kSplit);
+    k_split<HD><<<slots * sp.first[4], 256, 0, s>>>(sp);
+    if (cudaGetLastError() != cudaSuccess) return kErrCuda;
+    auto go = [&](auto* kernel, int smem, unsigned grid) {
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return kErrCuda;
+        kernel<<<grid, kThreads, smem, s>>>(a);
+        return cudaGetLastError() == cudaSuccess ? kOk : kErrCuda;
+    };
+    if (!backward) return go(&k_f32_fwd<HD>, FwdShape<HD>::SMEM, slots * p.heads);
+    if (int st = go(&k_f32_dkv<HD>, BwdShape<HD>::SMEM, slots * p.kv_heads)) return st;
+    return go(&k_f32_dq<HD>, BwdShape<HD>::SMEM, slots * p.heads);
+}
+
+}  // namespace
+
+size_t attention_packed_f32_workspace(long long tokens, int n_seqs, int heads, int kv_heads, int head_dim, int backward) {
+    return room(nullptr, tokens, n_seqs, heads, kv_heads, head_dim, backward).bytes;
+}
+
+int attention_packed_f32(const PackedParams& p, int backward, cudaStream_t s) {
+    const Room r = room(p.ws, p.tokens, p.n_seqs, p.heads, p.kv_heads, p.head_dim, backward);
+    Args a{};
+    if (!parts_map(&a.q, r.parts[0], p.tokens, p.heads, p.head_dim) ||
+        !parts_map(&a.k, r.parts[1], p.tokens, p.kv_heads, p.head_dim) ||
+        !parts_map(&a.v, r.parts[2], p.tokens, p.kv_heads, p.head_dim) ||
+        (backward && !parts_map(&a.g, r.parts[3], p.tokens, p.heads, p.head_dim)))
+        return kErrUnsupported;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) { cudaGetLastError(); return kErrCuda; }
+    a.cu = p.cu; a.n_seqs = p.n_seqs; a.heads = p.heads; a.kv_heads = p.kv_heads; a.group = p.heads / p.kv_heads;
+    a.causal = p.causal; a.zero_rest = p.zero_rest; a.tokens = p.tokens;
+    // 0 would turn a hidden score's infinity into NaN; 1e-30 weighs the rest alike.
+    a.c = p.scale == 0.f ? 1e-30f : p.scale * kLog2e;
+    a.scale = p.scale;
+    a.fq = r.factors[0]; a.fk = r.factors[1]; a.fv = r.factors[2]; a.fg = r.factors[3];
+    a.lse_in = p.lse_in; a.delta = r.delta;
+    a.out = static_cast<float*>(p.out); a.lse = p.lse;
+    a.dq = static_cast<float*>(p.dq); a.dk = static_cast<float*>(p.dk); a.dv = static_cast<float*>(p.dv);
+    a.err = device_error_word(dev);
+    if (!a.err) return kErrCuda;
+    switch (p.head_dim) {
+        case 32: return launch<32>(p, r, a, backward, s);
+        case 64: return launch<64>(p, r, a, backward, s);
+        default: return launch<128>(p, r, a, backward, s);
+    }
+}
+
+}  // namespace racb

@@ -40,6 +40,9 @@ size_t attention_packed_workspace(long long tokens, int n_seqs, int heads, int k
 // float16 and bfloat16, arguments checked.
 int attention_packed_tc(const PackedParams& p, cudaStream_t s);
 int attention_packed_backward_tc(const PackedParams& p, cudaStream_t s);
+// float32, arguments checked.
+size_t attention_packed_f32_workspace(long long tokens, int n_seqs, int heads, int kv_heads, int head_dim, int backward);
+int attention_packed_f32(const PackedParams& p, int backward, cudaStream_t s);
 bool rows_map(CUtensorMap* m, const Rows& r, int type, long long tokens, int heads, int hd);
 int attention_packed(const PackedParams& p, cudaStream_t s);
 int attention_packed_backward(const PackedParams& p, cudaStream_t s);
