@@ -12,38 +12,19 @@
 // Keys and values come through the page table by 16-byte asynchronous copies,
 // four warps of them, into a ring; hidden rows and bad pages become zeros on
 // the way, and their scores are masked by bits that the loading warps note.
-//
-// Work is split by keys, not by sequences: all tiles of all (sequence, head)
-// units stand in one line, cut into as many equal pieces as there are blocks,
-// so that caches of any lengths keep every SM busy.  Each block reads the
-// lengths and finds its piece; the host need not know them.  A unit that lies
-// in one piece is finished there; of one that is cut each piece leaves its
-// normalised sum and the logarithm of its weight, and a second kernel joins
-// them (its launch overlaps the first).
-#include "attn_common.cuh"
-#include "tensor_core.cuh"
+#include "cached_split.cuh"
 
 namespace racb {
 namespace {
 
 using namespace tc;
 
-constexpr int kKeys = 128;                 // keys of a tile
 constexpr int kRowTile = 128, kUnitRows = 256;
 // Warps 0-3, 4-7: softmax of row tile 0, 1; 8-11: loads; 12: matrix instructions; 13-15 fill the warpgroup.
 constexpr int kThreads = 512;
 constexpr int kLaunchRegs = 128, kMathRegs = 160, kLoadRegs = 104, kOtherRegs = 88;
 static_assert(kMathRegs * 256 + kLoadRegs * 128 + kOtherRegs * 128 <= kLaunchRegs * kThreads, "register split");
 constexpr int kInfo = 8;                   // tiles of key masks in flight
-
-struct Args {
-    CachedParams p;
-    float c;                               // scale * log2(e)
-    int rows, row_units, unit_rows;        // rows of a (sequence, kv head); units they make; rows of a unit
-    int copies;                            // of the rows in a tile: 4 up to 32 rows, 2 up to 64, 1
-    float *part, *part_lse;                // [2 * blocks, unit_rows, dim], [2 * blocks, unit_rows]
-    unsigned int* err;
-};
 
 template <int HD>
 struct Shape {
@@ -67,90 +48,6 @@ __device__ __forceinline__ uint32_t place(int r, int c) {
     constexpr int U = Sh::SW / 16;
     const int sw = U == 8 ? r & 7 : (r >> 1) & 3;
     return (c / U) * Sh::BOX + r * Sh::SW + (((c % U) ^ sw) << 4);
-}
-
-__device__ __forceinline__ int rows_in_cache(const CachedParams& p, int b) {
-    const long long cap = min((long long)p.table_width * p.page_size, 0x7fff0000LL);
-    const long long n = p.lengths[b];
-    return (int)(n < 0 ? 0 : (n > cap ? cap : n));
-}
-__device__ __forceinline__ int new_rows(const CachedParams& p, int b) {
-    return p.counts ? max(0, min(p.counts[b], p.nodes)) : p.nodes;
-}
-// Key tiles of a sequence: one at least, which writes the zeros of an empty one.
-__device__ __forceinline__ int tiles_of(const CachedParams& p, int b) {
-    return max(1, (rows_in_cache(p, b) + kKeys - 1) / kKeys);
-}
-
-// The piece of the line of tiles that a block works on, as segments of one unit each.
-struct Walk {
-    long long pos, end, at;                // at: position of sequence b's first tile
-    int b;
-};
-struct Segment {
-    int b, kvh, unit, tiles, j0, j1;       // key tiles [j0, j1) of `tiles`
-    long long pos;
-};
-__device__ __forceinline__ bool next(const Args& a, Walk& w, Segment& s) {
-    if (w.pos >= w.end) return false;
-    const long long per = (long long)a.p.kv_heads * a.row_units;
-    int n = tiles_of(a.p, w.b);
-    while (w.pos >= w.at + n * per) {
-        w.at += n * per;
-        ++w.b;
-        n = tiles_of(a.p, w.b);
-    }
-    const long long rel = w.pos - w.at, u = rel / n;
-    s.b = w.b;
-    s.kvh = (int)(u / a.row_units);
-    s.unit = (int)(u % a.row_units);
-    s.tiles = n;
-    s.j0 = (int)(rel % n);
-    s.j1 = (int)min((long long)n, s.j0 + w.end - w.pos);
-    s.pos = w.pos;
-    w.pos += s.j1 - s.j0;
-    return true;
-}
-
-// Sum over b < limit of the key tiles, by one warp.
-__device__ __forceinline__ long long tiles_before(const CachedParams& p, int limit) {
-    long long n = 0;
-    for (int b = threadIdx.x & 31; b < limit; b += 32) n += tiles_of(p, b);
-#pragma unroll
-    for (int off = 16; off; off >>= 1) n += __shfl_xor_sync(0xffffffffu, n, off);
-    return n;
-}
-
-// Block `blk` of n works on positions [total blk / n, total (blk + 1) / n), n the
-// blocks launched or, where that is less, the tiles there are: no piece is empty.
-__device__ __forceinline__ Walk piece(const Args& a, int blk, int blocks) {
-    const long long per = (long long)a.p.kv_heads * a.row_units, total = tiles_before(a.p, a.p.batch) * per;
-    const long long n_pieces = min((long long)blocks, total);
-    Walk w;
-    w.pos = blk < n_pieces ? total * blk / n_pieces : total;
-    w.end = blk < n_pieces ? total * (blk + 1) / n_pieces : total;
-    w.at = 0;
-    w.b = 0;
-    const int lane = threadIdx.x & 31;
-    for (int b0 = 0; b0 < a.p.batch && w.pos < w.end; b0 += 32) {
-        long long n = b0 + lane < a.p.batch ? tiles_of(a.p, b0 + lane) * per : 0;
-#pragma unroll
-        for (int off = 1; off < 32; off <<= 1) {
-            const long long x = __shfl_up_sync(0xffffffffu, n, off);
-            if (lane >= off) n += x;
-        }
-        // n: end of sequence b0 + lane, counted from w.at
-        const unsigned past = __ballot_sync(0xffffffffu, w.at + n > w.pos);
-        if (past) {
-            const int l = __ffs(past) - 1;
-            const long long before = __shfl_sync(0xffffffffu, n, l ? l - 1 : 0);
-            w.at += l ? before : 0;
-            w.b = b0 + l;
-            break;
-        }
-        w.at += __shfl_sync(0xffffffffu, n, 31);
-    }
-    return w;
 }
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool live) {
@@ -606,64 +503,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_cached_tc(const __grid_constant
     if (threadIdx.x == 0 && *gone) atomicOr(a.err, kErrTcWait);
 }
 
-// Joins the pieces of cut units: a warp a row, eight rows of one unit a block.
-template <typename T, int HD>
-__global__ void __launch_bounds__(256) k_cached_join(const __grid_constant__ Args a, int launched) {
-    const CachedParams& p = a.p;
-    const long long per = (long long)p.kv_heads * a.row_units;
-    const int parts = (a.unit_rows + 7) / 8, ur = (int)(blockIdx.x % parts) * 8 + (threadIdx.x >> 5);
-    const long long bu = blockIdx.x / parts;
-    const int b = (int)(bu / per), u = (int)(bu % per);
-    const int kvh = u / a.row_units, unit = u % a.row_units, group = p.heads / p.kv_heads;
-    const long long total = tiles_before(p, p.batch) * per;
-    const int n = tiles_of(p, b);
-    const long long blocks = min((long long)launched, total);
-    const long long t0 = tiles_before(p, b) * per + (long long)u * n;
-    const long long c0 = ((t0 + 1) * blocks - 1) / total, c1 = ((t0 + n) * blocks - 1) / total;
-    const int cnt = new_rows(p, b), lane = threadIdx.x & 31;
-    const long long s0 = 2 * c0 + (total * c0 / blocks == t0 ? 0 : 1);     // the first piece's place
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (c0 == c1) return;
-    const int r = unit * kUnitRows + ur, node = r / group;
-    if (ur >= a.unit_rows || r >= a.rows || (node >= cnt && !p.zero_rest)) return;
-    float acc[HD / 32], w = 0.f, m = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < HD / 32; ++i) acc[i] = 0.f;
-    if (node < cnt) {
-        // A running reference point: the pieces are read once.
-#pragma unroll 4
-        for (long long c = c0; c <= c1; ++c) {
-            const long long at = (c == c0 ? s0 : 2 * c) * a.unit_rows + ur;
-            const float x = a.part_lse[at], top = fmaxf(m, x), ref = top == -INFINITY ? 0.f : top;
-            const float keep = exp2_fast(m - ref), f = exp2_fast(x - ref);
-            m = top;
-            w = fmaf(w, keep, f);
-#pragma unroll
-            for (int i = 0; i < HD / 32; ++i) acc[i] = fmaf(f, a.part[at * HD + i * 32 + lane], acc[i] * keep);
-        }
-    }
-    T* out = static_cast<T*>(p.out) + (((long long)b * p.nodes + node) * p.heads + kvh * group + r % group) * HD;
-    const float f = w == 0.f ? 0.f : 1.f / w;
-#pragma unroll
-    for (int i = 0; i < HD / 32; ++i) out[i * 32 + lane] = from_f32<T>(acc[i] * f);
-}
-
 template <typename T, int HD>
 int launch(const Args& a, int blocks, cudaStream_t s) {
     if (cudaFuncSetAttribute(k_cached_tc<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<HD>::SMEM) != cudaSuccess)
         return kErrCuda;
     k_cached_tc<T, HD><<<blocks, kThreads, Shape<HD>::SMEM, s>>>(a);
     if (cudaGetLastError() != cudaSuccess) return kErrCuda;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)((long long)a.p.batch * a.p.kv_heads * a.row_units * ((a.unit_rows + 7) / 8)));
-    cfg.blockDim = dim3(256);
-    cfg.stream = s;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, k_cached_join<T, HD>, a, blocks) == cudaSuccess ? kOk : kErrCuda;
+    return launch_join<T, HD>(a, blocks, s);
 }
 
 template <typename T>
@@ -677,27 +523,14 @@ int by_dim(const Args& a, int blocks, cudaStream_t s) {
 
 }  // namespace
 
-// Two pieces a block.
 size_t attention_cached_tc_workspace(int blocks, int nodes, int heads, int kv_heads, int head_dim) {
-    const long long rows = (long long)nodes * (heads / kv_heads);
-    return (size_t)2 * blocks * (rows < kUnitRows ? rows : kUnitRows) * (head_dim + 1) * sizeof(float);
+    return pieces_bytes(blocks, kUnitRows, nodes, heads, kv_heads, head_dim);
 }
 
 int attention_cached_tc(const CachedParams& p, int blocks, cudaStream_t s) {
     Args a{};
-    a.p = p;
-    // 0 would turn a hidden score's infinity into NaN; 1e-30 weighs the rest alike.
-    a.c = p.scale == 0.f ? 1e-30f : p.scale * 1.4426950408889634f;
-    a.rows = p.nodes * (p.heads / p.kv_heads);
-    a.row_units = (a.rows + kUnitRows - 1) / kUnitRows;
-    a.unit_rows = a.rows < kUnitRows ? a.rows : kUnitRows;
+    if (int st = fill(a, p, kUnitRows, blocks)) return st;
     a.copies = a.unit_rows <= 32 ? 4 : a.unit_rows <= 64 ? 2 : 1;
-    a.part = static_cast<float*>(p.ws);
-    a.part_lse = a.part + (size_t)2 * blocks * a.unit_rows * p.head_dim;
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess) { cudaGetLastError(); return kErrCuda; }
-    a.err = device_error_word(dev);
-    if (!a.err) return kErrCuda;
     return p.type == kBF16 ? by_dim<__nv_bfloat16>(a, blocks, s) : by_dim<__half>(a, blocks, s);
 }
 
