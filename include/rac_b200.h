@@ -170,38 +170,46 @@ int rac_check_device_errors(void *stream);
 /* ── 4. packed prompts and paged caches ─────────────────────────────────── */
 /* Element types.  Sums, softmax statistics and gradients are held in 32 bits
  * whatever the type.  head_dim is 32, 64 or 128; query head h reads key/value
- * head h / (heads / kv_heads).  All pointers are device pointers except
- * `strides`, a host array of element strides; bases are 16-byte aligned and
- * strides are multiples of 16 bytes, the last axis is contiguous. */
+ * head h / (heads / kv_heads).  The arguments come in a structure in host
+ * memory, read before the call returns; all pointers in it are device
+ * pointers, 16-byte aligned where they point to elements.  Strides count
+ * elements and are multiples of 16 bytes; the last axis is contiguous. */
 #define RAC_F32  0
 #define RAC_F16  1
 #define RAC_BF16 2
 
 /* softmax(scale q k^T) v within each of n_seqs sequences laid end to end:
  * sequence i holds rows cu_seqlens[i] .. cu_seqlens[i+1]-1 (cu_seqlens[0] is
- * 0, n_seqs+1 rising int32), lengths of 0 allowed.  q [tokens, heads,
- * head_dim], k and v [tokens, kv_heads, head_dim]; strides = {q row, q head,
- * k row, k head, v row, v head}.  out [tokens, heads, head_dim] contiguous;
- * lse (optional) [heads, tokens], the natural logarithm of each row's sum.
- * Rows behind the last sequence stay as they are, or become zeros where
- * zero_rest is set.  workspace: rac_attention_packed_workspace() bytes,
- * 256-byte aligned (may be NULL where that is 0). */
+ * 0, n_seqs+1 rising int32), lengths of 0 allowed; its contents lead nowhere
+ * outside the tensors.  q [tokens, heads, head_dim], k and v [tokens,
+ * kv_heads, head_dim].  out [tokens, heads, head_dim] contiguous; lse
+ * (optional) [heads, tokens], the natural logarithm of each row's sum.  Rows
+ * behind the last sequence stay as they are, or become zeros where zero_rest
+ * is set.
+ *
+ * The backward call takes the forward's out and lse and the output's gradient
+ * dout, and writes dq like q, dk and dv like k (contiguous), zeros behind the
+ * last sequence.  The same inputs give the same bits.
+ *
+ * workspace: rac_attention_packed_workspace() bytes, 256-byte aligned (may be
+ * NULL where that is 0), free again when the call's kernels are done. */
+typedef struct {
+    const void *q, *k, *v;
+    const int *cu_seqlens;
+    void *out;
+    float *lse;
+    const void *dout;                     /* backward */
+    void *dq, *dk, *dv;                   /* backward */
+    void *workspace;
+    long long strides[8];                 /* q row, q head, k row, k head, v row, v head, dout row, dout head */
+    long long tokens, ws_bytes;
+    int n_seqs, heads, kv_heads, head_dim, dtype, is_causal, zero_rest;
+    float scale;
+} rac_attention_packed_args;
 long long rac_attention_packed_workspace(long long tokens, int n_seqs, int heads, int kv_heads, int head_dim,
                                          int dtype, int backward);
-int rac_attention_packed_async(const void *q, const void *k, const void *v, const long long *strides,
-                               const int *cu_seqlens, int n_seqs, long long tokens, int heads, int kv_heads,
-                               int head_dim, int dtype, int is_causal, float scale, void *out, float *lse,
-                               int zero_rest, void *workspace, long long ws_bytes, void *stream);
-/* Gradients of the above from the forward's out and lse: dq like q, dk and dv
- * like k (contiguous), zeros behind the last sequence.  strides = {q row, q
- * head, k row, k head, v row, v head, dout row, dout head}.  No atomics: the
- * same inputs give the same bits. */
-int rac_attention_packed_backward_async(const void *dout, const void *q, const void *k, const void *v,
-                                        const long long *strides, const void *out, const float *lse,
-                                        const int *cu_seqlens, int n_seqs, long long tokens, int heads,
-                                        int kv_heads, int head_dim, int dtype, int is_causal, float scale,
-                                        void *dq, void *dk, void *dv, void *workspace, long long ws_bytes,
-                                        void *stream);
+int rac_attention_packed_async(const rac_attention_packed_args *args, void *stream);
+int rac_attention_packed_backward_async(const rac_attention_packed_args *args, void *stream);
 
 /* Attention of new tokens over a paged cache.  Pages hold [kv_heads,
  * page_size, head_dim] each; cache row r of sequence b lies in page
@@ -211,39 +219,46 @@ int rac_attention_packed_backward_async(const void *dout, const void *q, const v
  * cache already.  New row i sees every row before the new ones and the new
  * rows j whose bit is set in tree[b, i] (int64 [batch, nodes]), j <= i where
  * tree is NULL; a row that sees nothing gives zeros.  q [batch, nodes, heads,
- * head_dim] with strides = {q batch, q node, q head, k page, k head, k row,
- * v page, v head, v row}; out contiguous, rows from counts[b] on as they were
- * or zeros (zero_rest).  Pages outside [0, n_pages) are not read: their rows
- * count as hidden and rac_check_device_errors() reports RAC_ERR_DEVICE.
- * workspace: rac_attention_cached_workspace() bytes, 256-byte aligned. */
+ * head_dim]; out contiguous, rows from counts[b] on as they were or zeros
+ * (zero_rest).  Pages outside [0, n_pages) are not read: their rows count as
+ * hidden and rac_check_device_errors() reports RAC_ERR_DEVICE.  workspace:
+ * rac_attention_cached_workspace() bytes on the current device, 256-byte
+ * aligned. */
+typedef struct {
+    const void *q, *k_pages, *v_pages;
+    const int *page_table, *lengths, *counts;
+    const long long *tree;
+    void *out;
+    void *workspace;
+    long long strides[9];                 /* q batch, node, head; k page, head, row; v page, head, row */
+    long long ws_bytes;
+    int table_width, n_pages, page_size, batch, nodes, heads, kv_heads, head_dim, dtype, zero_rest;
+    float scale;
+} rac_attention_cached_args;
 long long rac_attention_cached_workspace(int batch, int nodes, int heads, int kv_heads, int head_dim);
-int rac_attention_cached_async(const void *q, const void *k_pages, const void *v_pages, const long long *strides,
-                               const int *page_table, int table_width, int n_pages, int page_size,
-                               const int *lengths, const int *counts, const long long *tree, int batch, int nodes,
-                               int heads, int kv_heads, int head_dim, int dtype, float scale, void *out,
-                               int zero_rest, void *workspace, long long ws_bytes, void *stream);
+int rac_attention_cached_async(const rac_attention_cached_args *args, void *stream);
 
-/* Page operations.  strides = {k layer, page, head, row, v layer, page, head,
- * row, ...}.  Rows and pages outside the cache are skipped and reported as
- * above. */
-/* Rows cu_seqlens[b] .. of k and v (strides[8..11] = k row, k head, v row, v
- * head) to cache rows starts[b] .. of sequence b. */
-int rac_cache_append_async(void *k_pages, void *v_pages, const long long *strides, const void *k, const void *v,
-                           const int *page_table, int table_width, int n_pages, int page_size, const int *starts,
-                           const int *cu_seqlens, int batch, long long tokens, int kv_heads, int head_dim, int dtype,
-                           void *stream);
-/* Page src[i] to page dst[i], in every layer.  No page may be a destination
- * twice, nor a source and a destination (the copies run at once). */
-int rac_cache_copy_pages_async(void *k_pages, void *v_pages, const long long *strides, const int *src,
-                               const int *dst, int n, int layers, int n_pages, int page_size, int kv_heads,
-                               int head_dim, int dtype, void *stream);
+/* Page operations.  Rows and pages outside the cache are skipped and reported
+ * as above. */
+typedef struct {
+    void *k_pages, *v_pages;
+    const void *k, *v;                    /* append: new rows [tokens, kv_heads, head_dim] */
+    const int *page_table, *starts, *cu_seqlens;
+    const int *src, *dst;                 /* copy */
+    const int *accepted, *n_accepted;     /* compact */
+    long long strides[12];                /* k layer, page, head, row; v layer, page, head, row; k row, head; v row, head */
+    long long tokens;
+    int table_width, n_pages, page_size, batch, n, layers, kv_heads, head_dim, dtype;
+} rac_cache_args;
+/* Rows cu_seqlens[b] .. of k and v to cache rows starts[b] .. of sequence b. */
+int rac_cache_append_async(const rac_cache_args *args, void *stream);
+/* Page src[i] to page dst[i] for i < n, in every layer.  No page may be a
+ * destination twice, nor a source and a destination (the copies run at once). */
+int rac_cache_copy_pages_async(const rac_cache_args *args, void *stream);
 /* Cache row starts[b] + accepted[b, i] to row starts[b] + i for i <
- * n_accepted[b], in every layer; all of a sequence's rows are read before the
- * first is written.  nodes (the width of accepted) is at most 64. */
-int rac_cache_compact_async(void *k_pages, void *v_pages, const long long *strides, const int *page_table,
-                            int table_width, int n_pages, int page_size, const int *starts, const int *accepted,
-                            const int *n_accepted, int batch, int nodes, int layers, int kv_heads, int head_dim,
-                            int dtype, void *stream);
+ * n_accepted[b], in every layer; accepted is [batch, n], n at most 64.  All of a
+ * sequence's rows are read before the first is written. */
+int rac_cache_compact_async(const rac_cache_args *args, void *stream);
 
 /* ── op descriptors for rac_execute ─────────────────────────────────────── */
 typedef struct { const float *A, *B; float *C; int M, N, K; } rac_matmul_desc;

@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 import threading
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -33,6 +34,11 @@ class RacError(RuntimeError):
 class Float2(C.Structure):
     _fields_ = [("x", C.c_float), ("y", C.c_float)]
 
+
+# The argument structures of rac_b200.h section 4, field for field.
+PACKED_ARGS = struct.Struct("11P8q2q7if")   # rac_attention_packed_args
+CACHED_ARGS = struct.Struct("9P9qq10if4x")  # rac_attention_cached_args
+CACHE_ARGS = struct.Struct("11P12qq9i4x")   # rac_cache_args
 
 _lock = threading.Lock()
 _lib = None
@@ -101,18 +107,13 @@ _SIGS = {
     "rac_check_device_errors": (_i, [_vp]),
     "rac_attention": (None, [_vp, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i]),
     "rac_attention_packed_workspace": (_ll, [_ll, _i, _i, _i, _i, _i, _i]),
-    "rac_attention_packed_async": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _ll, _i, _i, _i, _i, _i, _f, _vp,
-                                        _vp, _i, _vp, _ll, _vp]),
-    "rac_attention_packed_backward_async": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _ll, _i,
-                                                 _i, _i, _i, _i, _f, _vp, _vp, _vp, _vp, _ll, _vp]),
+    "rac_attention_packed_async": (_i, [_vp, _vp]),
+    "rac_attention_packed_backward_async": (_i, [_vp, _vp]),
     "rac_attention_cached_workspace": (_ll, [_i, _i, _i, _i, _i]),
-    "rac_attention_cached_async": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _vp, _vp, _i, _i, _i,
-                                        _i, _i, _i, _f, _vp, _i, _vp, _ll, _vp]),
-    "rac_cache_append_async": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _vp, _i, _ll, _i, _i,
-                                    _i, _vp]),
-    "rac_cache_copy_pages_async": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp]),
-    "rac_cache_compact_async": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i,
-                                     _i, _vp]),
+    "rac_attention_cached_async": (_i, [_vp, _vp]),
+    "rac_cache_append_async": (_i, [_vp, _vp]),
+    "rac_cache_copy_pages_async": (_i, [_vp, _vp]),
+    "rac_cache_compact_async": (_i, [_vp, _vp]),
     "rac_attention_async": (_i, [_vp, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, _vp]),
 }
 

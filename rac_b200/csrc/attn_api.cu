@@ -24,15 +24,20 @@ int record(int st, const char* name) {
     return record_status(st, msg);
 }
 
-PackedParams packed(const void* q, const void* k, const void* v, const long long* strides, const int* cu, int n_seqs,
-                    long long tokens, int heads, int kv_heads, int head_dim, int dtype, int is_causal, float scale) {
+PackedParams packed(const rac_attention_packed_args& a) {
     PackedParams p{};
-    p.q = {q, strides[0], strides[1]};
-    p.k = {k, strides[2], strides[3]};
-    p.v = {v, strides[4], strides[5]};
-    p.cu = cu; p.n_seqs = n_seqs; p.tokens = tokens;
-    p.heads = heads; p.kv_heads = kv_heads; p.head_dim = head_dim;
-    p.type = dtype; p.causal = is_causal; p.scale = scale;
+    const long long* st = a.strides;
+    p.q = {a.q, st[0], st[1]};
+    p.k = {a.k, st[2], st[3]};
+    p.v = {a.v, st[4], st[5]};
+    p.dout = {a.dout, st[6], st[7]};
+    p.cu = a.cu_seqlens; p.n_seqs = a.n_seqs; p.tokens = a.tokens;
+    p.heads = a.heads; p.kv_heads = a.kv_heads; p.head_dim = a.head_dim;
+    p.type = a.dtype; p.causal = a.is_causal; p.scale = a.scale;
+    p.out = a.out; p.lse = a.lse; p.zero_rest = a.zero_rest;
+    p.out_in = a.out; p.lse_in = a.lse;
+    p.dq = a.dq; p.dk = a.dk; p.dv = a.dv;
+    p.ws = a.workspace; p.ws_bytes = a.ws_bytes > 0 ? (size_t)a.ws_bytes : 0;
     return p;
 }
 
@@ -46,32 +51,14 @@ RAC_API long long rac_attention_packed_workspace(long long tokens, int n_seqs, i
     return (long long)attention_packed_workspace(tokens, n_seqs, heads, kv_heads, head_dim, dtype, backward);
 }
 
-RAC_API int rac_attention_packed_async(const void* q, const void* k, const void* v, const long long* strides,
-                                       const int* cu_seqlens, int n_seqs, long long tokens, int heads, int kv_heads,
-                                       int head_dim, int dtype, int is_causal, float scale, void* out, float* lse,
-                                       int zero_rest, void* workspace, long long ws_bytes, void* stream) {
-    if (!strides) return record(kErrNullPtr, "rac_attention_packed_async");
-    PackedParams p = packed(q, k, v, strides, cu_seqlens, n_seqs, tokens, heads, kv_heads, head_dim, dtype, is_causal,
-                            scale);
-    p.out = out; p.lse = lse; p.zero_rest = zero_rest;
-    p.ws = workspace; p.ws_bytes = ws_bytes > 0 ? (size_t)ws_bytes : 0;
-    return record(attention_packed(p, static_cast<cudaStream_t>(stream)), "rac_attention_packed_async");
+RAC_API int rac_attention_packed_async(const rac_attention_packed_args* args, void* stream) {
+    if (!args) return record(kErrNullPtr, "rac_attention_packed_async");
+    return record(attention_packed(packed(*args), static_cast<cudaStream_t>(stream)), "rac_attention_packed_async");
 }
 
-RAC_API int rac_attention_packed_backward_async(const void* dout, const void* q, const void* k, const void* v,
-                                                const long long* strides, const void* out, const float* lse,
-                                                const int* cu_seqlens, int n_seqs, long long tokens, int heads,
-                                                int kv_heads, int head_dim, int dtype, int is_causal, float scale,
-                                                void* dq, void* dk, void* dv, void* workspace, long long ws_bytes,
-                                                void* stream) {
-    if (!strides) return record(kErrNullPtr, "rac_attention_packed_backward_async");
-    PackedParams p = packed(q, k, v, strides, cu_seqlens, n_seqs, tokens, heads, kv_heads, head_dim, dtype, is_causal,
-                            scale);
-    p.dout = {dout, strides[6], strides[7]};
-    p.out_in = out; p.lse_in = lse;
-    p.dq = dq; p.dk = dk; p.dv = dv;
-    p.ws = workspace; p.ws_bytes = ws_bytes > 0 ? (size_t)ws_bytes : 0;
-    return record(attention_packed_backward(p, static_cast<cudaStream_t>(stream)),
+RAC_API int rac_attention_packed_backward_async(const rac_attention_packed_args* args, void* stream) {
+    if (!args) return record(kErrNullPtr, "rac_attention_packed_backward_async");
+    return record(attention_packed_backward(packed(*args), static_cast<cudaStream_t>(stream)),
                   "rac_attention_packed_backward_async");
 }
 
@@ -80,59 +67,51 @@ RAC_API long long rac_attention_cached_workspace(int batch, int nodes, int heads
     return (long long)attention_cached_workspace(batch, nodes, heads, kv_heads, head_dim);
 }
 
-RAC_API int rac_attention_cached_async(const void* q, const void* k_pages, const void* v_pages,
-                                       const long long* strides, const int* page_table, int table_width, int n_pages,
-                                       int page_size, const int* lengths, const int* counts, const long long* tree,
-                                       int batch, int nodes, int heads, int kv_heads, int head_dim, int dtype,
-                                       float scale, void* out, int zero_rest, void* workspace, long long ws_bytes,
-                                       void* stream) {
-    if (!strides) return record(kErrNullPtr, "rac_attention_cached_async");
+RAC_API int rac_attention_cached_async(const rac_attention_cached_args* args, void* stream) {
+    if (!args) return record(kErrNullPtr, "rac_attention_cached_async");
+    const rac_attention_cached_args& a = *args;
+    const long long* st = a.strides;
     CachedParams p{};
-    p.q = q; p.q_batch = strides[0]; p.q_node = strides[1]; p.q_head = strides[2];
-    p.k = {const_cast<void*>(k_pages), strides[3], strides[4], strides[5], 0};
-    p.v = {const_cast<void*>(v_pages), strides[6], strides[7], strides[8], 0};
-    p.table = page_table; p.table_width = table_width; p.pages = n_pages; p.page_size = page_size;
-    p.lengths = lengths; p.counts = counts; p.tree = tree;
-    p.batch = batch; p.nodes = nodes; p.heads = heads; p.kv_heads = kv_heads; p.head_dim = head_dim; p.type = dtype;
-    p.scale = scale; p.out = out; p.zero_rest = zero_rest;
-    p.ws = workspace; p.ws_bytes = ws_bytes > 0 ? (size_t)ws_bytes : 0;
+    p.q = a.q; p.q_batch = st[0]; p.q_node = st[1]; p.q_head = st[2];
+    p.k = {const_cast<void*>(a.k_pages), st[3], st[4], st[5], 0};
+    p.v = {const_cast<void*>(a.v_pages), st[6], st[7], st[8], 0};
+    p.table = a.page_table; p.table_width = a.table_width; p.pages = a.n_pages; p.page_size = a.page_size;
+    p.lengths = a.lengths; p.counts = a.counts; p.tree = a.tree;
+    p.batch = a.batch; p.nodes = a.nodes; p.heads = a.heads; p.kv_heads = a.kv_heads; p.head_dim = a.head_dim;
+    p.type = a.dtype; p.scale = a.scale; p.out = a.out; p.zero_rest = a.zero_rest;
+    p.ws = a.workspace; p.ws_bytes = a.ws_bytes > 0 ? (size_t)a.ws_bytes : 0;
     return record(attention_cached(p, static_cast<cudaStream_t>(stream)), "rac_attention_cached_async");
 }
 
-RAC_API int rac_cache_append_async(void* k_pages, void* v_pages, const long long* strides, const void* k,
-                                   const void* v, const int* page_table, int table_width, int n_pages, int page_size,
-                                   const int* starts, const int* cu_seqlens, int batch, long long tokens,
-                                   int kv_heads, int head_dim, int dtype, void* stream) {
-    if (!strides) return record(kErrNullPtr, "rac_cache_append_async");
+RAC_API int rac_cache_append_async(const rac_cache_args* args, void* stream) {
+    if (!args) return record(kErrNullPtr, "rac_cache_append_async");
+    const rac_cache_args& a = *args;
     AppendParams p{};
-    p.k = pages(k_pages, strides); p.v = pages(v_pages, strides + 4);
-    p.nk = {k, strides[8], strides[9]}; p.nv = {v, strides[10], strides[11]};
-    p.table = page_table; p.table_width = table_width; p.pages = n_pages; p.page_size = page_size;
-    p.starts = starts; p.cu = cu_seqlens; p.batch = batch; p.tokens = tokens;
-    p.kv_heads = kv_heads; p.head_dim = head_dim; p.type = dtype;
+    p.k = pages(a.k_pages, a.strides); p.v = pages(a.v_pages, a.strides + 4);
+    p.nk = {a.k, a.strides[8], a.strides[9]}; p.nv = {a.v, a.strides[10], a.strides[11]};
+    p.table = a.page_table; p.table_width = a.table_width; p.pages = a.n_pages; p.page_size = a.page_size;
+    p.starts = a.starts; p.cu = a.cu_seqlens; p.batch = a.batch; p.tokens = a.tokens;
+    p.kv_heads = a.kv_heads; p.head_dim = a.head_dim; p.type = a.dtype;
     return record(cache_append(p, static_cast<cudaStream_t>(stream)), "rac_cache_append_async");
 }
 
-RAC_API int rac_cache_copy_pages_async(void* k_pages, void* v_pages, const long long* strides, const int* src,
-                                       const int* dst, int n, int layers, int n_pages, int page_size, int kv_heads,
-                                       int head_dim, int dtype, void* stream) {
-    if (!strides) return record(kErrNullPtr, "rac_cache_copy_pages_async");
+RAC_API int rac_cache_copy_pages_async(const rac_cache_args* args, void* stream) {
+    if (!args) return record(kErrNullPtr, "rac_cache_copy_pages_async");
+    const rac_cache_args& a = *args;
     CopyPagesParams p{};
-    p.k = pages(k_pages, strides); p.v = pages(v_pages, strides + 4);
-    p.src = src; p.dst = dst; p.n = n; p.layers = layers; p.pages = n_pages; p.page_size = page_size;
-    p.kv_heads = kv_heads; p.head_dim = head_dim; p.type = dtype;
+    p.k = pages(a.k_pages, a.strides); p.v = pages(a.v_pages, a.strides + 4);
+    p.src = a.src; p.dst = a.dst; p.n = a.n; p.layers = a.layers; p.pages = a.n_pages; p.page_size = a.page_size;
+    p.kv_heads = a.kv_heads; p.head_dim = a.head_dim; p.type = a.dtype;
     return record(cache_copy_pages(p, static_cast<cudaStream_t>(stream)), "rac_cache_copy_pages_async");
 }
 
-RAC_API int rac_cache_compact_async(void* k_pages, void* v_pages, const long long* strides, const int* page_table,
-                                    int table_width, int n_pages, int page_size, const int* starts,
-                                    const int* accepted, const int* n_accepted, int batch, int nodes, int layers,
-                                    int kv_heads, int head_dim, int dtype, void* stream) {
-    if (!strides) return record(kErrNullPtr, "rac_cache_compact_async");
+RAC_API int rac_cache_compact_async(const rac_cache_args* args, void* stream) {
+    if (!args) return record(kErrNullPtr, "rac_cache_compact_async");
+    const rac_cache_args& a = *args;
     CompactParams p{};
-    p.k = pages(k_pages, strides); p.v = pages(v_pages, strides + 4);
-    p.table = page_table; p.table_width = table_width; p.pages = n_pages; p.page_size = page_size;
-    p.starts = starts; p.accepted = accepted; p.n_accepted = n_accepted; p.batch = batch; p.nodes = nodes;
-    p.layers = layers; p.kv_heads = kv_heads; p.head_dim = head_dim; p.type = dtype;
+    p.k = pages(a.k_pages, a.strides); p.v = pages(a.v_pages, a.strides + 4);
+    p.table = a.page_table; p.table_width = a.table_width; p.pages = a.n_pages; p.page_size = a.page_size;
+    p.starts = a.starts; p.accepted = a.accepted; p.n_accepted = a.n_accepted; p.batch = a.batch; p.nodes = a.n;
+    p.layers = a.layers; p.kv_heads = a.kv_heads; p.head_dim = a.head_dim; p.type = a.dtype;
     return record(cache_compact(p, static_cast<cudaStream_t>(stream)), "rac_cache_compact_async");
 }

@@ -17,7 +17,7 @@ Every call needs CUDA tensors: there is no CPU path, and a CPU tensor is a
 """
 from __future__ import annotations
 
-import ctypes as C
+import functools
 
 import torch
 
@@ -365,110 +365,140 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: torch.Ten
 
 _ELEM = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 MAX_NEW_ROWS = 64            # new rows of a sequence that attention_cached takes (bits of a tree mask)
+_DIMS = (32, 64, 128)
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") \
+    else lambda i: torch.cuda.current_stream(i).cuda_stream
 
 
-def _elem(*ts: torch.Tensor) -> int:
-    dt = ts[0].dtype
-    if dt not in _ELEM:
-        raise ValueError(f"float32, float16 or bfloat16 tensors required, got {dt}")
-    if any(t.dtype != dt for t in ts):
-        raise ValueError(f"tensors of one type required, got {[str(t.dtype) for t in ts]}")
-    return _ELEM[dt]
+def _launch(name: str, args: bytes, device: int) -> None:
+    """Calls an entry point that takes an argument structure, on the device's current stream."""
+    if torch.cuda.current_device() == device:
+        _lib.call(name, args, _raw_stream(device))
+    else:
+        with torch.cuda.device(device):
+            _lib.call(name, args, _raw_stream(device))
 
 
-def _same_device(*ts: torch.Tensor) -> None:
-    _need_cuda(*ts)
-    if any(t is not None and t.device != ts[0].device for t in ts):
-        raise ValueError("tensors on one device required")
+def _elem(t: torch.Tensor, *more: torch.Tensor) -> int:
+    e = _ELEM.get(t.dtype)
+    if e is None:
+        raise ValueError(f"float32, float16 or bfloat16 tensors required, got {t.dtype}")
+    for x in more:
+        if x.dtype is not t.dtype:
+            raise ValueError(f"tensors of one type required, got {t.dtype} and {x.dtype}")
+    return e
+
+
+def _device(t: torch.Tensor, *more: torch.Tensor | None) -> int:
+    d = t.get_device()
+    if d < 0:
+        _need_cuda(t)
+    for x in more:
+        if x is not None and x.get_device() != d:
+            _need_cuda(x)
+            raise ValueError("tensors on one device required")
+    return d
 
 
 def _fits(t: torch.Tensor) -> bool:
     """Whether the kernels take t as it lies: contiguous last axis, 16-byte aligned base and strides, no axis
     expanded."""
     e = t.element_size()
-    return t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(
+    return (t.shape[-1] == 1 or t.stride(-1) == 1) and t.data_ptr() % 16 == 0 and all(
         s > 0 and s * e % 16 == 0 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1)
 
 
-def _lay(t: torch.Tensor) -> torch.Tensor:
-    return t if _fits(t) else t.clone(memory_format=torch.contiguous_format)
-
-
-def _strides(*ts_axes) -> "C.Array":
-    """Element strides of the given (tensor, axes); 0 for an axis of one place, whose stride may be anything."""
-    v = [t.stride(a) if t.shape[a] > 1 else 0 for t, axes in ts_axes for a in axes]
-    return (C.c_longlong * len(v))(*v)
+def _rows(t: torch.Tensor, width: int) -> tuple:
+    """(t or an aligned copy, its address, strides of its outer axes) for elements of `width` bytes."""
+    s = t.stride()
+    x = t.data_ptr()
+    y = x
+    for v in s[:-1]:
+        y |= v * width
+    if y & 15 or s[-1] != 1 or 0 in s:
+        if not _fits(t):
+            t = t.clone(memory_format=torch.contiguous_format)
+            x = t.data_ptr()
+        # The stride of an axis of one place may be anything.
+        s = tuple(v if n > 1 else 0 for v, n in zip(t.stride(), t.shape))
+    return t, x, s[:-1]
 
 
 def _index(name: str, t: torch.Tensor, shape: tuple, dtype=torch.int32) -> torch.Tensor:
-    if t.dtype not in (torch.int32, torch.int64):
-        raise ValueError(f"{name} must hold int32 or int64, got {t.dtype}")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
-    return t.to(dtype).contiguous()
+    if t.dtype is not dtype:
+        if t.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"{name} must hold int32 or int64, got {t.dtype}")
+        t = t.to(dtype)
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _check_heads(heads: int, kv_heads: int, hd: int) -> None:
-    if hd not in (32, 64, 128):
+    if hd not in _DIMS:
         raise ValueError(f"head size 32, 64 or 128 required, got {hd}")
     if kv_heads < 1 or heads < 1 or heads % kv_heads:
         raise ValueError(f"the query heads ({heads}) must be a multiple of the key/value heads ({kv_heads})")
 
 
-def _check_out(name: str, out: torch.Tensor, shape: tuple, dtype) -> torch.Tensor:
-    if tuple(out.shape) != tuple(shape) or out.dtype != dtype or not out.is_contiguous() or out.data_ptr() % 16:
+def _check_out(name: str, out: torch.Tensor, shape: tuple, dtype) -> None:
+    if out.shape != shape or out.dtype is not dtype or not out.is_contiguous() or out.data_ptr() % 16:
         raise ValueError(f"{name} must be a contiguous, 16-byte aligned {tuple(shape)} of {dtype}")
-    return out
+
+
+def _like(t: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def _check_packed(q, k, v, cu_seqlens):
-    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
+    """(element type, cu_seqlens as int32, tokens, heads, kv_heads, dim)"""
+    qs, ks = q.shape, k.shape
+    if len(qs) != 3 or len(ks) != 3:
         raise ValueError("attention_packed: q [tokens, heads, dim] and k, v [tokens, kv_heads, dim] required")
-    if k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
-        raise ValueError(f"attention_packed: shapes {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)} differ")
-    _check_heads(q.shape[1], k.shape[1], q.shape[2])
+    t, h, hd = qs
+    if v.shape != ks or ks[0] != t or ks[2] != hd:
+        raise ValueError(f"attention_packed: shapes {tuple(qs)}, {tuple(ks)}, {tuple(v.shape)} differ")
+    _check_heads(h, ks[1], hd)
     if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
         raise ValueError("attention_packed: cu_seqlens must be 1-D and start with 0")
-    elem = _elem(q, k, v)
-    return elem, _index("cu_seqlens", cu_seqlens, (cu_seqlens.numel(),))
+    return _elem(q, k, v), _index("cu_seqlens", cu_seqlens, cu_seqlens.shape), t, h, ks[1], hd
 
 
-def _workspace(n: int, like: torch.Tensor):
-    return torch.empty(n, dtype=torch.uint8, device=like.device) if n > 0 else None
-
-
-def _scale(scale, hd: int) -> float:
-    return hd ** -0.5 if scale is None else float(scale)
+def _packed_workspace(like, *sizes):
+    n = _lib.lib().rac_attention_packed_workspace(*sizes) if sizes[-2] == 0 or sizes[-1] else 0
+    return (like.new_empty(n, dtype=torch.uint8), n) if n else (None, 0)
 
 
 def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,
                      is_causal: bool = True, scale: float | None = None, out: torch.Tensor | None = None,
                      lse: torch.Tensor | None = None) -> torch.Tensor:
     """softmax(scale q k^T) v within each sequence of a packed batch, on q [tokens, heads, dim] and
-    k, v [tokens, kv_heads, dim] (float32, float16 or bfloat16; head h reads key/value head
-    h // (heads // kv_heads)).  Sequence i holds rows cu_seqlens[i] .. cu_seqlens[i + 1] - 1; cu_seqlens
+    k, v [tokens, kv_heads, dim] (float32, float16 or bfloat16; dim 32, 64 or 128; head h reads key/value
+    head h // (heads // kv_heads)).  Sequence i holds rows cu_seqlens[i] .. cu_seqlens[i + 1] - 1; cu_seqlens
     starts with 0 and rises, lengths of 0 are allowed.  It stays on the device: its values are not checked,
     and no values lead outside the tensors.  scale None is dim ** -0.5.
 
     Rows behind the last sequence keep what `out` holds; without `out` they are zeros.  What lies in another
-    sequence, NaN included, reaches no row.  `lse`, a float32 [heads, tokens], receives the logarithm of each
-    row's sum, which attention_packed_backward needs."""
-    elem, cu = _check_packed(q, k, v, cu_seqlens)
-    t, h, hd = q.shape
+    sequence, NaN included, reaches no row.  (Within a sequence a NaN or an infinity in v reaches every row of
+    the 128 whose keys it stands among, hidden or not.)  `lse`, a float32 [heads, tokens], receives the
+    logarithm of each row's sum, which attention_packed_backward needs."""
+    elem, cu, t, h, kv, hd = _check_packed(q, k, v, cu_seqlens)
     if out is not None:
         _check_out("out", out, q.shape, q.dtype)
     if lse is not None:
         _check_out("lse", lse, (h, t), torch.float32)
-    _same_device(q, k, v, cu, out, lse)
-    q, k, v = _lay(q), _lay(k), _lay(v)
-    o = torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else out
-    with torch.cuda.device(q.device):
-        n = cu.numel() - 1
-        ws = _workspace(_lib.lib().rac_attention_packed_workspace(t, n, h, k.shape[1], hd, elem, 0), q)
-        _lib.call("rac_attention_packed_async", q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                  _strides((q, (0, 1)), (k, (0, 1)), (v, (0, 1))), cu.data_ptr(), n, t, h, k.shape[1],
-                  hd, elem, int(bool(is_causal)), _scale(scale, hd), o.data_ptr(), _ptr(lse), int(out is None),
-                  _ptr(ws), ws.numel() if ws is not None else 0, _stream(q))
+    d = _device(q, k, v, cu, out, lse)
+    w = 2 if elem else 4
+    q, qp, qs = _rows(q, w)
+    k, kp, ks = _rows(k, w)
+    v, vp, vs = _rows(v, w)
+    o = _like(q) if out is None else out
+    n = cu.shape[0] - 1
+    ws, ws_n = _packed_workspace(q, t, n, h, kv, hd, elem, 0)
+    _launch("rac_attention_packed_async", _lib.PACKED_ARGS.pack(
+        qp, kp, vp, cu.data_ptr(), o.data_ptr(), 0 if lse is None else lse.data_ptr(), 0, 0, 0, 0,
+        ws.data_ptr() if ws_n else 0, *qs, *ks, *vs, 0, 0, t, ws_n, n, h, kv, hd, elem, bool(is_causal), out is None,
+        hd ** -0.5 if scale is None else scale), d)
     return o
 
 
@@ -477,44 +507,56 @@ def attention_packed_backward(grad_out: torch.Tensor, q: torch.Tensor, k: torch.
                               is_causal: bool = True, scale: float | None = None):
     """Gradients (dq, dk, dv) of attention_packed from its out and lse; the key/value heads' sum over the
     query heads that read them.  Rows behind the last sequence get zeros.  The same inputs give the same bits."""
-    elem, cu = _check_packed(q, k, v, cu_seqlens)
+    elem, cu, t, h, kv, hd = _check_packed(q, k, v, cu_seqlens)
     if grad_out.shape != q.shape:
         raise ValueError(f"grad_out must be {tuple(q.shape)}, got {tuple(grad_out.shape)}")
     _elem(q, grad_out)
-    t, h, hd = q.shape
     _check_out("out", out, q.shape, q.dtype)
     _check_out("lse", lse, (h, t), torch.float32)
-    _same_device(q, k, v, cu, grad_out, out, lse)
-    q, k, v, g = _lay(q), _lay(k), _lay(v), _lay(grad_out)
-    dq = torch.empty_like(q, memory_format=torch.contiguous_format)
-    dk = torch.empty_like(k, memory_format=torch.contiguous_format)
-    dv = torch.empty_like(v, memory_format=torch.contiguous_format)
-    with torch.cuda.device(q.device):
-        n = cu.numel() - 1
-        ws = _workspace(_lib.lib().rac_attention_packed_workspace(t, n, h, k.shape[1], hd, elem, 1), q)
-        _lib.call("rac_attention_packed_backward_async", g.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                  _strides((q, (0, 1)), (k, (0, 1)), (v, (0, 1)), (g, (0, 1))), out.data_ptr(), lse.data_ptr(),
-                  cu.data_ptr(), n, t, h, k.shape[1], hd, elem, int(bool(is_causal)), _scale(scale, hd),
-                  dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(ws), ws.numel() if ws is not None else 0,
-                  _stream(q))
+    d = _device(q, k, v, cu, grad_out, out, lse)
+    w = 2 if elem else 4
+    q, qp, qs = _rows(q, w)
+    k, kp, ks = _rows(k, w)
+    v, vp, vs = _rows(v, w)
+    g, gp, gs = _rows(grad_out, w)
+    dq, dk, dv = _like(q), _like(k), _like(v)
+    n = cu.shape[0] - 1
+    ws, ws_n = _packed_workspace(q, t, n, h, kv, hd, elem, 1)
+    _launch("rac_attention_packed_backward_async", _lib.PACKED_ARGS.pack(
+        qp, kp, vp, cu.data_ptr(), out.data_ptr(), lse.data_ptr(), gp, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+        ws.data_ptr() if ws_n else 0, *qs, *ks, *vs, *gs, t, ws_n, n, h, kv, hd, elem, bool(is_causal), 1,
+        hd ** -0.5 if scale is None else scale), d)
     return dq, dk, dv
 
 
 def _check_pages(k_pages, v_pages, layers: bool):
-    """(type, [layers,] pages, kv_heads, page_size, dim) of a cache's two page tensors."""
-    want = (4, 5) if layers else (4,)
-    if k_pages.dim() not in want or k_pages.shape != v_pages.shape:
-        raise ValueError("k_pages and v_pages must be alike, " + ("[layers, " if layers else "[") +
+    """(type, strides [layer,] page, head, row of k, of v, pages, kv_heads, page_size, dim) of two page tensors."""
+    s = k_pages.shape
+    if len(s) != 4 and not (layers and len(s) == 5) or v_pages.shape != s:
+        raise ValueError("k_pages and v_pages must be alike, " + ("[[layers,] " if layers else "[") +
                          "pages, kv_heads, page_size, dim]")
-    e = k_pages.element_size()
-    if k_pages.shape[-1] * e % 16 or k_pages.shape[-1] * e > 512:
-        raise ValueError(f"pages' rows must be whole 16-byte units and 512 bytes at most, got {k_pages.shape[-1] * e}")
-    if k_pages.shape[-2] < 1 or k_pages.shape[-3] < 1:
-        raise ValueError("pages must hold at least one row and one head")
     elem = _elem(k_pages, v_pages)
+    row = s[-1] * (2 if elem else 4)
+    if row % 16 or row > 512:
+        raise ValueError(f"pages' rows must be whole 16-byte units and 512 bytes at most, got {row}")
+    if s[-2] < 1 or s[-3] < 1:
+        raise ValueError("pages must hold at least one row and one head")
     if not _fits(k_pages) or not _fits(v_pages):
         raise ValueError("pages need a contiguous last axis and 16-byte aligned rows")
-    return elem, k_pages.shape[-4], k_pages.shape[-3], k_pages.shape[-2], k_pages.shape[-1]
+    return elem, k_pages.stride()[:-1], v_pages.stride()[:-1], s[-4], s[-3], s[-2], s[-1]
+
+
+def _check_table(table: torch.Tensor, b: int) -> torch.Tensor:
+    s = table.shape
+    if len(s) != 2 or s[0] != b:
+        raise ValueError(f"page_table must be [{b}, pages of the longest], got {tuple(s)}")
+    return _index("page_table", table, s)
+
+
+@functools.lru_cache(maxsize=256)
+def _cached_workspace(device: int, b: int, n: int, h: int, kv: int, hd: int) -> int:
+    with torch.cuda.device(device):
+        return _lib.lib().rac_attention_cached_workspace(b, n, h, kv, hd)
 
 
 def attention_cached(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
@@ -531,43 +573,38 @@ def attention_cached(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     sees nothing gives zeros.  Rows from counts[b] on keep what `out` holds; without `out` they are zeros.
     Cache rows behind lengths[b] may hold anything.  A page number outside the cache is not followed: its rows
     count as hidden, and check_device_errors() raises."""
-    if q.dim() != 4:
+    qs = q.shape
+    if len(qs) != 4:
         raise ValueError("attention_cached: q [batch, nodes, heads, dim] required")
-    b, n, h, hd = q.shape
+    b, n, h, hd = qs
     if n > MAX_NEW_ROWS:
         raise ValueError(f"attention_cached: at most {MAX_NEW_ROWS} new rows a sequence, got {n}")
-    if k_pages.dim() != 4 or k_pages.shape[-1] != hd:
+    ks = k_pages.shape
+    if len(ks) != 4 or ks[3] != hd:
         raise ValueError(f"attention_cached: pages [pages, kv_heads, page_size, {hd}] required")
-    _check_heads(h, k_pages.shape[1], hd)
-    _elem(q, k_pages, v_pages)
-    if page_table.dim() != 2 or page_table.shape[0] != b:
-        raise ValueError(f"page_table must be [{b}, pages of the longest], got {tuple(page_table.shape)}")
-    table = _index("page_table", page_table, page_table.shape)
+    _check_heads(h, ks[1], hd)
+    _elem(q, k_pages)
+    table = _check_table(page_table, b)
     lens = _index("lengths", lengths, (b,))
     cnt = _index("counts", counts, (b,)) if counts is not None else None
-    if tree is not None and tree.dtype != torch.int64:
-        raise ValueError(f"tree must hold int64 masks, got {tree.dtype}")
-    tr = _index("tree", tree, (b, n), torch.int64) if tree is not None else None
-    elem, pages, kv, page, _ = _check_pages(k_pages, v_pages, False)
+    if tree is not None:
+        if tree.dtype is not torch.int64:
+            raise ValueError(f"tree must hold int64 masks, got {tree.dtype}")
+        tree = _index("tree", tree, (b, n), torch.int64)
+    elem, kst, vst, pages, kv, page, _ = _check_pages(k_pages, v_pages, False)
     if out is not None:
-        _check_out("out", out, q.shape, q.dtype)
-    _same_device(q, k_pages, v_pages, table, lens, cnt, tr, out)
-    q = _lay(q)
-    o = torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else out
-    with torch.cuda.device(q.device):
-        ws = _workspace(_lib.lib().rac_attention_cached_workspace(b, n, h, kv, hd), q)
-        _lib.call("rac_attention_cached_async", q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
-                  _strides((q, (0, 1, 2)), (k_pages, (0, 1, 2)), (v_pages, (0, 1, 2))), table.data_ptr(),
-                  table.shape[1], pages, page, lens.data_ptr(), _ptr(cnt), _ptr(tr), b, n, h, kv, hd, elem,
-                  _scale(scale, hd), o.data_ptr(), int(out is None), _ptr(ws), ws.numel() if ws is not None else 0,
-                  _stream(q))
+        _check_out("out", out, qs, q.dtype)
+    d = _device(q, k_pages, v_pages, table, lens, cnt, tree, out)
+    q, qp, qst = _rows(q, 2 if elem else 4)
+    o = _like(q) if out is None else out
+    ws_n = _cached_workspace(d, b, n, h, kv, hd)
+    ws = q.new_empty(ws_n, dtype=torch.uint8)
+    _launch("rac_attention_cached_async", _lib.CACHED_ARGS.pack(
+        qp, k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(), lens.data_ptr(),
+        0 if cnt is None else cnt.data_ptr(), 0 if tree is None else tree.data_ptr(), o.data_ptr(), ws.data_ptr(),
+        *qst, *kst, *vst, ws_n, table.shape[1], pages, page, b, n, h, kv, hd, elem, out is None,
+        hd ** -0.5 if scale is None else scale), d)
     return o
-
-
-def _page_strides(k_pages, v_pages, *more):
-    """{layer, page, head, row} strides of both tensors, then those of `more`."""
-    lead = [x if x.dim() == 5 else x.unsqueeze(0) for x in (k_pages, v_pages)]
-    return _strides((lead[0], (0, 1, 2, 3)), (lead[1], (0, 1, 2, 3)), *more)
 
 
 def cache_append_(k_pages: torch.Tensor, v_pages: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
@@ -575,23 +612,25 @@ def cache_append_(k_pages: torch.Tensor, v_pages: torch.Tensor, k: torch.Tensor,
     """Writes new rows k, v [tokens, kv_heads, dim] into a cache's pages [pages, kv_heads, page_size, dim], in
     place: row cu_seqlens[b] + i to cache row starts[b] + i of sequence b.  Rows behind the last sequence are
     not written.  A row whose page is outside the cache is skipped, and check_device_errors() raises."""
-    if k.dim() != 3 or k.shape != v.shape or k_pages.dim() != 4 or k.shape[1] != k_pages.shape[1] or \
-            k.shape[2] != k_pages.shape[3]:
-        raise ValueError(f"cache_append_: rows {tuple(k.shape)}, {tuple(v.shape)} do not fit pages {tuple(k_pages.shape)}")
-    _elem(k_pages, v_pages, k, v)
+    s, ps = k.shape, k_pages.shape
+    if len(s) != 3 or v.shape != s or len(ps) != 4 or s[1] != ps[1] or s[2] != ps[3]:
+        raise ValueError(f"cache_append_: rows {tuple(s)}, {tuple(v.shape)} do not fit pages {tuple(ps)}")
+    _elem(k_pages, k, v)
     b = starts.numel()
-    if page_table.dim() != 2 or page_table.shape[0] != b:
-        raise ValueError(f"page_table must be [{b}, pages of the longest], got {tuple(page_table.shape)}")
-    table, at = _index("page_table", page_table, page_table.shape), _index("starts", starts, (b,))
+    table, at = _check_table(page_table, b), _index("starts", starts, (b,))
     cu = _index("cu_seqlens", cu_seqlens, (b + 1,))
-    elem, pages, kv, page, hd = _check_pages(k_pages, v_pages, False)
-    _same_device(k_pages, v_pages, k, v, table, at, cu)
-    k, v = _lay(k), _lay(v)
-    with torch.cuda.device(k_pages.device):
-        _lib.call("rac_cache_append_async", k_pages.data_ptr(), v_pages.data_ptr(),
-                  _page_strides(k_pages, v_pages, (k, (0, 1)), (v, (0, 1))), k.data_ptr(), v.data_ptr(),
-                  table.data_ptr(), table.shape[1], pages, page, at.data_ptr(), cu.data_ptr(), b, k.shape[0], kv, hd,
-                  elem, _stream(k_pages))
+    elem, kst, vst, pages, kv, page, hd = _check_pages(k_pages, v_pages, False)
+    d = _device(k_pages, v_pages, k, v, table, at, cu)
+    w = 2 if elem else 4
+    k, kp, ks = _rows(k, w)
+    v, vp, vs = _rows(v, w)
+    _launch("rac_cache_append_async", _lib.CACHE_ARGS.pack(
+        k_pages.data_ptr(), v_pages.data_ptr(), kp, vp, table.data_ptr(), at.data_ptr(), cu.data_ptr(), 0, 0, 0, 0,
+        0, *kst, 0, *vst, *ks, *vs, s[0], table.shape[1], pages, page, b, 0, 1, kv, hd, elem), d)
+
+
+def _layered(st: tuple) -> tuple:
+    return st if len(st) == 4 else (0, *st)
 
 
 def cache_copy_pages_(k_pages: torch.Tensor, v_pages: torch.Tensor, src: torch.Tensor, dst: torch.Tensor) -> None:
@@ -600,14 +639,13 @@ def cache_copy_pages_(k_pages: torch.Tensor, v_pages: torch.Tensor, src: torch.T
     Page numbers outside the cache are skipped, and check_device_errors() raises."""
     if src.dim() != 1 or dst.shape != src.shape:
         raise ValueError(f"src and dst must be 1-D and alike, got {tuple(src.shape)} and {tuple(dst.shape)}")
-    s, d = _index("src", src, src.shape), _index("dst", dst, src.shape)
-    elem, pages, kv, page, hd = _check_pages(k_pages, v_pages, True)
-    _same_device(k_pages, v_pages, s, d)
-    layers = k_pages.shape[0] if k_pages.dim() == 5 else 1
-    with torch.cuda.device(k_pages.device):
-        _lib.call("rac_cache_copy_pages_async", k_pages.data_ptr(), v_pages.data_ptr(),
-                  _page_strides(k_pages, v_pages), s.data_ptr(), d.data_ptr(), s.numel(), layers, pages, page, kv, hd,
-                  elem, _stream(k_pages))
+    s, t = _index("src", src, src.shape), _index("dst", dst, src.shape)
+    elem, kst, vst, pages, kv, page, hd = _check_pages(k_pages, v_pages, True)
+    d = _device(k_pages, v_pages, s, t)
+    layers = k_pages.shape[0] if len(kst) == 4 else 1
+    _launch("rac_cache_copy_pages_async", _lib.CACHE_ARGS.pack(
+        k_pages.data_ptr(), v_pages.data_ptr(), 0, 0, 0, 0, 0, s.data_ptr(), t.data_ptr(), 0, 0,
+        *_layered(kst), *_layered(vst), 0, 0, 0, 0, 0, 0, pages, page, 0, s.shape[0], layers, kv, hd, elem), d)
 
 
 def cache_compact_(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, starts: torch.Tensor,
@@ -618,19 +656,18 @@ def cache_compact_(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: tor
     all read before the first is written, so the nodes may come in any order.  Sequences that share a page
     must not both move rows in it."""
     b = starts.numel()
-    if accepted.dim() != 2 or accepted.shape[0] != b or accepted.shape[1] > MAX_NEW_ROWS:
-        raise ValueError(f"accepted must be [{b}, at most {MAX_NEW_ROWS}], got {tuple(accepted.shape)}")
-    if page_table.dim() != 2 or page_table.shape[0] != b:
-        raise ValueError(f"page_table must be [{b}, pages of the longest], got {tuple(page_table.shape)}")
-    table, at = _index("page_table", page_table, page_table.shape), _index("starts", starts, (b,))
-    acc, n_acc = _index("accepted", accepted, accepted.shape), _index("n_accepted", n_accepted, (b,))
-    elem, pages, kv, page, hd = _check_pages(k_pages, v_pages, True)
-    _same_device(k_pages, v_pages, table, at, acc, n_acc)
-    layers = k_pages.shape[0] if k_pages.dim() == 5 else 1
-    with torch.cuda.device(k_pages.device):
-        _lib.call("rac_cache_compact_async", k_pages.data_ptr(), v_pages.data_ptr(), _page_strides(k_pages, v_pages),
-                  table.data_ptr(), table.shape[1], pages, page, at.data_ptr(), acc.data_ptr(), n_acc.data_ptr(), b,
-                  acc.shape[1], layers, kv, hd, elem, _stream(k_pages))
+    s = accepted.shape
+    if len(s) != 2 or s[0] != b or s[1] > MAX_NEW_ROWS:
+        raise ValueError(f"accepted must be [{b}, at most {MAX_NEW_ROWS}], got {tuple(s)}")
+    table, at = _check_table(page_table, b), _index("starts", starts, (b,))
+    acc, n_acc = _index("accepted", accepted, s), _index("n_accepted", n_accepted, (b,))
+    elem, kst, vst, pages, kv, page, hd = _check_pages(k_pages, v_pages, True)
+    d = _device(k_pages, v_pages, table, at, acc, n_acc)
+    layers = k_pages.shape[0] if len(kst) == 4 else 1
+    _launch("rac_cache_compact_async", _lib.CACHE_ARGS.pack(
+        k_pages.data_ptr(), v_pages.data_ptr(), 0, 0, table.data_ptr(), at.data_ptr(), 0, 0, 0, acc.data_ptr(),
+        n_acc.data_ptr(), *_layered(kst), *_layered(vst), 0, 0, 0, 0, 0, table.shape[1], pages, page, b, s[1], layers,
+        kv, hd, elem), d)
 
 
 def check_device_errors(device=None) -> None:

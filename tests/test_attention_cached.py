@@ -223,16 +223,13 @@ def test_refusals():
 
 
 def test_c_entry_refuses():
-    import ctypes
     L = _lib.lib()
-    st = (ctypes.c_longlong * 9)(*[64] * 9)
-    one = ctypes.c_void_p(256)
 
-    def call(q=one, heads=4, kv=2, hd=64, dt=0, nodes=1, batch=1, page=16, strides=st, ws=0):
-        return L.rac_attention_cached_async(q, one, one, strides, one, 4, 8, page, one, None, None, batch, nodes, heads,
-                                            kv, hd, dt, 1.0, one, 0, None, ws, None)
+    def call(q=256, heads=4, kv=2, hd=64, dt=0, nodes=1, batch=1, page=16):
+        return L.rac_attention_cached_async(_lib.CACHED_ARGS.pack(
+            q, 256, 256, 256, 256, 0, 0, 256, 0, *[64] * 9, 0, 4, 8, page, batch, nodes, heads, kv, hd, dt, 0, 1.0), None)
 
     assert call(nodes=65) == -2 and call(heads=3) == -2 and call(page=0) == -2 and call(batch=-1) == -2
-    assert call(hd=96) == -5 and call(dt=9) == -5 and call(q=ctypes.c_void_p(264)) == -5
-    assert call(q=None) == -1 and call(strides=None) == -1
+    assert call(hd=96) == -5 and call(dt=9) == -5 and call(q=264) == -5
+    assert call(q=0) == -1 and L.rac_attention_cached_async(None, None) == -1
     assert call(batch=0) == 0 and call(nodes=0) == 0

@@ -253,23 +253,20 @@ def test_refusals():
 
 
 def test_c_entry_refuses():
-    import ctypes
     from rac_b200 import _lib
     L = _lib.lib()
-    st = (ctypes.c_longlong * 8)(*[64] * 8)
-    one = ctypes.c_void_p(256)
 
-    def fwd(heads=4, kv=2, hd=64, dt=0, tokens=8, q=one, strides=st):
-        return L.rac_attention_packed_async(q, one, one, strides, one, 1, tokens, heads, kv, hd, dt, 1, 1.0, one, None,
-                                            0, None, 0, None)
+    def fwd(heads=4, kv=2, hd=64, dt=0, tokens=8, q=256, stride=64, name="rac_attention_packed_async"):
+        return getattr(L, name)(_lib.PACKED_ARGS.pack(q, 256, 256, 256, 256, 256, 256, 256, 256, 256, 0, *[stride] * 8,
+                                                      tokens, 0, 1, heads, kv, hd, dt, 1, 0, 1.0), None)
 
-    assert fwd(heads=5) == -2 and fwd(kv=0) == -2 and fwd(tokens=-1) == -2
-    assert fwd(hd=80) == -5 and fwd(dt=3) == -5
-    assert fwd(q=None) == -1 and fwd(strides=None) == -1
-    assert fwd(q=ctypes.c_void_p(257)) == -5
-    odd = (ctypes.c_longlong * 8)(*[66] * 8)
-    assert fwd(dt=1, strides=odd) == -5
-    assert fwd(tokens=0) == 0
+    for name in ("rac_attention_packed_async", "rac_attention_packed_backward_async"):
+        assert fwd(heads=5, name=name) == -2 and fwd(kv=0, name=name) == -2 and fwd(tokens=-1, name=name) == -2
+        assert fwd(hd=80, name=name) == -5 and fwd(dt=3, name=name) == -5
+        assert fwd(q=0, name=name) == -1 and getattr(L, name)(None, None) == -1
+        assert fwd(q=264, name=name) == -5 and fwd(dt=1, stride=66, name=name) == -5
+        assert fwd(name=name) == -3                                          # no workspace
+        assert fwd(tokens=0, name=name) == 0
 
 
 # ── in the modules ─────────────────────────────────────────────────────────

@@ -126,6 +126,22 @@ def test_refusals():
             call()
 
 
+def test_c_entries_refuse():
+    L = _lib.lib()
+
+    def call(name, k=256, pages=8, page=16, kv=2, hd=64, dt=0, n=4, layers=1, batch=2, tokens=4, stride=64):
+        return getattr(L, name)(_lib.CACHE_ARGS.pack(k, *[256] * 10, *[stride] * 12, tokens, 4, pages, page, batch, n,
+                                                     layers, kv, hd, dt), None)
+
+    for name in ("rac_cache_append_async", "rac_cache_copy_pages_async", "rac_cache_compact_async"):
+        assert call(name, page=0) == -2 and call(name, kv=0) == -2 and call(name, dt=5) == -2
+        assert call(name, k=0) == -1 and getattr(L, name)(None, None) == -1
+        assert call(name, k=264) == -5 and call(name, hd=65) == -5 and call(name, stride=65) == -5
+    assert call("rac_cache_append_async", tokens=-1) == -2 and call("rac_cache_append_async", tokens=0) == 0
+    assert call("rac_cache_copy_pages_async", n=-1) == -2 and call("rac_cache_copy_pages_async", n=0) == 0
+    assert call("rac_cache_compact_async", n=65) == -2 and call("rac_cache_compact_async", batch=0) == 0
+
+
 # ── RACPagedCache: the accounts are the host's and need no GPU ─────────────
 
 @pytest.fixture
