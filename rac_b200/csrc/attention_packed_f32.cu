@@ -37,6 +37,7 @@ struct SplitArgs {
     float* delta;                          // [heads, tokens]
     const int* cu;
     int n_seqs;
+    int negate;                            // q's parts are those of -q (a negative scale: the kernels take its size)
     long long tokens;
 };
 
@@ -87,7 +88,7 @@ __global__ void __launch_bounds__(256) k_split(const SplitArgs a) {
     if (m > 0.f) frexpf(m, &e);            // m < 2^e
     e = max(14 - e, -112);
     e = min(e, 120);
-    const float f = ldexpf(1.f, e);
+    const float f = ldexpf(w == 0 && a.negate ? -1.f : 1.f, e);
     if (threadIdx.x == 0) a.factors[w][(long long)slot * a.heads[w] + h] = ldexpf(1.f, -e);
     __half* p = a.parts[w] + (t.start * 2 * a.heads[w] + h) * HD + lane * 4;
 #pragma unroll
@@ -113,7 +114,8 @@ struct Args {
     const int* cu;
     int n_seqs, heads, kv_heads, group, causal, zero_rest;
     long long tokens;
-    float c, scale;                        // scale * log2(e), scale
+    float c, scale;                        // |scale| log2(e), scale
+    int split;                             // dk, dv: one query head a block, to be added up
     const float *fq, *fk, *fv, *fg;        // factors
     const float *lse_in, *delta;
     float *out, *lse, *dq, *dk, *dv;
@@ -342,7 +344,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_fwd(const __grid_constant__
         const int w = warp >> 2, lr = (warp & 3) * 32 + lane, row = t.row0 + lr;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, ts = tS + lanes + 64 * w, to = tO + lanes + 128 * w;
         const float cq = a.c * a.fq[slot_of(t, t.row0) * a.heads + head];
-        const bool neg = a.c < 0.f;
         float o[HD], m = -INFINITY, l = 0.f;
 #pragma unroll
         for (int i = 0; i < HD; ++i) o[i] = 0.f;
@@ -354,19 +355,27 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_fwd(const __grid_constant__
             if (!ok) break;
             fence_after();
             const int lim = min(t.len, a.causal ? row + 1 : t.len) - j * kNarrow;     // keys below are seen
-            const bool part = lim < kNarrow;
-            const float hide = neg ? INFINITY : -INFINITY;
-            float y = hide;
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                uint32_t s[32];
-                ld32(s, ts + 32 * b);
+            const bool part = __any_sync(0xffffffffu, lim < kNarrow);
+            auto scores = [&](uint32_t (&x)[32], int b) {
+                ld32(x, ts + 32 * b);
                 wait_ld();
+                if (part) {
 #pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    const float x = part && 32 * b + i >= lim ? hide : __uint_as_float(s[i]);
-                    y = neg ? fminf(y, x) : fmaxf(y, x);
+                    for (int i = 0; i < 32; ++i)
+                        if (32 * b + i >= lim) x[i] = 0xff800000u;
                 }
+            };
+            // The scores are read twice, and the loops stay loops: what the warps run through
+            // for a tile has to stay in the instruction cache.
+            float y = -INFINITY;
+#pragma unroll 1
+            for (int b = 0; b < 2; ++b) {
+                uint32_t x[32];
+                scores(x, b);
+                float z[4] = {__uint_as_float(x[0]), __uint_as_float(x[1]), __uint_as_float(x[2]), __uint_as_float(x[3])};
+#pragma unroll
+                for (int i = 4; i < 32; ++i) z[i & 3] = fmaxf(z[i & 3], __uint_as_float(x[i]));
+                y = fmaxf(y, fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])));
             }
             const float top = y * c;
             // The reference point moves only when a weight would pass 2^8.
@@ -379,15 +388,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_fwd(const __grid_constant__
             }
             // Weights carry 2^6, which keeps their second parts above the smallest half.
             const float ref = m == -INFINITY ? 0.f : m - 6.f;
-#pragma unroll
+#pragma unroll 1
             for (int b = 0; b < 2; ++b) {
-                uint32_t s[32];
+                uint32_t x[32];
                 float p[32], add[4] = {0.f, 0.f, 0.f, 0.f};
-                ld32(s, ts + 32 * b);
-                wait_ld();
+                scores(x, b);
 #pragma unroll
                 for (int i = 0; i < 32; ++i) {
-                    p[i] = part && 32 * b + i >= lim ? 0.f : exp2_fast(fmaf(__uint_as_float(s[i]), c, -ref));
+                    p[i] = exp2_fast(fmaf(__uint_as_float(x[i]), c, -ref));
                     add[i & 3] += p[i];
                 }
                 l += (add[0] + add[1]) + (add[2] + add[3]);
@@ -482,12 +490,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_dkv(const __grid_constant__
     volatile int* gone = reinterpret_cast<volatile int*>(tmem_base + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-    const int kvh = blockIdx.x % a.kv_heads;
-    const PackedTile t = packed_tile(a.cu, a.n_seqs, a.tokens, kWide, blockIdx.x / a.kv_heads);
+    // Sums of a group's heads, or of one of them.
+    const int outs = a.split ? a.heads : a.kv_heads, each = a.split ? 1 : a.group;
+    const int oh = blockIdx.x % outs, kvh = a.split ? oh / a.group : oh, head0 = oh * each;
+    const PackedTile t = packed_tile(a.cu, a.n_seqs, a.tokens, kWide, blockIdx.x / outs);
     if (t.row0 >= t.len) return;
-    const long long out_row = (long long)a.kv_heads * HD;
-    float* dk = a.dk + (t.start * a.kv_heads + kvh) * HD;
-    float* dv = a.dv + (t.start * a.kv_heads + kvh) * HD;
+    const long long out_row = (long long)outs * HD;
+    float* dk = a.dk + (t.start * outs + oh) * HD;
+    float* dv = a.dv + (t.start * outs + oh) * HD;
     if (t.seq == a.n_seqs) {
         zero_rows_out(dk, out_row, HD, t.row0, t.len);
         zero_rows_out(dv, out_row, HD, t.row0, t.len);
@@ -495,7 +505,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_dkv(const __grid_constant__
     }
     const int first = a.causal ? t.row0 / kNarrow : 0;             // query tiles that see these keys
     const int nq = (t.len + kNarrow - 1) / kNarrow - first;
-    const int n = nq * a.group;
+    const int n = nq * each;
     const bool ragged = t.len % kNarrow != 0;                      // the last query tile of each head
 
     if (threadIdx.x == 0) {
@@ -513,7 +523,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_dkv(const __grid_constant__
     __syncthreads();
     fence_after();
     const uint32_t tm = *tmem_base, tS = tm, tP = tm + 64, tV = tm + 128, tK = tm + 256;
-    auto head_of = [&](int i) { return kvh * a.group + i / nq; };
+    auto head_of = [&](int i) { return head0 + i / nq; };
     auto row_of = [&](int i) { return (first + i % nq) * kNarrow; };
 
     if (warp >= 8) {
@@ -643,6 +653,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_dkv(const __grid_constant__
             if (!ok) break;
             fence_after();
             const int see = a.causal ? row - q0 - 32 * half : -1;          // columns from here on see this key
+            const bool part = __any_sync(0xffffffffu, see > 0);
             const float* lse = st_lse + sl * kNarrow + 32 * half;
             const float* dd = st_d + sl * kNarrow + 32 * half;
             float p[32];
@@ -651,8 +662,18 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_dkv(const __grid_constant__
                 ld32(s, s0);
                 wait_ld();
 #pragma unroll
-                for (int x = 0; x < 32; ++x)
-                    p[x] = x < see ? 0.f : exp2_fast(fmaf(__uint_as_float(s[x]), c, -lse[x]));
+                for (int x = 0; x < 32; x += 4) {
+                    const float4 z = *reinterpret_cast<const float4*>(lse + x);
+                    p[x] = exp2_fast(fmaf(__uint_as_float(s[x]), c, -z.x));
+                    p[x + 1] = exp2_fast(fmaf(__uint_as_float(s[x + 1]), c, -z.y));
+                    p[x + 2] = exp2_fast(fmaf(__uint_as_float(s[x + 2]), c, -z.z));
+                    p[x + 3] = exp2_fast(fmaf(__uint_as_float(s[x + 3]), c, -z.w));
+                }
+                if (part) {
+#pragma unroll
+                    for (int x = 0; x < 32; ++x)
+                        if (x < see) p[x] = 0.f;
+                }
                 put_parts(s0, p);
             }
             wait_st();
@@ -669,8 +690,18 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_dkv(const __grid_constant__
                 ld32(s, p0);
                 wait_ld();
 #pragma unroll
-                for (int x = 0; x < 32; ++x)
-                    p[x] = x < see ? 0.f : p[x] * fmaf(__uint_as_float(s[x]), acc_factor<HD>(), -dd[x]);
+                for (int x = 0; x < 32; x += 4) {
+                    const float4 z = *reinterpret_cast<const float4*>(dd + x);
+                    p[x] *= fmaf(__uint_as_float(s[x]), acc_factor<HD>(), -z.x);
+                    p[x + 1] *= fmaf(__uint_as_float(s[x + 1]), acc_factor<HD>(), -z.y);
+                    p[x + 2] *= fmaf(__uint_as_float(s[x + 2]), acc_factor<HD>(), -z.z);
+                    p[x + 3] *= fmaf(__uint_as_float(s[x + 3]), acc_factor<HD>(), -z.w);
+                }
+                if (part) {
+#pragma unroll
+                    for (int x = 0; x < 32; ++x)
+                        if (x < see) p[x] = 0.f;
+                }
                 put_parts(p0, p);
             }
             wait_st();
@@ -689,12 +720,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_dkv(const __grid_constant__
         if (ok) add_k(n - 1);
         if (ok && row < t.len) {
             if (HD == 32) {
-                store32((half ? dk : dv) + row * out_row, av, half ? a.scale : 1.f);
+                store32((half ? dk : dv) + row * out_row, av, half ? fabsf(a.scale) : 1.f);
             } else {
 #pragma unroll
                 for (int b = 0; b < W / 32; ++b) {
                     store32(dv + row * out_row + W * half + 32 * b, av + 32 * b, 1.f);
-                    store32(dk + row * out_row + W * half + 32 * b, ak + 32 * b, a.scale);
+                    store32(dk + row * out_row + W * half + 32 * b, ak + 32 * b, fabsf(a.scale));
                 }
             }
         }
@@ -863,8 +894,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_dq(const __grid_constant__ 
             ld32(s, p0);
             wait_ld();
 #pragma unroll
-            for (int x = 0; x < 32; ++x)
-                p[x] = x >= lim ? 0.f : p[x] * fmaf(__uint_as_float(s[x]), acc_factor<HD>(), -du);
+            for (int x = 0; x < 32; ++x) p[x] *= fmaf(__uint_as_float(s[x]), acc_factor<HD>(), -du);
+            if (__any_sync(0xffffffffu, lim < 32)) {
+#pragma unroll
+                for (int x = 0; x < 32; ++x)
+                    if (x >= lim) p[x] = 0.f;
+            }
             put_parts(s0, p);
             wait_st();
             fence_before();
@@ -884,14 +919,39 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_dq(const __grid_constant__ 
     if (threadIdx.x == 0 && *gone) atomicOr(a.err, kErrTcWait);
 }
 
+// dk and dv of a key/value head from those of its query heads, in their order.
+__global__ void __launch_bounds__(256) k_add_heads(const float* __restrict__ dk, const float* __restrict__ dv,
+                                                   float* __restrict__ ok, float* __restrict__ ov, int group, int hd,
+                                                   long long n) {
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;         // float4 of an output
+    if (i >= n) return;
+    const long long row = i / (hd / 4), c = i % (hd / 4);
+    for (int t = 0; t < 2; ++t) {
+        const float4* in = reinterpret_cast<const float4*>(t ? dv : dk) + row * group * (hd / 4) + c;
+        float4 s = in[0];
+        for (int g = 1; g < group; ++g) {
+            const float4 x = in[(long long)g * (hd / 4)];
+            s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
+        }
+        reinterpret_cast<float4*>(t ? ov : ok)[i] = s;
+    }
+}
+
 // ── launches ──────────────────────────────────────────────────────────────
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
-// Workspace: parts of q, k, v (and dO), their factors, and D.
+// Fewer blocks than twice the SMs leave some idle while others go through a whole
+// group: then each query head has a block of its own.  2048 tokens of 16 heads (4
+// key/value heads): 64 busy blocks 181 us, 256 of them MEASURED us with the sums.
+bool by_head(long long tokens, int heads, int kv_heads) {
+    return heads > kv_heads && tokens / kWide * kv_heads < 2 * 148;
+}
+
+// Workspace: parts of q, k, v (and dO), their factors, D, and dk and dv by query head.
 struct Room {
     __half* parts[4];
     float* factors[4];
-    float* delta;
+    float *delta, *dk, *dv;
     size_t bytes;
 };
 Room room(void* ws, long long tokens, int n_seqs, int heads, int kv_heads, int hd, int backward) {
@@ -910,6 +970,12 @@ Room room(void* ws, long long tokens, int n_seqs, int heads, int kv_heads, int h
     }
     r.delta = reinterpret_cast<float*>(p + at);
     if (backward) at += up256((size_t)tokens * heads * sizeof(float));
+    if (backward && by_head(tokens, heads, kv_heads)) {
+        r.dk = reinterpret_cast<float*>(p + at);
+        at += up256((size_t)tokens * heads * hd * sizeof(float));
+        r.dv = reinterpret_cast<float*>(p + at);
+        at += up256((size_t)tokens * heads * hd * sizeof(float));
+    }
     r.bytes = at;
     return r;
 }
@@ -932,7 +998,7 @@ int launch(const PackedParams& p, const Room& r, Args& a, bool backward, cudaStr
         sp.parts[i] = r.parts[i]; sp.factors[i] = r.factors[i];
     }
     sp.out = static_cast<const float*>(p.out_in); sp.delta = r.delta;
-    sp.cu = p.cu; sp.n_seqs = p.n_seqs; sp.tokens = p.tokens;
+    sp.negate = p.scale < 0.f; sp.cu = p.cu; sp.n_seqs = p.n_seqs; sp.tokens = p.tokens;
     const unsigned slots = (unsigned)packed_slots(p.tokens, p.n_seqs, kSplit);
     k_split<HD><<<slots * sp.first[4], 256, 0, s>>>(sp);
     if (cudaGetLastError() != cudaSuccess) return kErrCuda;
@@ -942,7 +1008,15 @@ int launch(const PackedParams& p, const Room& r, Args& a, bool backward, cudaStr
         return cudaGetLastError() == cudaSuccess ? kOk : kErrCuda;
     };
     if (!backward) return go(&k_f32_fwd<HD>, FwdShape<HD>::SMEM, slots * p.heads);
-    if (int st = go(&k_f32_dkv<HD>, BwdShape<HD>::SMEM, slots * p.kv_heads)) return st;
+    a.split = by_head(p.tokens, p.heads, p.kv_heads);
+    if (a.split) { a.dk = r.dk; a.dv = r.dv; }
+    if (int st = go(&k_f32_dkv<HD>, BwdShape<HD>::SMEM, slots * (a.split ? p.heads : p.kv_heads))) return st;
+    if (a.split) {
+        const long long n = p.tokens * p.kv_heads * (HD / 4);
+        k_add_heads<<<(unsigned)((n + 255) / 256), 256, 0, s>>>(r.dk, r.dv, static_cast<float*>(p.dk),
+                                                                static_cast<float*>(p.dv), a.group, HD, n);
+        if (cudaGetLastError() != cudaSuccess) return kErrCuda;
+    }
     return go(&k_f32_dq<HD>, BwdShape<HD>::SMEM, slots * p.heads);
 }
 
@@ -965,7 +1039,7 @@ int attention_packed_f32(const PackedParams& p, int backward, cudaStream_t s) {
     a.cu = p.cu; a.n_seqs = p.n_seqs; a.heads = p.heads; a.kv_heads = p.kv_heads; a.group = p.heads / p.kv_heads;
     a.causal = p.causal; a.zero_rest = p.zero_rest; a.tokens = p.tokens;
     // 0 would turn a hidden score's infinity into NaN; 1e-30 weighs the rest alike.
-    a.c = p.scale == 0.f ? 1e-30f : p.scale * kLog2e;
+    a.c = p.scale == 0.f ? 1e-30f : fabsf(p.scale) * kLog2e;
     a.scale = p.scale;
     a.fq = r.factors[0]; a.fk = r.factors[1]; a.fv = r.factors[2]; a.fg = r.factors[3];
     a.lse_in = p.lse_in; a.delta = r.delta;

@@ -48,14 +48,22 @@ __global__ void __launch_bounds__(256) k_cache_append(const AppendArgs a) {
         return;
     }
     const long long slot = row % a.page_size;
-    for (int e = lane; e < 2 * a.kv_heads * a.vecs; e += 32) {
-        const int c = e % a.vecs, hk = e / a.vecs, h = hk >> 1;
-        if (hk & 1)
-            *reinterpret_cast<uint4*>(a.v.p + pg * a.v.page + h * a.v.head + slot * a.v.row + c * 16) =
-                *reinterpret_cast<const uint4*>(a.nv + tok * a.nv_row + h * a.nv_head + c * 16);
-        else
-            *reinterpret_cast<uint4*>(a.k.p + pg * a.k.page + h * a.k.head + slot * a.k.row + c * 16) =
-                *reinterpret_cast<const uint4*>(a.nk + tok * a.nk_row + h * a.nk_head + c * 16);
+    const char *sk = a.nk + tok * a.nk_row, *sv = a.nv + tok * a.nv_row;
+    char *dk = a.k.p + pg * a.k.page + slot * a.k.row, *dv = a.v.p + pg * a.v.page + slot * a.v.row;
+    // Eight units a lane are read before the first is written: one trip to memory, not eight.
+    const int n = 2 * a.kv_heads * a.vecs;
+    for (int e0 = lane; e0 < n; e0 += 8 * 32) {
+        uint4 x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int e = e0 + 32 * i, hk = e / a.vecs, c = e - hk * a.vecs, h = hk >> 1;
+            if (e < n) x[i] = *reinterpret_cast<const uint4*>(hk & 1 ? sv + h * a.nv_head + c * 16 : sk + h * a.nk_head + c * 16);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int e = e0 + 32 * i, hk = e / a.vecs, c = e - hk * a.vecs, h = hk >> 1;
+            if (e < n) *reinterpret_cast<uint4*>(hk & 1 ? dv + h * a.v.head + c * 16 : dk + h * a.k.head + c * 16) = x[i];
+        }
     }
 }
 
@@ -66,7 +74,9 @@ struct CopyArgs {
     unsigned int* err;
 };
 
-// Grid (parts of a page, page, layer and tensor).
+// Grid (parts of a page, page, layer and tensor).  A thread reads eight units
+// before it writes the first.  FLAT: the page is one run of memory.
+template <bool FLAT>
 __global__ void __launch_bounds__(256) k_cache_copy(const CopyArgs a) {
     const Units& x = a.x[blockIdx.z & 1];
     const long long layer = blockIdx.z >> 1;
@@ -78,11 +88,19 @@ __global__ void __launch_bounds__(256) k_cache_copy(const CopyArgs a) {
     const char* s = x.p + layer * x.layer + from * x.page;
     char* d = x.p + layer * x.layer + to * x.page;
     const int n = a.rows * a.heads * a.vecs;
-    for (int e = blockIdx.x * 256 + threadIdx.x; e < n; e += gridDim.x * 256) {
-        const int c = e % a.vecs, r = e / a.vecs;
-        const long long at = (r / a.rows) * x.head + (r % a.rows) * x.row + c * 16;
-        *reinterpret_cast<uint4*>(d + at) = *reinterpret_cast<const uint4*>(s + at);
-    }
+    auto place = [&](int e) -> long long {
+        if (FLAT) return (long long)e * 16;
+        const int r = e / a.vecs, c = e - r * a.vecs, h = r / a.rows;
+        return h * x.head + (r - h * a.rows) * x.row + c * 16;
+    };
+    const int e0 = blockIdx.x * 2048 + threadIdx.x;
+    uint4 u[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (e0 + 256 * i < n) u[i] = __ldcs(reinterpret_cast<const uint4*>(s + place(e0 + 256 * i)));
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (e0 + 256 * i < n) __stcs(reinterpret_cast<uint4*>(d + place(e0 + 256 * i)), u[i]);
 }
 
 struct CompactArgs {
@@ -180,7 +198,10 @@ int cache_copy_pages(const CopyPagesParams& p, cudaStream_t s) {
     const long long vecs = (long long)a.rows * a.heads * a.vecs;
     if (vecs >= (1LL << 31)) return kErrInvalidDim;
     const unsigned parts = (unsigned)((vecs + 2047) / 2048);
-    k_cache_copy<<<dim3(parts, p.n, 2 * p.layers), 256, 0, s>>>(a);
+    const dim3 grid(parts, p.n, 2 * p.layers);
+    const auto flat = [&](const Pages& x) { return x.row == p.head_dim && x.head == (long long)p.page_size * x.row; };
+    if (flat(p.k) && flat(p.v)) k_cache_copy<true><<<grid, 256, 0, s>>>(a);
+    else k_cache_copy<false><<<grid, 256, 0, s>>>(a);
     return launched();
 }
 
