@@ -12,7 +12,7 @@
 // The tensor core adds into its 32-bit sums by cutting off (measured: 1e-7 of
 // the sum for each instruction of 16 summed values, all in one direction, so
 // that 1024 of them lose 1e-4).  So a sum in tensor memory is never carried on
-// from one tile of 64 to the next: it is added to 32-bit registers, rounded to
+// from one tile to the next: it is added to 32-bit registers, rounded to
 // nearest, where the tile's factor is applied as well.  Within a product the
 // small parts come first.
 #include "attn_common.cuh"
@@ -25,7 +25,11 @@ using namespace tc;
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kSplit = 128;                // rows that share a factor
-constexpr int kWide = 128, kNarrow = 64;   // rows of the tile that stays and of those that pass by
+constexpr int kWide = 128, kBoxRows = 64;  // rows of a tile that stays in place, of a TMA box
+// A product of 64 columns takes the matrix unit as long as one of 128 (64 cycles
+// an instruction), so that the tiles that pass by have 128 rows as well, except
+// in the backward kernels at dim 128, which have no room for them.
+template <int HD> constexpr int narrow() { return HD == 128 ? 64 : 128; }
 
 // ── parts ─────────────────────────────────────────────────────────────────
 struct SplitArgs {
@@ -117,6 +121,7 @@ struct Args {
     float c, scale;                        // |scale| log2(e), scale
     int split;                             // dk, dv: one query head a block, to be added up
     const float *fq, *fk, *fv, *fg;        // factors
+    const __half *pq, *pk, *pv, *pg;       // parts
     const float *lse_in, *delta;
     float *out, *lse, *dq, *dk, *dv;
     unsigned int* err;
@@ -127,11 +132,11 @@ struct Shape {
     static constexpr int SW = HD * 2 < 128 ? HD * 2 : 128;
     static constexpr int BOXES = HD * 2 / SW;
     // A part of a tile: its boxes of all rows; the other part behind it.
-    static constexpr int PART64 = kNarrow * HD * 2, PART128 = kWide * HD * 2;
-    static constexpr int TILE64 = 2 * PART64, TILE128 = 2 * PART128;
+    static constexpr int part(int rows) { return rows * HD * 2; }
+    static constexpr int tile(int rows) { return 2 * rows * HD * 2; }
 };
 
-// One part-pair of a tile of ROWS rows (64 or 128): boxes [rows, SW] one after another.
+// Both parts of a tile of ROWS rows (64 or 128): boxes [rows, SW] one after another.
 template <int HD, int ROWS>
 __device__ __forceinline__ void load_parts(uint8_t* dst, const CUtensorMap* m, int head, int heads, int row, uint64_t* bar) {
     using Sh = Shape<HD>;
@@ -140,51 +145,79 @@ __device__ __forceinline__ void load_parts(uint8_t* dst, const CUtensorMap* m, i
 #pragma unroll
         for (int b = 0; b < Sh::BOXES; ++b)
 #pragma unroll
-            for (int r = 0; r < ROWS; r += kNarrow)
+            for (int r = 0; r < ROWS; r += kBoxRows)
                 load_3d(dst + part * ROWS * HD * 2 + (b * ROWS + r) * Sh::SW, m, b * (Sh::SW / 2), part * heads + head,
                         row + r, bar);
 }
 
-// Rows [r0, 64) of both parts become zeros, by one warp.
-template <int HD>
+// Rows [r0, ROWS) of both parts become zeros, by one warp.
+template <int HD, int ROWS>
 __device__ __forceinline__ void zero_parts(uint8_t* tile, int r0) {
     using Sh = Shape<HD>;
-    const int n = (kNarrow - r0) * (Sh::SW / 16), lane = threadIdx.x & 31;
+    const int n = (ROWS - r0) * (Sh::SW / 16), lane = threadIdx.x & 31;
     for (int e = lane; e < n * Sh::BOXES * 2; e += 32)
-        *reinterpret_cast<uint4*>(tile + (e / n) * kNarrow * Sh::SW + r0 * Sh::SW + (e % n) * 16) = make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(tile + (e / n) * ROWS * Sh::SW + r0 * Sh::SW + (e % n) * 16) = make_uint4(0, 0, 0, 0);
 }
 
-// D = A B^T over HD: A 128 rows, B 64 rows, both in parts.
-template <int HD>
+// D = A B^T over HD: A 128 rows, B N rows, both in parts.
+template <int HD, int N>
 __device__ __forceinline__ void parts_rows(uint32_t d, uint32_t a, uint32_t b) {
     using Sh = Shape<HD>;
-    constexpr uint32_t instr = instruction<__half>(kWide, kNarrow, false);
+    constexpr uint32_t instr = instruction<__half>(kWide, N, false);
 #pragma unroll
     for (int t = 0; t < 3; ++t) {          // lo hi, hi lo, hi hi
-        const uint64_t da = operand<Sh::SW>(a + (t == 0 ? Sh::PART128 : 0), 16, 8 * Sh::SW);
-        const uint64_t db = operand<Sh::SW>(b + (t == 1 ? Sh::PART64 : 0), 16, 8 * Sh::SW);
+        const uint64_t da = operand<Sh::SW>(a + (t == 0 ? Sh::part(kWide) : 0), 16, 8 * Sh::SW);
+        const uint64_t db = operand<Sh::SW>(b + (t == 1 ? Sh::part(N) : 0), 16, 8 * Sh::SW);
 #pragma unroll
         for (int k = 0; k < HD; k += 16)
             mma_ss(d, da + (((k * 2 / Sh::SW) * kWide * Sh::SW + (k * 2) % Sh::SW) >> 4),
-                   db + (((k * 2 / Sh::SW) * kNarrow * Sh::SW + (k * 2) % Sh::SW) >> 4), instr, t > 0 || k > 0);
+                   db + (((k * 2 / Sh::SW) * N * Sh::SW + (k * 2) % Sh::SW) >> 4), instr, t > 0 || k > 0);
     }
 }
-// D = W B: W [128, 64] in tensor memory, for each 32 columns 16 of hi and 16 of
-// lo; B 64 rows in parts, summed over.
+// The same with A's rows in tensor memory: HD / 2 columns of hi, then of lo.
+template <int HD, int N>
+__device__ __forceinline__ void parts_rows_t(uint32_t d, uint32_t a, uint32_t b) {
+    using Sh = Shape<HD>;
+    constexpr uint32_t instr = instruction<__half>(kWide, N, false);
+#pragma unroll
+    for (int t = 0; t < 3; ++t) {
+        const uint64_t db = operand<Sh::SW>(b + (t == 1 ? Sh::part(N) : 0), 16, 8 * Sh::SW);
+#pragma unroll
+        for (int k = 0; k < HD; k += 16)
+            mma_ts(d, a + (t == 0 ? HD / 2 : 0) + k / 2, db + (((k * 2 / Sh::SW) * N * Sh::SW + (k * 2) % Sh::SW) >> 4),
+                   instr, t > 0 || k > 0);
+    }
+}
+// One part of a row, from global memory to the HD / 2 columns at addr of the thread's lane.
 template <int HD>
+__device__ __forceinline__ void put_row(uint32_t addr, const __half* row, bool live) {
+#pragma unroll
+    for (int b = 0; b < HD / 32; ++b) {
+        uint32_t x[16];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint4 u = live ? *reinterpret_cast<const uint4*>(row + 32 * b + 8 * i) : make_uint4(0, 0, 0, 0);
+            x[4 * i] = u.x; x[4 * i + 1] = u.y; x[4 * i + 2] = u.z; x[4 * i + 3] = u.w;
+        }
+        st16(addr + 16 * b, x);
+    }
+}
+// D = W B: W [128, N] in tensor memory, for each 32 columns 16 of hi and 16 of
+// lo; B N rows in parts, summed over.
+template <int HD, int N>
 __device__ __forceinline__ void parts_weights(uint32_t d, uint32_t w, uint32_t b) {
     using Sh = Shape<HD>;
     constexpr uint32_t instr = instruction<__half>(kWide, HD, true);
 #pragma unroll
     for (int t = 0; t < 3; ++t) {
-        const uint64_t db = operand<Sh::SW>(b + (t == 1 ? Sh::PART64 : 0), kNarrow * Sh::SW, 8 * Sh::SW);
+        const uint64_t db = operand<Sh::SW>(b + (t == 1 ? Sh::part(N) : 0), N * Sh::SW, 8 * Sh::SW);
 #pragma unroll
-        for (int k = 0; k < kNarrow; k += 16)
+        for (int k = 0; k < N; k += 16)
             mma_ts(d, w + (k / 32) * 32 + (k % 32) / 2 + (t == 0 ? 16 : 0), db + (k * Sh::SW >> 4), instr, t > 0 || k > 0);
     }
 }
 // 32 weights of a row as parts, to the columns that parts_weights reads.
-__device__ __forceinline__ void put_parts(uint32_t addr, const float (&p)[32]) {
+__device__ __forceinline__ void put_parts(uint32_t addr, const float* p) {
     uint32_t hi[16], lo[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
@@ -223,15 +256,17 @@ static_assert(kMathRegs * 256 + kOtherRegs * 128 <= kLaunchRegs * kThreads, "reg
 // Slot (of 128 rows) of a row of a sequence.
 __device__ __forceinline__ long long slot_of(const PackedTile& t, int row) { return t.start / kSplit + t.seq + row / kSplit; }
 
+constexpr int kKeysF32 = 128;              // keys of a tile, forward
+
 // ── forward ───────────────────────────────────────────────────────────────
 // The warpgroups take the key tiles in turn, each with its own scores, its own
 // reference point and its own sum in registers; the two join at the end.
 template <int HD>
 struct FwdShape {
     using Sh = Shape<HD>;
-    static constexpr int STAGES = HD == 128 ? 4 : HD == 64 ? 8 : 12;
-    static constexpr int BARS = Sh::TILE128 + STAGES * Sh::TILE64, SMEM = BARS + 512;
-    static_assert(STAGES * Sh::TILE64 >= kWide * (HD + 1) * 4 + kWide * 8, "room to join");
+    static constexpr int STAGES = HD == 128 ? 3 : 6, TILE = Sh::tile(kWide);
+    static constexpr int BARS = STAGES * TILE, SMEM = BARS + 512;
+    static_assert(STAGES * TILE >= kWide * (HD + 1) * 4 + kWide * 8, "room to join");
     static_assert(SMEM <= 227 * 1024, "shared memory");
 };
 
@@ -239,12 +274,12 @@ template <int HD>
 __global__ void __launch_bounds__(kThreads, 1) k_f32_fwd(const __grid_constant__ Args a) {
     using Sh = Shape<HD>;
     using Fs = FwdShape<HD>;
-    constexpr int ST = Fs::STAGES;
+    constexpr int ST = Fs::STAGES, TILE = Fs::TILE;
     extern __shared__ __align__(1024) uint8_t sm[];
-    uint8_t *qs = sm, *ring = sm + Sh::TILE128;
+    uint8_t* ring = sm;
     uint64_t* bars = reinterpret_cast<uint64_t*>(sm + Fs::BARS);
     uint64_t *full = bars, *empty = full + ST, *q_full = empty + ST, *fixed = q_full + 1, *s_ready = fixed + 1,
-             *p_ready = s_ready + 2, *o_ready = p_ready + 2, *joined = o_ready + 2;
+             *p_ready = s_ready + 2, *o_ready = p_ready + 2, *o_taken = o_ready + 2, *joined = o_taken + 1;
     uint32_t* tmem_base = reinterpret_cast<uint32_t*>(joined + 1);
     volatile int* gone = reinterpret_cast<volatile int*>(tmem_base + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -259,13 +294,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_fwd(const __grid_constant__
         return;
     }
     const int last = a.causal ? min(t.row0 + kWide, t.len) : t.len;
-    const int n = (last + kNarrow - 1) / kNarrow;
-    const bool ragged = n * kNarrow > t.len;
+    const int n = (last + kKeysF32 - 1) / kKeysF32;
+    const bool ragged = n * kKeysF32 > t.len;
 
     if (threadIdx.x == 0) {
         *gone = 0;
         for (int i = 0; i < ST; ++i) { bar_init(full + i, 1); bar_init(empty + i, 1); }
-        bar_init(q_full, 1); bar_init(fixed, 1); bar_init(joined, 128);
+        bar_init(q_full, 256); bar_init(fixed, 1); bar_init(joined, 128); bar_init(o_taken, 128);
         for (int w = 0; w < 2; ++w) { bar_init(s_ready + w, 1); bar_init(p_ready + w, 128); bar_init(o_ready + w, 1); }
         bar_init_done();
     }
@@ -273,7 +308,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_fwd(const __grid_constant__
     fence_before();
     __syncthreads();
     fence_after();
-    const uint32_t tm = *tmem_base, tS = tm, tO = tm + 256;    // S: 64 columns each, O: 128 each
+    const uint32_t tm = *tmem_base, tS = tm, tO = tm + 256, tQ = tm + 384;     // S twice; O; Q: both parts
 
     // The ring holds K0, K1, V0, K2, V1, K3, ...: entry of K_j, of V_j.
     auto k_entry = [](int j) { return j < 2 ? j : 2 * j - 1; };
@@ -284,16 +319,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_fwd(const __grid_constant__
         if (warp == 9) {
             if (lane == 0) {
                 const int r0 = (int)t.start;
-                bar_expect(q_full, Sh::TILE128);
-                load_parts<HD, kWide>(qs, &a.q, head, a.heads, r0 + t.row0, q_full);
                 int e = 0;
                 bool ok = true;
                 auto load = [&](const CUtensorMap* m, int j) {
                     const int st = e % ST;
                     if (e >= ST) ok = bar_wait(empty + st, (e / ST - 1) & 1, gone);
                     if (!ok) return;
-                    bar_expect(full + st, Sh::TILE64);
-                    load_parts<HD, kNarrow>(ring + st * Sh::TILE64, m, kvh, a.kv_heads, r0 + j * kNarrow, full + st);
+                    bar_expect(full + st, TILE);
+                    load_parts<HD, kKeysF32>(ring + st * TILE, m, kvh, a.kv_heads, r0 + j * kKeysF32, full + st);
                     ++e;
                 };
                 load(&a.k, 0);
@@ -307,7 +340,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_fwd(const __grid_constant__
             if (ragged) {
                 const int e = v_entry(n - 1), st = e % ST;
                 if (bar_wait(full + st, (e / ST) & 1, gone)) {
-                    zero_parts<HD>(ring + st * Sh::TILE64, t.len - (n - 1) * kNarrow);
+                    zero_parts<HD, kKeysF32>(ring + st * TILE, t.len - (n - 1) * kKeysF32);
                     fence_async_smem();
                 }
                 __syncwarp();
@@ -318,20 +351,25 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_fwd(const __grid_constant__
                 auto scores = [&](int j) {
                     const int e = k_entry(j), st = e % ST;
                     if (!bar_wait(full + st, (e / ST) & 1, gone)) return false;
-                    parts_rows<HD>(tS + 64 * (j & 1), smem(qs), smem(ring + st * Sh::TILE64));
+                    parts_rows_t<HD, kKeysF32>(tS + 128 * (j & 1), tQ, smem(ring + st * TILE));
                     commit(s_ready + (j & 1));
                     commit(empty + st);
                     return true;
                 };
-                bool ok = bar_wait(q_full, 0, gone) && scores(0);
+                bool ok = bar_wait(q_full, 0, gone);
+                fence_after();
+                ok = ok && scores(0);
                 if (ok && n > 1) ok = scores(1);
                 for (int j = 0; ok && j < n; ++j) {
                     const int e = v_entry(j), st = e % ST, w = j & 1;
                     ok = bar_wait(full + st, (e / ST) & 1, gone) && (!(ragged && j == n - 1) || bar_wait(fixed, 0, gone)) &&
                          bar_wait(p_ready + w, (j >> 1) & 1, gone);
                     if (!ok) break;
+                    // One block of sums: the other warpgroup has to have taken the last.
+                    if (j) ok = bar_wait(o_taken, (j - 1) & 1, gone);
+                    if (!ok) break;
                     fence_after();
-                    parts_weights<HD>(tO + 128 * w, tS + 64 * w, smem(ring + st * Sh::TILE64));
+                    parts_weights<HD, kKeysF32>(tO, tS + 128 * w, smem(ring + st * TILE));
                     commit(o_ready + w);
                     commit(empty + st);
                     if (j + 2 < n) ok = scores(j + 2);
@@ -342,20 +380,24 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_fwd(const __grid_constant__
     } else {
         more_registers<kMathRegs>();
         const int w = warp >> 2, lr = (warp & 3) * 32 + lane, row = t.row0 + lr;
-        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, ts = tS + lanes + 64 * w, to = tO + lanes + 128 * w;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, ts = tS + lanes + 128 * w, to = tO + lanes;
+        put_row<HD>(tQ + lanes + w * (HD / 2), a.pq + ((t.start + row) * 2 * a.heads + w * a.heads + head) * HD, row < t.len);
+        wait_st();
+        fence_before();
+        bar_arrive(q_full);
         const float cq = a.c * a.fq[slot_of(t, t.row0) * a.heads + head];
         float o[HD], m = -INFINITY, l = 0.f;
 #pragma unroll
         for (int i = 0; i < HD; ++i) o[i] = 0.f;
         bool ok = true;
         for (int j = w; j < n; j += 2) {
-            const long long ks = slot_of(t, j * kNarrow) * a.kv_heads + kvh;
+            const long long ks = slot_of(t, j * kKeysF32) * a.kv_heads + kvh;
             const float c = cq * a.fk[ks], fv = a.fv[ks];
             ok = __all_sync(0xffffffffu, bar_wait(s_ready + w, (j >> 1) & 1, gone));
             if (!ok) break;
             fence_after();
-            const int lim = min(t.len, a.causal ? row + 1 : t.len) - j * kNarrow;     // keys below are seen
-            const bool part = __any_sync(0xffffffffu, lim < kNarrow);
+            const int lim = min(t.len, a.causal ? row + 1 : t.len) - j * kKeysF32;     // keys below are seen
+            const bool part = __any_sync(0xffffffffu, lim < kKeysF32);
             auto scores = [&](uint32_t (&x)[32], int b) {
                 ld32(x, ts + 32 * b);
                 wait_ld();
@@ -369,7 +411,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_fwd(const __grid_constant__
             // for a tile has to stay in the instruction cache.
             float y = -INFINITY;
 #pragma unroll 1
-            for (int b = 0; b < 2; ++b) {
+            for (int b = 0; b < kKeysF32 / 32; ++b) {
                 uint32_t x[32];
                 scores(x, b);
                 float z[4] = {__uint_as_float(x[0]), __uint_as_float(x[1]), __uint_as_float(x[2]), __uint_as_float(x[3])};
@@ -389,7 +431,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_fwd(const __grid_constant__
             // Weights carry 2^6, which keeps their second parts above the smallest half.
             const float ref = m == -INFINITY ? 0.f : m - 6.f;
 #pragma unroll 1
-            for (int b = 0; b < 2; ++b) {
+            for (int b = 0; b < kKeysF32 / 32; ++b) {
                 uint32_t x[32];
                 float p[32], add[4] = {0.f, 0.f, 0.f, 0.f};
                 scores(x, b);
@@ -409,6 +451,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_fwd(const __grid_constant__
             fence_after();
 #pragma unroll
             for (int b = 0; b < HD / 32; ++b) take32(o + 32 * b, to + 32 * b, fv);
+            fence_before();
+            bar_arrive(o_taken);
         }
         // All products are done when both warpgroups are through: the ring is free.
         float* jo = reinterpret_cast<float*>(ring);
@@ -464,23 +508,24 @@ template <int HD>
 struct BwdShape {
     using Sh = Shape<HD>;
     // Places of Q (dk/dv) or K (dq), which a later product reads again, and of dO or V.
-    static constexpr int A = HD == 128 ? 2 : 3, B = HD == 128 ? 1 : 3;
-    static constexpr int RING = 2 * Sh::TILE128, STAT = RING + (A + B) * Sh::TILE64, BARS = STAT + 2 * 2 * kNarrow * 4;
+    static constexpr int A = HD == 32 ? 3 : 2, B = HD == 128 ? 1 : 2;
+    static constexpr int N = narrow<HD>(), TILE = Sh::tile(N), KEPT = Sh::tile(kWide);
+    static constexpr int RING = 2 * KEPT, STAT = RING + (A + B) * TILE, BARS = STAT + 2 * 2 * N * 4;
     static constexpr int SMEM = BARS + 512;
     static_assert(SMEM <= 227 * 1024, "shared memory");
 };
 
-// dk and dv of 128 keys: query tiles of 64 pass by, of all heads of the group.
+// dk and dv of 128 keys: query tiles pass by, of all heads of the group.
 // The order is dV(i), S(i+1), dK(i), dP(i+1); P(i) lies in S(i)'s columns, dS(i) in dP(i)'s.
 template <int HD>
 __global__ void __launch_bounds__(kThreads, 1) k_f32_dkv(const __grid_constant__ Args a) {
     using Sh = Shape<HD>;
     using Bs = BwdShape<HD>;
-    constexpr int NA = Bs::A, NB = Bs::B;
+    constexpr int NA = Bs::A, NB = Bs::B, N = Bs::N, TILE = Bs::TILE, C = N / 2;
     extern __shared__ __align__(1024) uint8_t sm[];
-    uint8_t *ks = sm, *vs = sm + Sh::TILE128, *qr = sm + Bs::RING, *gr = qr + NA * Sh::TILE64;
+    uint8_t *ks = sm, *vs = sm + Bs::KEPT, *qr = sm + Bs::RING, *gr = qr + NA * TILE;
     float* st_lse = reinterpret_cast<float*>(sm + Bs::STAT);       // [2][64]
-    float* st_d = st_lse + 2 * kNarrow;
+    float* st_d = st_lse + 2 * N;
     uint64_t* bars = reinterpret_cast<uint64_t*>(sm + Bs::BARS);
     uint64_t *q_full = bars, *q_empty = q_full + NA, *q_fixed = q_empty + NA, *g_full = q_fixed + NA, *g_empty = g_full + NB,
              *g_fixed = g_empty + NB, *kv_full = g_fixed + NB, *stat_full = kv_full + 1,
@@ -503,10 +548,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_dkv(const __grid_constant__
         zero_rows_out(dv, out_row, HD, t.row0, t.len);
         return;
     }
-    const int first = a.causal ? t.row0 / kNarrow : 0;             // query tiles that see these keys
-    const int nq = (t.len + kNarrow - 1) / kNarrow - first;
+    const int first = a.causal ? t.row0 / N : 0;             // query tiles that see these keys
+    const int nq = (t.len + N - 1) / N - first;
     const int n = nq * each;
-    const bool ragged = t.len % kNarrow != 0;                      // the last query tile of each head
+    const bool ragged = t.len % N != 0;                      // the last query tile of each head
 
     if (threadIdx.x == 0) {
         *gone = 0;
@@ -522,9 +567,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_dkv(const __grid_constant__
     fence_before();
     __syncthreads();
     fence_after();
-    const uint32_t tm = *tmem_base, tS = tm, tP = tm + 64, tV = tm + 128, tK = tm + 256;
+    const uint32_t tm = *tmem_base, tS = tm, tP = tm + N, tV = tm + 2 * N, tK = tV + (HD == 128 ? 128 : 64);
     auto head_of = [&](int i) { return head0 + i / nq; };
-    auto row_of = [&](int i) { return (first + i % nq) * kNarrow; };
+    auto row_of = [&](int i) { return (first + i % nq) * N; };
 
     if (warp >= 8) {
         fewer_registers<kOtherRegs>();
@@ -532,22 +577,22 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_dkv(const __grid_constant__
             // `fixed` tells that the rows behind the sequence are cleared (their weights
             // are 0, 0 times another sequence's NaN is not).
             if (lane == 0) {
-                bar_expect(kv_full, 2 * Sh::TILE128);
+                bar_expect(kv_full, 2 * Bs::KEPT);
                 load_parts<HD, kWide>(ks, &a.k, kvh, a.kv_heads, (int)t.start + t.row0, kv_full);
                 load_parts<HD, kWide>(vs, &a.v, kvh, a.kv_heads, (int)t.start + t.row0, kv_full);
             }
             auto load = [&](const CUtensorMap* m, int i, uint8_t* r, uint64_t* full, uint64_t* empty, uint64_t* fixed, int n_places) {
                 const int st = i % n_places;
-                uint8_t* dst = r + st * Sh::TILE64;
+                uint8_t* dst = r + st * TILE;
                 if (!__all_sync(0xffffffffu, i < n_places || bar_wait(empty + st, (i / n_places - 1) & 1, gone))) return false;
                 if (lane == 0) {
-                    bar_expect(full + st, Sh::TILE64);
-                    load_parts<HD, kNarrow>(dst, m, head_of(i), a.heads, (int)t.start + row_of(i), full + st);
+                    bar_expect(full + st, TILE);
+                    load_parts<HD, N>(dst, m, head_of(i), a.heads, (int)t.start + row_of(i), full + st);
                 }
                 __syncwarp();
                 if (ragged && i % nq == nq - 1) {
                     if (!__all_sync(0xffffffffu, bar_wait(full + st, (i / n_places) & 1, gone))) return false;
-                    zero_parts<HD>(dst, t.len % kNarrow);
+                    zero_parts<HD, N>(dst, t.len % N);
                     fence_async_smem();
                     __syncwarp();
                 }
@@ -561,14 +606,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_dkv(const __grid_constant__
                 auto scores = [&](int i) {
                     const int st = i % NA;
                     if (!bar_wait(q_full + st, (i / NA) & 1, gone) || !bar_wait(q_fixed + st, (i / NA) & 1, gone)) return false;
-                    parts_rows<HD>(tS, smem(ks), smem(qr + st * Sh::TILE64));
+                    parts_rows<HD, N>(tS, smem(ks), smem(qr + st * TILE));
                     commit(s_ready);
                     return true;
                 };
                 auto dps = [&](int i) {
                     const int st = i % NB;
                     if (!bar_wait(g_full + st, (i / NB) & 1, gone) || !bar_wait(g_fixed + st, (i / NB) & 1, gone)) return false;
-                    parts_rows<HD>(tP, smem(vs), smem(gr + st * Sh::TILE64));
+                    parts_rows<HD, N>(tP, smem(vs), smem(gr + st * TILE));
                     commit(dp_ready);
                     return true;
                 };
@@ -578,13 +623,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_dkv(const __grid_constant__
                     ok = bar_wait(p_ready, i & 1, gone);
                     if (!ok) break;
                     fence_after();
-                    parts_weights<HD>(tV, tS, smem(gr + (i % NB) * Sh::TILE64));
+                    parts_weights<HD, N>(tV, tS, smem(gr + (i % NB) * TILE));
                     commit(dv_done);
                     commit(g_empty + i % NB);
                     ok = (!more || scores(i + 1)) && bar_wait(ds_ready, i & 1, gone);
                     if (!ok) break;
                     fence_after();
-                    parts_weights<HD>(tK, tP, smem(qr + (i % NA) * Sh::TILE64));
+                    parts_weights<HD, N>(tK, tP, smem(qr + (i % NA) * TILE));
                     commit(dk_done);
                     commit(q_empty + i % NA);
                     ok = !more || dps(i + 1);
@@ -598,7 +643,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_dkv(const __grid_constant__
                 const bool ok = i < 2 || bar_wait(stat_empty + sl, (i / 2 - 1) & 1, gone);
                 if (!__all_sync(0xffffffffu, ok)) break;
                 const float up = ds_up<HD>(a.fg[slot_of(t, row_of(i)) * a.heads + h], fv) * kPDown;
-                for (int r = lane; r < kNarrow; r += 32) {
+                for (int r = lane; r < N; r += 32) {
                     const int row = row_of(i) + r;
                     float x = INFINITY, d = 0.f;
                     if (row < t.len) {
@@ -606,8 +651,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_dkv(const __grid_constant__
                         x = x == -INFINITY ? INFINITY : x * kLog2e - kPUp;
                         d = a.delta[(long long)h * a.tokens + t.start + row] * up;
                     }
-                    st_lse[sl * kNarrow + r] = x;
-                    st_d[sl * kNarrow + r] = d;
+                    st_lse[sl * N + r] = x;
+                    st_d[sl * N + r] = d;
                 }
                 __syncwarp();
                 if (lane == 0) bar_arrive(stat_full + sl);
@@ -617,7 +662,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_dkv(const __grid_constant__
         more_registers<kMathRegs>();
         const int half = warp >> 2, row = t.row0 + (warp & 3) * 32 + lane;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t s0 = tS + lanes + 32 * half, p0 = tP + lanes + 32 * half;
+        const uint32_t s0 = tS + lanes + C * half, p0 = tP + lanes + C * half;
         // Half the columns of dv and dk each (dim 32: one warpgroup has dv, the other dk).
         constexpr int W = HD == 32 ? 32 : HD / 2;
         const uint32_t v0 = tV + lanes + (HD == 32 ? 0 : W * half), k0 = tK + lanes + (HD == 32 ? 0 : W * half);
@@ -652,29 +697,30 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_dkv(const __grid_constant__
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             fence_after();
-            const int see = a.causal ? row - q0 - 32 * half : -1;          // columns from here on see this key
+            const int see = a.causal ? row - q0 - C * half : -1;          // columns from here on see this key
             const bool part = __any_sync(0xffffffffu, see > 0);
-            const float* lse = st_lse + sl * kNarrow + 32 * half;
-            const float* dd = st_d + sl * kNarrow + 32 * half;
-            float p[32];
-            {
+            const float* lse = st_lse + sl * N + C * half;
+            const float* dd = st_d + sl * N + C * half;
+            float p[C];
+#pragma unroll
+            for (int b = 0; b < C; b += 32) {
                 uint32_t s[32];
-                ld32(s, s0);
+                ld32(s, s0 + b);
                 wait_ld();
 #pragma unroll
                 for (int x = 0; x < 32; x += 4) {
-                    const float4 z = *reinterpret_cast<const float4*>(lse + x);
-                    p[x] = exp2_fast(fmaf(__uint_as_float(s[x]), c, -z.x));
-                    p[x + 1] = exp2_fast(fmaf(__uint_as_float(s[x + 1]), c, -z.y));
-                    p[x + 2] = exp2_fast(fmaf(__uint_as_float(s[x + 2]), c, -z.z));
-                    p[x + 3] = exp2_fast(fmaf(__uint_as_float(s[x + 3]), c, -z.w));
+                    const float4 z = *reinterpret_cast<const float4*>(lse + b + x);
+                    p[b + x] = exp2_fast(fmaf(__uint_as_float(s[x]), c, -z.x));
+                    p[b + x + 1] = exp2_fast(fmaf(__uint_as_float(s[x + 1]), c, -z.y));
+                    p[b + x + 2] = exp2_fast(fmaf(__uint_as_float(s[x + 2]), c, -z.z));
+                    p[b + x + 3] = exp2_fast(fmaf(__uint_as_float(s[x + 3]), c, -z.w));
                 }
                 if (part) {
 #pragma unroll
                     for (int x = 0; x < 32; ++x)
-                        if (x < see) p[x] = 0.f;
+                        if (b + x < see) p[b + x] = 0.f;
                 }
-                put_parts(s0, p);
+                put_parts(s0 + b, p + b);
             }
             wait_st();
             fence_before();
@@ -685,24 +731,25 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_dkv(const __grid_constant__
             ok = __all_sync(0xffffffffu, bar_wait(dp_ready, i & 1, gone));
             if (!ok) break;
             fence_after();
-            {
+#pragma unroll
+            for (int b = 0; b < C; b += 32) {
                 uint32_t s[32];
-                ld32(s, p0);
+                ld32(s, p0 + b);
                 wait_ld();
 #pragma unroll
                 for (int x = 0; x < 32; x += 4) {
-                    const float4 z = *reinterpret_cast<const float4*>(dd + x);
-                    p[x] *= fmaf(__uint_as_float(s[x]), acc_factor<HD>(), -z.x);
-                    p[x + 1] *= fmaf(__uint_as_float(s[x + 1]), acc_factor<HD>(), -z.y);
-                    p[x + 2] *= fmaf(__uint_as_float(s[x + 2]), acc_factor<HD>(), -z.z);
-                    p[x + 3] *= fmaf(__uint_as_float(s[x + 3]), acc_factor<HD>(), -z.w);
+                    const float4 z = *reinterpret_cast<const float4*>(dd + b + x);
+                    p[b + x] *= fmaf(__uint_as_float(s[x]), acc_factor<HD>(), -z.x);
+                    p[b + x + 1] *= fmaf(__uint_as_float(s[x + 1]), acc_factor<HD>(), -z.y);
+                    p[b + x + 2] *= fmaf(__uint_as_float(s[x + 2]), acc_factor<HD>(), -z.z);
+                    p[b + x + 3] *= fmaf(__uint_as_float(s[x + 3]), acc_factor<HD>(), -z.w);
                 }
                 if (part) {
 #pragma unroll
                     for (int x = 0; x < 32; ++x)
-                        if (x < see) p[x] = 0.f;
+                        if (b + x < see) p[b + x] = 0.f;
                 }
-                put_parts(p0, p);
+                put_parts(p0 + b, p + b);
             }
             wait_st();
             fence_before();
@@ -737,15 +784,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_dkv(const __grid_constant__
     if (threadIdx.x == 0 && *gone) atomicOr(a.err, kErrTcWait);
 }
 
-// dq of 128 queries: key tiles of 64 pass by.  S has two blocks of columns, dS(j)
+// dq of 128 queries: key tiles pass by.  S has two blocks of columns, dS(j)
 // lies in S(j)'s; the order is dP(j+1), dQ(j), S(j+2).
 template <int HD>
 __global__ void __launch_bounds__(kThreads, 1) k_f32_dq(const __grid_constant__ Args a) {
     using Sh = Shape<HD>;
     using Bs = BwdShape<HD>;
-    constexpr int NA = Bs::A, NB = Bs::B;
+    constexpr int NA = Bs::A, NB = Bs::B, N = Bs::N, TILE = Bs::TILE, C = N / 2;
     extern __shared__ __align__(1024) uint8_t sm[];
-    uint8_t *qs = sm, *gs = sm + Sh::TILE128, *kr = sm + Bs::RING, *vr = kr + NA * Sh::TILE64;
+    uint8_t *qs = sm, *gs = sm + Bs::KEPT, *kr = sm + Bs::RING, *vr = kr + NA * TILE;
     uint64_t* bars = reinterpret_cast<uint64_t*>(sm + Bs::BARS);
     uint64_t *k_full = bars, *k_empty = k_full + NA, *v_full = k_empty + NA, *v_empty = v_full + NB, *fixed = v_empty + NB,
              *qg_full = fixed + 1, *s_ready = qg_full + 1,
@@ -764,8 +811,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_dq(const __grid_constant__ 
         return;
     }
     const int last = a.causal ? min(t.row0 + kWide, t.len) : t.len;
-    const int n = (last + kNarrow - 1) / kNarrow;
-    const bool ragged = n * kNarrow > t.len;
+    const int n = (last + N - 1) / N;
+    const bool ragged = n * N > t.len;
 
     if (threadIdx.x == 0) {
         *gone = 0;
@@ -779,31 +826,31 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_dq(const __grid_constant__ 
     fence_before();
     __syncthreads();
     fence_after();
-    const uint32_t tm = *tmem_base, tS = tm, tP = tm + 128, tQ = tm + 256;
+    const uint32_t tm = *tmem_base, tS = tm, tP = tm + 2 * N, tQ = tm + 3 * N;
 
     if (warp >= 8) {
         fewer_registers<kOtherRegs>();
         if (warp == 9) {
             if (lane == 0) {
                 const int r0 = (int)t.start;
-                bar_expect(qg_full, 2 * Sh::TILE128);
+                bar_expect(qg_full, 2 * Bs::KEPT);
                 load_parts<HD, kWide>(qs, &a.q, head, a.heads, r0 + t.row0, qg_full);
                 load_parts<HD, kWide>(gs, &a.g, head, a.heads, r0 + t.row0, qg_full);
                 for (int j = 0; j < n; ++j) {
                     const int sa = j % NA, sb = j % NB;
                     if (j >= NA && !bar_wait(k_empty + sa, (j / NA - 1) & 1, gone)) break;
-                    bar_expect(k_full + sa, Sh::TILE64);
-                    load_parts<HD, kNarrow>(kr + sa * Sh::TILE64, &a.k, kvh, a.kv_heads, r0 + j * kNarrow, k_full + sa);
+                    bar_expect(k_full + sa, TILE);
+                    load_parts<HD, N>(kr + sa * TILE, &a.k, kvh, a.kv_heads, r0 + j * N, k_full + sa);
                     if (j >= NB && !bar_wait(v_empty + sb, (j / NB - 1) & 1, gone)) break;
-                    bar_expect(v_full + sb, Sh::TILE64);
-                    load_parts<HD, kNarrow>(vr + sb * Sh::TILE64, &a.v, kvh, a.kv_heads, r0 + j * kNarrow, v_full + sb);
+                    bar_expect(v_full + sb, TILE);
+                    load_parts<HD, N>(vr + sb * TILE, &a.v, kvh, a.kv_heads, r0 + j * N, v_full + sb);
                 }
             }
             __syncwarp();
             if (ragged) {                   // keys behind the sequence: their dS is 0, 0 times NaN would not be
                 const int st = (n - 1) % NA;
                 if (bar_wait(k_full + st, ((n - 1) / NA) & 1, gone)) {
-                    zero_parts<HD>(kr + st * Sh::TILE64, t.len - (n - 1) * kNarrow);
+                    zero_parts<HD, N>(kr + st * TILE, t.len - (n - 1) * N);
                     fence_async_smem();
                 }
                 __syncwarp();
@@ -813,13 +860,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_dq(const __grid_constant__ 
             if (lane == 0) {
                 auto scores = [&](int j) {
                     if (!bar_wait(k_full + j % NA, (j / NA) & 1, gone)) return false;
-                    parts_rows<HD>(tS + 64 * (j & 1), smem(qs), smem(kr + (j % NA) * Sh::TILE64));
+                    parts_rows<HD, N>(tS + N * (j & 1), smem(qs), smem(kr + (j % NA) * TILE));
                     commit(s_ready + (j & 1));
                     return true;
                 };
                 auto dps = [&](int j) {
                     if (!bar_wait(v_full + j % NB, (j / NB) & 1, gone)) return false;
-                    parts_rows<HD>(tP, smem(gs), smem(vr + (j % NB) * Sh::TILE64));
+                    parts_rows<HD, N>(tP, smem(gs), smem(vr + (j % NB) * TILE));
                     commit(dp_ready);
                     commit(v_empty + j % NB);
                     return true;
@@ -833,7 +880,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_dq(const __grid_constant__ 
                     if (j + 1 < n) ok = dps(j + 1);
                     if (ok && ragged && j == n - 1) ok = bar_wait(fixed, 0, gone);
                     if (!ok) break;
-                    parts_weights<HD>(tQ, tS + 64 * (j & 1), smem(kr + (j % NA) * Sh::TILE64));
+                    parts_weights<HD, N>(tQ, tS + N * (j & 1), smem(kr + (j % NA) * TILE));
                     commit(dq_done);
                     commit(k_empty + j % NA);
                     if (j + 2 < n) ok = scores(j + 2);
@@ -846,7 +893,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_dq(const __grid_constant__ 
         const int half = warp >> 2, row = t.row0 + (warp & 3) * 32 + lane;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         constexpr int W = HD == 32 ? 32 : HD / 2;
-        const uint32_t q0 = tQ + lanes + (HD == 32 ? 0 : W * half), p0 = tP + lanes + 32 * half;
+        const uint32_t q0 = tQ + lanes + (HD == 32 ? 0 : W * half), p0 = tP + lanes + C * half;
         const long long qslot = slot_of(t, t.row0) * a.heads + head;
         const float fq = a.fq[qslot], fg = a.fg[qslot];
         float lse = INFINITY, d = 0.f, acc[W];
@@ -871,19 +918,22 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_dq(const __grid_constant__ 
             fence_before();
         };
         for (int j = 0; j < n; ++j) {
-            const uint32_t s0 = tS + lanes + 64 * (j & 1) + 32 * half;
-            const long long ks = slot_of(t, j * kNarrow) * a.kv_heads + kvh;
+            const uint32_t s0 = tS + lanes + N * (j & 1) + C * half;
+            const long long ks = slot_of(t, j * N) * a.kv_heads + kvh;
             const float fk = a.fk[ks], fv = a.fv[ks], c = a.c * fq * fk;
             ok = __all_sync(0xffffffffu, bar_wait(s_ready + (j & 1), (j >> 1) & 1, gone));
             if (!ok) break;
             fence_after();
-            const int lim = min(t.len, a.causal ? row + 1 : t.len) - j * kNarrow - 32 * half;
-            float p[32];
-            uint32_t s[32];
-            ld32(s, s0);
-            wait_ld();
+            const int lim = min(t.len, a.causal ? row + 1 : t.len) - j * N - C * half;
+            float p[C];
 #pragma unroll
-            for (int x = 0; x < 32; ++x) p[x] = exp2_fast(fmaf(__uint_as_float(s[x]), c, -lse));
+            for (int b = 0; b < C; b += 32) {
+                uint32_t s[32];
+                ld32(s, s0 + b);
+                wait_ld();
+#pragma unroll
+                for (int x = 0; x < 32; ++x) p[b + x] = exp2_fast(fmaf(__uint_as_float(s[x]), c, -lse));
+            }
             if (j) add_q(j - 1);
             if (!ok) break;
             const float up = ds_up<HD>(fg, fv), du = d * up * kPDown;
@@ -891,16 +941,21 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_dq(const __grid_constant__ 
             ok = __all_sync(0xffffffffu, bar_wait(dp_ready, j & 1, gone));
             if (!ok) break;
             fence_after();
-            ld32(s, p0);
-            wait_ld();
+            const bool part = __any_sync(0xffffffffu, lim < C);
 #pragma unroll
-            for (int x = 0; x < 32; ++x) p[x] *= fmaf(__uint_as_float(s[x]), acc_factor<HD>(), -du);
-            if (__any_sync(0xffffffffu, lim < 32)) {
+            for (int b = 0; b < C; b += 32) {
+                uint32_t s[32];
+                ld32(s, p0 + b);
+                wait_ld();
 #pragma unroll
-                for (int x = 0; x < 32; ++x)
-                    if (x >= lim) p[x] = 0.f;
+                for (int x = 0; x < 32; ++x) p[b + x] *= fmaf(__uint_as_float(s[x]), acc_factor<HD>(), -du);
+                if (part) {
+#pragma unroll
+                    for (int x = 0; x < 32; ++x)
+                        if (b + x >= lim) p[b + x] = 0.f;
+                }
+                put_parts(s0 + b, p + b);
             }
-            put_parts(s0, p);
             wait_st();
             fence_before();
             bar_arrive(ds_ready);
@@ -984,7 +1039,7 @@ bool parts_map(CUtensorMap* m, const __half* p, long long tokens, int heads, int
     const int sw = hd * 2 < 128 ? hd * 2 : 128;
     const uint64_t dims[3] = {(uint64_t)hd, (uint64_t)2 * heads, (uint64_t)tokens};
     const uint64_t strides[2] = {(uint64_t)hd * 2, (uint64_t)2 * heads * hd * 2};
-    const uint32_t box[3] = {(uint32_t)(sw / 2), 1, (uint32_t)kNarrow};
+    const uint32_t box[3] = {(uint32_t)(sw / 2), 1, (uint32_t)kBoxRows};
     return encode_tensor(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, p, dims, strides, box, sw);
 }
 
@@ -1041,6 +1096,7 @@ int attention_packed_f32(const PackedParams& p, int backward, cudaStream_t s) {
     // 0 would turn a hidden score's infinity into NaN; 1e-30 weighs the rest alike.
     a.c = p.scale == 0.f ? 1e-30f : fabsf(p.scale) * kLog2e;
     a.scale = p.scale;
+    a.pq = r.parts[0]; a.pk = r.parts[1]; a.pv = r.parts[2]; a.pg = r.parts[3];
     a.fq = r.factors[0]; a.fk = r.factors[1]; a.fv = r.factors[2]; a.fg = r.factors[3];
     a.lse_in = p.lse_in; a.delta = r.delta;
     a.out = static_cast<float*>(p.out); a.lse = p.lse;
