@@ -76,34 +76,20 @@ __device__ __forceinline__ void load_scores(uint32_t (&v)[32], uint32_t ts, int 
             if (!(see >> i & 1)) v[i] = hide;
     }
 }
-// The largest score times c, whatever c's sign.
-__device__ __forceinline__ float largest(const uint32_t (&v)[32], bool neg) {
-    float z[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) z[i] = __uint_as_float(v[i]);
-    if (neg) {
-#pragma unroll
-        for (int i = 4; i < 32; ++i) z[i & 3] = fminf(z[i & 3], __uint_as_float(v[i]));
-        return fminf(fminf(z[0], z[1]), fminf(z[2], z[3]));
-    }
-#pragma unroll
-    for (int i = 4; i < 32; ++i) z[i & 3] = fmaxf(z[i & 3], __uint_as_float(v[i]));
-    return fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3]));
-}
+__device__ __forceinline__ float largest(const uint32_t (&v)[32], bool neg) { return neg ? smallest32(v) : largest32(v); }
 // Weights exp2(c s - ref) of 32 keys, packed to ts + 16 b; returns their sum.
 template <typename T>
 __device__ __forceinline__ float put_weights(const uint32_t (&v)[32], uint32_t ts, int b, float c, float ref) {
     uint32_t q[16];
-    float add[4] = {0.f, 0.f, 0.f, 0.f};
+    float2 add[2] = {both(0.f), both(0.f)};
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-        const float e0 = exp2_fast(fmaf(__uint_as_float(v[2 * i]), c, -ref));
-        const float e1 = exp2_fast(fmaf(__uint_as_float(v[2 * i + 1]), c, -ref));
-        add[i & 3] += e0 + e1;
-        q[i] = pack2<T>(e0, e1);
+        const float2 e = exp2_both(__ffma2_rn(pair(v[2 * i], v[2 * i + 1]), both(c), both(-ref)));
+        add[i & 1] = __fadd2_rn(add[i & 1], e);
+        q[i] = pack2<T>(e.x, e.y);
     }
     st16(ts + 16 * b, q);
-    return (add[0] + add[1]) + (add[2] + add[3]);
+    return (add[0].x + add[0].y) + (add[1].x + add[1].y);
 }
 
 template <typename T, int HD>
@@ -505,8 +491,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_cached_tc(const __grid_constant
 
 template <typename T, int HD>
 int launch(const Args& a, int blocks, cudaStream_t s) {
-    if (cudaFuncSetAttribute(k_cached_tc<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<HD>::SMEM) != cudaSuccess)
-        return kErrCuda;
+    if (!allow_smem<&k_cached_tc<T, HD>>(Shape<HD>::SMEM)) return kErrCuda;
     k_cached_tc<T, HD><<<blocks, kThreads, Shape<HD>::SMEM, s>>>(a);
     if (cudaGetLastError() != cudaSuccess) return kErrCuda;
     return launch_join<T, HD>(a, blocks, s);

@@ -46,12 +46,21 @@ static bool room_ok(const PackedParams& p, int backward) {
     return n == 0 || (p.ws && p.ws_bytes >= n && (reinterpret_cast<uintptr_t>(p.ws) & 15u) == 0);
 }
 
+// A thread of autograd's may have no context yet, which the tensor maps need.
+static int bind_device() {
+    int dev = 0;
+    if (cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) return kOk;
+    cudaGetLastError();
+    return kErrCuda;
+}
+
 int attention_packed(const PackedParams& p, cudaStream_t s) {
     if (int st = check(p)) return st;
     if (p.tokens == 0) return kOk;
     if (!p.out) return kErrNullPtr;
     if (reinterpret_cast<uintptr_t>(p.out) & 15u) return kErrUnsupported;
     if (!room_ok(p, 0)) return kErrAlloc;
+    if (int st = bind_device()) return st;
     return p.type == kF32 ? attention_packed_f32(p, 0, s) : attention_packed_tc(p, s);
 }
 
@@ -63,6 +72,7 @@ int attention_packed_backward(const PackedParams& p, cudaStream_t s) {
     if (!room_ok(p, 1)) return kErrAlloc;
     for (const void* x : {p.out_in, (const void*)p.dq, (const void*)p.dk, (const void*)p.dv})
         if (reinterpret_cast<uintptr_t>(x) & 15u) return kErrUnsupported;
+    if (int st = bind_device()) return st;
     return p.type == kF32 ? attention_packed_f32(p, 1, s) : attention_packed_backward_tc(p, s);
 }
 

@@ -86,16 +86,11 @@ __device__ __forceinline__ void zero_rows(uint8_t* tile, int r0) {
         *reinterpret_cast<uint4*>(tile + (e / n) * Sh::BOX + r0 * Sh::SW + (e % n) * 16) = make_uint4(0, 0, 0, 0);
 }
 
-// D (+)= A B^T over HD, both tiles row-major in shared memory.
+// D = A B^T over HD, both tiles row-major in shared memory.
 template <typename T, int HD>
 __device__ __forceinline__ void mma_rows(uint32_t d, const uint8_t* a, const uint8_t* b) {
     using Sh = Shape<HD>;
-    constexpr uint32_t instr = instruction<T>(kTile, kTile, false);
-    for (int k = 0; k < HD; k += 16) {
-        const uint32_t off = (k * 2 / Sh::SW) * Sh::BOX + (k * 2) % Sh::SW;
-        mma_ss(d, operand<Sh::SW>(smem(a) + off, 16, 8 * Sh::SW), operand<Sh::SW>(smem(b) + off, 16, 8 * Sh::SW), instr,
-               k > 0);
-    }
+    product_ss<HD / 16, Sh::SW>(d, smem(a), smem(b), Sh::BOX, instruction<T>(kTile, kTile, false));
 }
 // D (+)= W B, W [128, 128] packed in tensor memory (columns 0-31 and 64-95 of its
 // block), B's rows summed over.
@@ -103,9 +98,10 @@ template <typename T, int HD>
 __device__ __forceinline__ void mma_weights(uint32_t d, uint32_t w, const uint8_t* b, bool add) {
     using Sh = Shape<HD>;
     constexpr uint32_t instr = instruction<T>(kTile, HD, true);
+    const uint64_t db = operand<Sh::SW>(smem(b), Sh::BOX, 8 * Sh::SW);
+#pragma unroll
     for (int k = 0; k < kTile; k += 16)
-        mma_ts(d, w + (k < 64 ? k / 2 : 64 + (k - 64) / 2), operand<Sh::SW>(smem(b) + k * Sh::SW, Sh::BOX, 8 * Sh::SW),
-               instr, add || k > 0);
+        mma_ts(d, w + (k < 64 ? k / 2 : 64 + (k - 64) / 2), db + (k * Sh::SW >> 4), instr, add || k > 0);
 }
 
 // A row of HD sums, times f, to global memory.
@@ -147,7 +143,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_packed_dkv_tc(const __grid_cons
     constexpr int NA = Sh::A, NB = Sh::B;
     extern __shared__ __align__(1024) uint8_t sm[];
     uint8_t *ks = sm, *vs = sm + Sh::TILE, *qr = sm + 2 * Sh::TILE, *gr = qr + NA * Sh::TILE;
-    float* st_lse = reinterpret_cast<float*>(sm + Sh::STAT);       // [2][128]
+    float* st_lse = reinterpret_cast<float*>(sm + Sh::STAT);       // negative; [2][128]
     float* st_d = st_lse + 2 * kTile;
     uint64_t* bars = reinterpret_cast<uint64_t*>(sm + Sh::BARS);
     uint64_t *kv_full = bars, *q_full = bars + 1, *q_empty = q_full + NA, *g_full = q_empty + NA, *g_empty = g_full + NB,
@@ -286,8 +282,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_packed_dkv_tc(const __grid_cons
                         x = x == -INFINITY ? INFINITY : x * kLog2e - p_shift<T>();
                         d = a.delta[at + row] * gf;
                     }
-                    st_lse[sl * kTile + r] = x;
-                    st_d[sl * kTile + r] = d;
+                    st_lse[sl * kTile + r] = -x;
+                    st_d[sl * kTile + r] = -d;
                 }
                 __syncwarp();
                 if (lane == 0) bar_arrive(stat_full + sl);
@@ -310,27 +306,27 @@ __global__ void __launch_bounds__(kThreads, 1) k_packed_dkv_tc(const __grid_cons
             const int see = diag ? row - t.row0 - 64 * half : -1;          // columns from here on see this key
             const float* lse = st_lse + sl * kTile + 64 * half;
             const float* dd = st_d + sl * kTile + 64 * half;
-            float p[64];
+            float2 p[32];
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
                 uint32_t s[32], w[16];
                 ld32(s, s0 + 32 * b);
                 wait_ld();
 #pragma unroll
-                for (int x = 0; x < 32; x += 4) {
-                    const float4 m = *reinterpret_cast<const float4*>(lse + 32 * b + x);
-                    p[32 * b + x] = exp2_fast(fmaf(__uint_as_float(s[x]), a.c, -m.x));
-                    p[32 * b + x + 1] = exp2_fast(fmaf(__uint_as_float(s[x + 1]), a.c, -m.y));
-                    p[32 * b + x + 2] = exp2_fast(fmaf(__uint_as_float(s[x + 2]), a.c, -m.z));
-                    p[32 * b + x + 3] = exp2_fast(fmaf(__uint_as_float(s[x + 3]), a.c, -m.w));
+                for (int x = 0; x < 16; x += 2) {
+                    const float4 m = *reinterpret_cast<const float4*>(lse + 32 * b + 2 * x);
+                    p[16 * b + x] = exp2_both(__ffma2_rn(pair(s[2 * x], s[2 * x + 1]), both(a.c), make_float2(m.x, m.y)));
+                    p[16 * b + x + 1] = exp2_both(__ffma2_rn(pair(s[2 * x + 2], s[2 * x + 3]), both(a.c), make_float2(m.z, m.w)));
                 }
                 if (diag) {
 #pragma unroll
-                    for (int x = 0; x < 32; ++x)
-                        if (32 * b + x < see) p[32 * b + x] = 0.f;
+                    for (int x = 0; x < 16; ++x) {
+                        if (32 * b + 2 * x < see) p[16 * b + x].x = 0.f;
+                        if (32 * b + 2 * x + 1 < see) p[16 * b + x].y = 0.f;
+                    }
                 }
 #pragma unroll
-                for (int x = 0; x < 16; ++x) w[x] = pack2<T>(p[32 * b + 2 * x], p[32 * b + 2 * x + 1]);
+                for (int x = 0; x < 16; ++x) w[x] = pack2<T>(p[16 * b + x].x, p[16 * b + x].y);
                 st16(s0 + 16 * b, w);
             }
             wait_st();
@@ -346,14 +342,18 @@ __global__ void __launch_bounds__(kThreads, 1) k_packed_dkv_tc(const __grid_cons
                 ld32(s, p0 + 32 * b);
                 wait_ld();
 #pragma unroll
-                for (int x = 0; x < 32; x += 4) {
-                    const float4 m = *reinterpret_cast<const float4*>(dd + 32 * b + x);
-                    float e[4] = {fmaf(__uint_as_float(s[x]), gf, -m.x), fmaf(__uint_as_float(s[x + 1]), gf, -m.y),
-                                  fmaf(__uint_as_float(s[x + 2]), gf, -m.z), fmaf(__uint_as_float(s[x + 3]), gf, -m.w)};
-#pragma unroll
-                    for (int y = 0; y < 4; ++y) e[y] = 32 * b + x + y < see ? 0.f : e[y] * p[32 * b + x + y];
-                    w[x / 2] = pack2<T>(e[0], e[1]);
-                    w[x / 2 + 1] = pack2<T>(e[2], e[3]);
+                for (int x = 0; x < 16; x += 2) {
+                    const float4 m = *reinterpret_cast<const float4*>(dd + 32 * b + 2 * x);
+                    float2 e0 = __fmul2_rn(p[16 * b + x], __ffma2_rn(pair(s[2 * x], s[2 * x + 1]), both(gf), make_float2(m.x, m.y)));
+                    float2 e1 = __fmul2_rn(p[16 * b + x + 1], __ffma2_rn(pair(s[2 * x + 2], s[2 * x + 3]), both(gf), make_float2(m.z, m.w)));
+                    if (diag) {
+                        if (32 * b + 2 * x < see) e0.x = 0.f;
+                        if (32 * b + 2 * x + 1 < see) e0.y = 0.f;
+                        if (32 * b + 2 * x + 2 < see) e1.x = 0.f;
+                        if (32 * b + 2 * x + 3 < see) e1.y = 0.f;
+                    }
+                    w[x] = pack2<T>(e0.x, e0.y);
+                    w[x + 1] = pack2<T>(e1.x, e1.y);
                 }
                 st16(p0 + 16 * b, w);
             }
@@ -503,14 +503,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_packed_dq_tc(const __grid_const
             if (!ok) break;
             fence_after();
             const int lim = min(t.len, a.causal ? row + 1 : t.len) - j * kTile - 64 * half;   // columns below are seen
-            float p[64];
+            float2 p[32];
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
                 uint32_t s[32];
                 ld32(s, s0 + 32 * b);
                 wait_ld();
 #pragma unroll
-                for (int x = 0; x < 32; ++x) p[32 * b + x] = exp2_fast(fmaf(__uint_as_float(s[x]), a.c, -lse));
+                for (int x = 0; x < 16; ++x)
+                    p[16 * b + x] = exp2_both(__ffma2_rn(pair(s[2 * x], s[2 * x + 1]), both(a.c), both(-lse)));
             }
             ok = bar_wait(dp_ready, j & 1, gone);
             ok = __all_sync(0xffffffffu, ok);
@@ -523,14 +524,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_packed_dq_tc(const __grid_const
                 ld32(s, p0 + 32 * b);
                 wait_ld();
 #pragma unroll
-                for (int x = 0; x < 32; ++x) p[32 * b + x] *= fmaf(__uint_as_float(s[x]), gf, -d);
-                if (part) {
-#pragma unroll
-                    for (int x = 0; x < 32; ++x)
-                        if (32 * b + x >= lim) p[32 * b + x] = 0.f;
+                for (int x = 0; x < 16; ++x) {
+                    float2 e = __fmul2_rn(p[16 * b + x], __ffma2_rn(pair(s[2 * x], s[2 * x + 1]), both(gf), both(-d)));
+                    if (part) {
+                        if (32 * b + 2 * x >= lim) e.x = 0.f;
+                        if (32 * b + 2 * x + 1 >= lim) e.y = 0.f;
+                    }
+                    w[x] = pack2<T>(e.x, e.y);
                 }
-#pragma unroll
-                for (int x = 0; x < 16; ++x) w[x] = pack2<T>(p[32 * b + 2 * x], p[32 * b + 2 * x + 1]);
                 st16(s0 + 16 * b, w);
             }
             wait_st();
@@ -598,9 +599,7 @@ int launch_bwd(const BwdArgs& a, const PackedParams& p, cudaStream_t s) {
         p, const_cast<float*>(a.delta), top);
     if (cudaGetLastError() != cudaSuccess) return kErrCuda;
     const unsigned slots = (unsigned)packed_slots(a.tokens, a.n_seqs, kTile);
-    if (cudaFuncSetAttribute(k_packed_dkv_tc<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::SMEM) != cudaSuccess ||
-        cudaFuncSetAttribute(k_packed_dq_tc<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::SMEM) != cudaSuccess)
-        return kErrCuda;
+    if (!allow_smem<&k_packed_dkv_tc<T, HD>>(Sh::SMEM) || !allow_smem<&k_packed_dq_tc<T, HD>>(Sh::SMEM)) return kErrCuda;
     k_packed_dkv_tc<T, HD><<<slots * a.kv_heads, kThreads, Sh::SMEM, s>>>(a);
     if (cudaGetLastError() != cudaSuccess) return kErrCuda;
     k_packed_dq_tc<T, HD><<<slots * a.heads, kThreads, Sh::SMEM, s>>>(a);

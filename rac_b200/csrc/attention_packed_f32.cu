@@ -217,29 +217,30 @@ __device__ __forceinline__ void parts_weights(uint32_t d, uint32_t w, uint32_t b
     }
 }
 // 32 weights of a row as parts, to the columns that parts_weights reads.
-__device__ __forceinline__ void put_parts(uint32_t addr, const float* p) {
+__device__ __forceinline__ void put_parts(uint32_t addr, const float2* p) {
     uint32_t hi[16], lo[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-        hi[i] = pack2<__half>(p[2 * i], p[2 * i + 1]);
-        const __half2 h = *reinterpret_cast<const __half2*>(&hi[i]);
-        lo[i] = pack2<__half>(p[2 * i] - __low2float(h), p[2 * i + 1] - __high2float(h));
+        hi[i] = pack2<__half>(p[i].x, p[i].y);
+        const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi[i]));
+        const float2 d = __ffma2_rn(h, both(-1.f), p[i]);
+        lo[i] = pack2<__half>(d.x, d.y);
     }
     st16(addr, hi);
     st16(addr + 16, lo);
 }
 // acc += f * 32 columns.
-__device__ __forceinline__ void take32(float* acc, uint32_t addr, float f) {
+__device__ __forceinline__ void take32(float2* acc, uint32_t addr, float f) {
     uint32_t o[32];
     ld32(o, addr);
     wait_ld();
 #pragma unroll
-    for (int i = 0; i < 32; ++i) acc[i] = fmaf(__uint_as_float(o[i]), f, acc[i]);
+    for (int i = 0; i < 16; ++i) acc[i] = __ffma2_rn(pair(o[2 * i], o[2 * i + 1]), both(f), acc[i]);
 }
-__device__ __forceinline__ void store32(float* dst, const float* v, float f) {
+__device__ __forceinline__ void store32(float* dst, const float2* v, float f) {
 #pragma unroll
-    for (int i = 0; i < 32; i += 4)
-        *reinterpret_cast<float4*>(dst + i) = make_float4(v[i] * f, v[i + 1] * f, v[i + 2] * f, v[i + 3] * f);
+    for (int i = 0; i < 16; i += 2)
+        *reinterpret_cast<float4*>(dst + 2 * i) = make_float4(v[i].x * f, v[i].y * f, v[i + 1].x * f, v[i + 1].y * f);
 }
 __device__ __forceinline__ void zero_rows_out(float* dst, long long row_stride, int hd, int row0, int len) {
     const int n = min(kWide, len - row0) * (hd / 4);
@@ -386,9 +387,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_fwd(const __grid_constant__
         fence_before();
         bar_arrive(q_full);
         const float cq = a.c * a.fq[slot_of(t, t.row0) * a.heads + head];
-        float o[HD], m = -INFINITY, l = 0.f;
+        float m = -INFINITY, l = 0.f;
+        float2 o[HD / 2];
 #pragma unroll
-        for (int i = 0; i < HD; ++i) o[i] = 0.f;
+        for (int i = 0; i < HD / 2; ++i) o[i] = both(0.f);
         bool ok = true;
         for (int j = w; j < n; j += 2) {
             const long long ks = slot_of(t, j * kKeysF32) * a.kv_heads + kvh;
@@ -414,10 +416,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_fwd(const __grid_constant__
             for (int b = 0; b < kKeysF32 / 32; ++b) {
                 uint32_t x[32];
                 scores(x, b);
-                float z[4] = {__uint_as_float(x[0]), __uint_as_float(x[1]), __uint_as_float(x[2]), __uint_as_float(x[3])};
-#pragma unroll
-                for (int i = 4; i < 32; ++i) z[i & 3] = fmaxf(z[i & 3], __uint_as_float(x[i]));
-                y = fmaxf(y, fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])));
+                y = fmaxf(y, largest32(x));
             }
             const float top = y * c;
             // The reference point moves only when a weight would pass 2^8.
@@ -426,21 +425,21 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_fwd(const __grid_constant__
                 m = top;
                 l *= up;
 #pragma unroll
-                for (int i = 0; i < HD; ++i) o[i] *= up;
+                for (int i = 0; i < HD / 2; ++i) o[i] = __fmul2_rn(o[i], both(up));
             }
             // Weights carry 2^6, which keeps their second parts above the smallest half.
             const float ref = m == -INFINITY ? 0.f : m - 6.f;
 #pragma unroll 1
             for (int b = 0; b < kKeysF32 / 32; ++b) {
                 uint32_t x[32];
-                float p[32], add[4] = {0.f, 0.f, 0.f, 0.f};
+                float2 p[16], add[2] = {both(0.f), both(0.f)};
                 scores(x, b);
 #pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    p[i] = exp2_fast(fmaf(__uint_as_float(x[i]), c, -ref));
-                    add[i & 3] += p[i];
+                for (int i = 0; i < 16; ++i) {
+                    p[i] = exp2_both(__ffma2_rn(pair(x[2 * i], x[2 * i + 1]), both(c), both(-ref)));
+                    add[i & 1] = __fadd2_rn(add[i & 1], p[i]);
                 }
-                l += (add[0] + add[1]) + (add[2] + add[3]);
+                l += (add[0].x + add[0].y) + (add[1].x + add[1].y);
                 put_parts(ts + 32 * b, p);
             }
             wait_st();
@@ -450,7 +449,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_fwd(const __grid_constant__
             if (!ok) break;
             fence_after();
 #pragma unroll
-            for (int b = 0; b < HD / 32; ++b) take32(o + 32 * b, to + 32 * b, fv);
+            for (int b = 0; b < HD / 32; ++b) take32(o + 16 * b, to + 32 * b, fv);
             fence_before();
             bar_arrive(o_taken);
         }
@@ -464,7 +463,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_fwd(const __grid_constant__
                 if (ok) {
                     jm[lr] = make_float2(m, l);
 #pragma unroll
-                    for (int i = 0; i < HD; ++i) jo[lr * (HD + 1) + i] = o[i];
+                    for (int i = 0; i < HD / 2; ++i) {
+                        jo[lr * (HD + 1) + 2 * i] = o[i].x;
+                        jo[lr * (HD + 1) + 2 * i + 1] = o[i].y;
+                    }
                 }
                 bar_arrive(joined);
             }
@@ -477,12 +479,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_fwd(const __grid_constant__
                 l = l * f0 + z.y * f1;
                 m = M;
 #pragma unroll
-                for (int i = 0; i < HD; ++i) o[i] = o[i] * f0 + jo[lr * (HD + 1) + i] * f1;
+                for (int i = 0; i < HD / 2; ++i)
+                    o[i] = make_float2(o[i].x * f0 + jo[lr * (HD + 1) + 2 * i] * f1, o[i].y * f0 + jo[lr * (HD + 1) + 2 * i + 1] * f1);
             }
             if (ok && row < t.len) {
                 const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-                for (int b = 0; b < HD / 32; ++b) store32(out + row * out_row + 32 * b, o + 32 * b, inv);
+                for (int b = 0; b < HD / 32; ++b) store32(out + row * out_row + 32 * b, o + 16 * b, inv);
                 if (a.lse)
                     a.lse[(long long)head * a.tokens + t.start + row] =
                         l == 0.f ? -INFINITY : (m - 6.f) * 0.69314718055994531f + logf(l);
@@ -524,7 +527,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_dkv(const __grid_constant__
     constexpr int NA = Bs::A, NB = Bs::B, N = Bs::N, TILE = Bs::TILE, C = N / 2;
     extern __shared__ __align__(1024) uint8_t sm[];
     uint8_t *ks = sm, *vs = sm + Bs::KEPT, *qr = sm + Bs::RING, *gr = qr + NA * TILE;
-    float* st_lse = reinterpret_cast<float*>(sm + Bs::STAT);       // [2][64]
+    float* st_lse = reinterpret_cast<float*>(sm + Bs::STAT);       // negative; [2][64]
     float* st_d = st_lse + 2 * N;
     uint64_t* bars = reinterpret_cast<uint64_t*>(sm + Bs::BARS);
     uint64_t *q_full = bars, *q_empty = q_full + NA, *q_fixed = q_empty + NA, *g_full = q_fixed + NA, *g_empty = g_full + NB,
@@ -651,8 +654,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_dkv(const __grid_constant__
                         x = x == -INFINITY ? INFINITY : x * kLog2e - kPUp;
                         d = a.delta[(long long)h * a.tokens + t.start + row] * up;
                     }
-                    st_lse[sl * N + r] = x;
-                    st_d[sl * N + r] = d;
+                    st_lse[sl * N + r] = -x;
+                    st_d[sl * N + r] = -d;
                 }
                 __syncwarp();
                 if (lane == 0) bar_arrive(stat_full + sl);
@@ -668,13 +671,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_dkv(const __grid_constant__
         const uint32_t v0 = tV + lanes + (HD == 32 ? 0 : W * half), k0 = tK + lanes + (HD == 32 ? 0 : W * half);
         const long long ks = slot_of(t, t.row0) * a.kv_heads + kvh;
         const float fk = a.fk[ks], fv = a.fv[ks];
-        float av[W], ak[HD == 32 ? 1 : W];
+        float2 av[W / 2], ak[W / 2];
 #pragma unroll
-        for (int i = 0; i < W; ++i) av[i] = 0.f;
-        if (HD != 32) {
-#pragma unroll
-            for (int i = 0; i < W; ++i) ak[i % (HD == 32 ? 1 : W)] = 0.f;
-        }
+        for (int i = 0; i < W / 2; ++i) av[i] = ak[i] = both(0.f);
         bool ok = true;
         float take_k = 0.f;                // factor of the dK tile that has not been taken yet
         auto add_k = [&](int i) {
@@ -685,7 +684,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_dkv(const __grid_constant__
                 if (half == 1) take32(av, k0, take_k);
             } else {
 #pragma unroll
-                for (int b = 0; b < W / 32; ++b) take32(ak + 32 * b, k0 + 32 * b, take_k);
+                for (int b = 0; b < W / 32; ++b) take32(ak + 16 * b, k0 + 32 * b, take_k);
             }
             fence_before();
         };
@@ -701,26 +700,26 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_dkv(const __grid_constant__
             const bool part = __any_sync(0xffffffffu, see > 0);
             const float* lse = st_lse + sl * N + C * half;
             const float* dd = st_d + sl * N + C * half;
-            float p[C];
+            float2 p[C / 2];
 #pragma unroll
-            for (int b = 0; b < C; b += 32) {
+            for (int b = 0; b < C / 2; b += 16) {
                 uint32_t s[32];
-                ld32(s, s0 + b);
+                ld32(s, s0 + 2 * b);
                 wait_ld();
 #pragma unroll
-                for (int x = 0; x < 32; x += 4) {
-                    const float4 z = *reinterpret_cast<const float4*>(lse + b + x);
-                    p[b + x] = exp2_fast(fmaf(__uint_as_float(s[x]), c, -z.x));
-                    p[b + x + 1] = exp2_fast(fmaf(__uint_as_float(s[x + 1]), c, -z.y));
-                    p[b + x + 2] = exp2_fast(fmaf(__uint_as_float(s[x + 2]), c, -z.z));
-                    p[b + x + 3] = exp2_fast(fmaf(__uint_as_float(s[x + 3]), c, -z.w));
+                for (int x = 0; x < 16; x += 2) {
+                    const float4 z = *reinterpret_cast<const float4*>(lse + 2 * (b + x));      // -lse
+                    p[b + x] = exp2_both(__ffma2_rn(pair(s[2 * x], s[2 * x + 1]), both(c), make_float2(z.x, z.y)));
+                    p[b + x + 1] = exp2_both(__ffma2_rn(pair(s[2 * x + 2], s[2 * x + 3]), both(c), make_float2(z.z, z.w)));
                 }
                 if (part) {
 #pragma unroll
-                    for (int x = 0; x < 32; ++x)
-                        if (b + x < see) p[b + x] = 0.f;
+                    for (int x = 0; x < 16; ++x) {
+                        if (2 * (b + x) < see) p[b + x].x = 0.f;
+                        if (2 * (b + x) + 1 < see) p[b + x].y = 0.f;
+                    }
                 }
-                put_parts(s0 + b, p + b);
+                put_parts(s0 + 2 * b, p + b);
             }
             wait_st();
             fence_before();
@@ -732,24 +731,25 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_dkv(const __grid_constant__
             if (!ok) break;
             fence_after();
 #pragma unroll
-            for (int b = 0; b < C; b += 32) {
+            for (int b = 0; b < C / 2; b += 16) {
                 uint32_t s[32];
-                ld32(s, p0 + b);
+                ld32(s, p0 + 2 * b);
                 wait_ld();
 #pragma unroll
-                for (int x = 0; x < 32; x += 4) {
-                    const float4 z = *reinterpret_cast<const float4*>(dd + b + x);
-                    p[b + x] *= fmaf(__uint_as_float(s[x]), acc_factor<HD>(), -z.x);
-                    p[b + x + 1] *= fmaf(__uint_as_float(s[x + 1]), acc_factor<HD>(), -z.y);
-                    p[b + x + 2] *= fmaf(__uint_as_float(s[x + 2]), acc_factor<HD>(), -z.z);
-                    p[b + x + 3] *= fmaf(__uint_as_float(s[x + 3]), acc_factor<HD>(), -z.w);
+                for (int x = 0; x < 16; x += 2) {
+                    const float4 z = *reinterpret_cast<const float4*>(dd + 2 * (b + x));       // -D
+                    const float2 f = both(acc_factor<HD>());
+                    p[b + x] = __fmul2_rn(p[b + x], __ffma2_rn(pair(s[2 * x], s[2 * x + 1]), f, make_float2(z.x, z.y)));
+                    p[b + x + 1] = __fmul2_rn(p[b + x + 1], __ffma2_rn(pair(s[2 * x + 2], s[2 * x + 3]), f, make_float2(z.z, z.w)));
                 }
                 if (part) {
 #pragma unroll
-                    for (int x = 0; x < 32; ++x)
-                        if (b + x < see) p[b + x] = 0.f;
+                    for (int x = 0; x < 16; ++x) {
+                        if (2 * (b + x) < see) p[b + x].x = 0.f;
+                        if (2 * (b + x) + 1 < see) p[b + x].y = 0.f;
+                    }
                 }
-                put_parts(p0 + b, p + b);
+                put_parts(p0 + 2 * b, p + b);
             }
             wait_st();
             fence_before();
@@ -760,7 +760,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_dkv(const __grid_constant__
             fence_after();
             if (HD != 32 || half == 0) {
 #pragma unroll
-                for (int b = 0; b < W / 32; ++b) take32(av + 32 * b, v0 + 32 * b, fg * kPDown);
+                for (int b = 0; b < W / 32; ++b) take32(av + 16 * b, v0 + 32 * b, fg * kPDown);
             }
             fence_before();
         }
@@ -771,8 +771,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_dkv(const __grid_constant__
             } else {
 #pragma unroll
                 for (int b = 0; b < W / 32; ++b) {
-                    store32(dv + row * out_row + W * half + 32 * b, av + 32 * b, 1.f);
-                    store32(dk + row * out_row + W * half + 32 * b, ak + 32 * b, fabsf(a.scale));
+                    store32(dv + row * out_row + W * half + 32 * b, av + 16 * b, 1.f);
+                    store32(dk + row * out_row + W * half + 32 * b, ak + 16 * b, fabsf(a.scale));
                 }
             }
         }
@@ -896,9 +896,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_dq(const __grid_constant__ 
         const uint32_t q0 = tQ + lanes + (HD == 32 ? 0 : W * half), p0 = tP + lanes + C * half;
         const long long qslot = slot_of(t, t.row0) * a.heads + head;
         const float fq = a.fq[qslot], fg = a.fg[qslot];
-        float lse = INFINITY, d = 0.f, acc[W];
+        float lse = INFINITY, d = 0.f;
+        float2 acc[W / 2];
 #pragma unroll
-        for (int i = 0; i < W; ++i) acc[i] = 0.f;
+        for (int i = 0; i < W / 2; ++i) acc[i] = both(0.f);
         if (row < t.len) {
             const long long at = (long long)head * a.tokens + t.start + row;
             lse = a.lse_in[at];
@@ -913,7 +914,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_dq(const __grid_constant__ 
             fence_after();
             if (HD != 32 || half == 0) {
 #pragma unroll
-                for (int b = 0; b < W / 32; ++b) take32(acc + 32 * b, q0 + 32 * b, take_f);
+                for (int b = 0; b < W / 32; ++b) take32(acc + 16 * b, q0 + 32 * b, take_f);
             }
             fence_before();
         };
@@ -925,14 +926,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_dq(const __grid_constant__ 
             if (!ok) break;
             fence_after();
             const int lim = min(t.len, a.causal ? row + 1 : t.len) - j * N - C * half;
-            float p[C];
+            float2 p[C / 2];
 #pragma unroll
-            for (int b = 0; b < C; b += 32) {
+            for (int b = 0; b < C / 2; b += 16) {
                 uint32_t s[32];
-                ld32(s, s0 + b);
+                ld32(s, s0 + 2 * b);
                 wait_ld();
 #pragma unroll
-                for (int x = 0; x < 32; ++x) p[b + x] = exp2_fast(fmaf(__uint_as_float(s[x]), c, -lse));
+                for (int x = 0; x < 16; ++x)
+                    p[b + x] = exp2_both(__ffma2_rn(pair(s[2 * x], s[2 * x + 1]), both(c), both(-lse)));
             }
             if (j) add_q(j - 1);
             if (!ok) break;
@@ -943,18 +945,21 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_dq(const __grid_constant__ 
             fence_after();
             const bool part = __any_sync(0xffffffffu, lim < C);
 #pragma unroll
-            for (int b = 0; b < C; b += 32) {
+            for (int b = 0; b < C / 2; b += 16) {
                 uint32_t s[32];
-                ld32(s, p0 + b);
+                ld32(s, p0 + 2 * b);
                 wait_ld();
 #pragma unroll
-                for (int x = 0; x < 32; ++x) p[b + x] *= fmaf(__uint_as_float(s[x]), acc_factor<HD>(), -du);
+                for (int x = 0; x < 16; ++x)
+                    p[b + x] = __fmul2_rn(p[b + x], __ffma2_rn(pair(s[2 * x], s[2 * x + 1]), both(acc_factor<HD>()), both(-du)));
                 if (part) {
 #pragma unroll
-                    for (int x = 0; x < 32; ++x)
-                        if (b + x >= lim) p[b + x] = 0.f;
+                    for (int x = 0; x < 16; ++x) {
+                        if (2 * (b + x) >= lim) p[b + x].x = 0.f;
+                        if (2 * (b + x) + 1 >= lim) p[b + x].y = 0.f;
+                    }
                 }
-                put_parts(s0 + b, p + b);
+                put_parts(s0 + 2 * b, p + b);
             }
             wait_st();
             fence_before();
@@ -964,7 +969,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_dq(const __grid_constant__ 
         if (ok && row < t.len && (HD != 32 || half == 0)) {
 #pragma unroll
             for (int b = 0; b < W / 32; ++b)
-                store32(dq + row * out_row + (HD == 32 ? 0 : W * half) + 32 * b, acc + 32 * b, a.scale);
+                store32(dq + row * out_row + (HD == 32 ? 0 : W * half) + 32 * b, acc + 16 * b, a.scale);
         }
     }
     fence_before();
@@ -1043,6 +1048,13 @@ bool parts_map(CUtensorMap* m, const __half* p, long long tokens, int heads, int
     return encode_tensor(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, p, dims, strides, box, sw);
 }
 
+template <auto* Kernel>
+int go(const Args& a, int smem, unsigned grid, cudaStream_t s) {
+    if (!allow_smem<Kernel>(smem)) return kErrCuda;
+    Kernel<<<grid, kThreads, smem, s>>>(a);
+    return cudaGetLastError() == cudaSuccess ? kOk : kErrCuda;
+}
+
 template <int HD>
 int launch(const PackedParams& p, const Room& r, Args& a, bool backward, cudaStream_t s) {
     SplitArgs sp{};
@@ -1057,22 +1069,17 @@ int launch(const PackedParams& p, const Room& r, Args& a, bool backward, cudaStr
     const unsigned slots = (unsigned)packed_slots(p.tokens, p.n_seqs, kSplit);
     k_split<HD><<<slots * sp.first[4], 256, 0, s>>>(sp);
     if (cudaGetLastError() != cudaSuccess) return kErrCuda;
-    auto go = [&](auto* kernel, int smem, unsigned grid) {
-        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return kErrCuda;
-        kernel<<<grid, kThreads, smem, s>>>(a);
-        return cudaGetLastError() == cudaSuccess ? kOk : kErrCuda;
-    };
-    if (!backward) return go(&k_f32_fwd<HD>, FwdShape<HD>::SMEM, slots * p.heads);
+    if (!backward) return go<&k_f32_fwd<HD>>(a, FwdShape<HD>::SMEM, slots * p.heads, s);
     a.split = by_head(p.tokens, p.heads, p.kv_heads);
     if (a.split) { a.dk = r.dk; a.dv = r.dv; }
-    if (int st = go(&k_f32_dkv<HD>, BwdShape<HD>::SMEM, slots * (a.split ? p.heads : p.kv_heads))) return st;
+    if (int st = go<&k_f32_dkv<HD>>(a, BwdShape<HD>::SMEM, slots * (a.split ? p.heads : p.kv_heads), s)) return st;
     if (a.split) {
         const long long n = p.tokens * p.kv_heads * (HD / 4);
         k_add_heads<<<(unsigned)((n + 255) / 256), 256, 0, s>>>(r.dk, r.dv, static_cast<float*>(p.dk),
                                                                 static_cast<float*>(p.dv), a.group, HD, n);
         if (cudaGetLastError() != cudaSuccess) return kErrCuda;
     }
-    return go(&k_f32_dq<HD>, BwdShape<HD>::SMEM, slots * p.heads);
+    return go<&k_f32_dq<HD>>(a, BwdShape<HD>::SMEM, slots * p.heads, s);
 }
 
 }  // namespace

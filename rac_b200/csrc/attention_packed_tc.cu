@@ -133,12 +133,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_packed_fwd_tc(const __grid_cons
         if (lane == 0) {
             constexpr uint32_t iqk = instruction<T>(kRows, kKeys, false), ipv = instruction<T>(kRows, HD, true);
             auto scores = [&](int w, int i) {           // S_w = Q_w K^T, K in ring entry i
-                const uint32_t qa = smem(qs + w * Sh::TILE), kb = smem(ring + (i % ST) * Sh::TILE);
-                for (int d = 0; d < HD; d += 16) {
-                    const uint32_t off = (d * 2 / Sh::SW) * Sh::BOX + (d * 2) % Sh::SW;
-                    mma_ss(tm + Sh::S0 + w * kKeys, operand<Sh::SW>(qa + off, 16, 8 * Sh::SW),
-                           operand<Sh::SW>(kb + off, 16, 8 * Sh::SW), iqk, d > 0);
-                }
+                product_ss<HD / 16, Sh::SW>(tm + Sh::S0 + w * kKeys, smem(qs + w * Sh::TILE), smem(ring + (i % ST) * Sh::TILE),
+                                            Sh::BOX, iqk);
                 commit(&s_ready[w]);
             };
             bool ok = bar_wait(&q_full, 0, &gone) && bar_wait(&full[0], 0, &gone);
@@ -157,10 +153,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_packed_fwd_tc(const __grid_cons
                     ok = bar_wait(&p_ready[w], j & 1, &gone);
                     if (!ok) break;
                     fence_after();
-                    const uint32_t vb = smem(ring + (vi % ST) * Sh::TILE);
+                    const uint64_t vb = operand<Sh::SW>(smem(ring + (vi % ST) * Sh::TILE), Sh::BOX, 8 * Sh::SW);
+#pragma unroll
                     for (int k = 0; k < kKeys; k += 16)
-                        mma_ts(tm + Sh::O0 + w * HD, tm + Sh::S0 + w * kKeys + k / 2,
-                               operand<Sh::SW>(vb + k * Sh::SW, Sh::BOX, 8 * Sh::SW), ipv, j > 0 || k > 0);
+                        mma_ts(tm + Sh::O0 + w * HD, tm + Sh::S0 + w * kKeys + k / 2, vb + (k * Sh::SW >> 4), ipv, j > 0 || k > 0);
                     if (j + 1 < n_tiles[w]) scores(w, ki);
                     else commit(&o_ready[w]);
                 }
@@ -201,16 +197,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_packed_fwd_tc(const __grid_cons
             }
             float x[4];
 #pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                x[b] = __uint_as_float(s[b][0]);
-                if (neg) {
-#pragma unroll
-                    for (int i = 1; i < 32; ++i) x[b] = fminf(x[b], __uint_as_float(s[b][i]));
-                } else {
-#pragma unroll
-                    for (int i = 1; i < 32; ++i) x[b] = fmaxf(x[b], __uint_as_float(s[b][i]));
-                }
-            }
+            for (int b = 0; b < 4; ++b) x[b] = neg ? smallest32(s[b]) : largest32(s[b]);
             float top = (neg ? fminf(fminf(x[0], x[1]), fminf(x[2], x[3])) : fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]))) * a.c;
             if (top == -INFINITY) top = j ? m : 0.f;
             // The reference point moves only when a weight would pass 2^8: most
@@ -231,20 +218,20 @@ __global__ void __launch_bounds__(kThreads, 1) k_packed_fwd_tc(const __grid_cons
                     st32(to + 32 * b, o);
                 }
             }
-            float add[4] = {0.f, 0.f, 0.f, 0.f};
+            const float2 c2 = both(a.c), m2 = both(-m);
+            float2 add[2] = {both(0.f), both(0.f)};
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
                 uint32_t p[16];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const float e0 = exp2_fast(fmaf(__uint_as_float(s[b][2 * i]), a.c, -m));
-                    const float e1 = exp2_fast(fmaf(__uint_as_float(s[b][2 * i + 1]), a.c, -m));
-                    add[b] += e0 + e1;
-                    p[i] = pack2<T>(e0, e1);
+                    const float2 e = exp2_both(__ffma2_rn(pair(s[b][2 * i], s[b][2 * i + 1]), c2, m2));
+                    add[i & 1] = __fadd2_rn(add[i & 1], e);
+                    p[i] = pack2<T>(e.x, e.y);
                 }
                 st16(ts + 16 * b, p);
             }
-            l += (add[0] + add[1]) + (add[2] + add[3]);
+            l += (add[0].x + add[0].y) + (add[1].x + add[1].y);
             wait_st();
             fence_before();
             bar_arrive(&p_ready[w]);
@@ -286,9 +273,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_packed_fwd_tc(const __grid_cons
 
 template <typename T, int HD>
 int launch_fwd(const FwdArgs& a, cudaStream_t s) {
-    if (cudaFuncSetAttribute(k_packed_fwd_tc<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<HD>::SMEM) !=
-        cudaSuccess)
-        return kErrCuda;
+    if (!allow_smem<&k_packed_fwd_tc<T, HD>>(Shape<HD>::SMEM)) return kErrCuda;
     const unsigned grid = (unsigned)(packed_slots(a.tokens, a.n_seqs, 2 * kRows) * a.heads);
     k_packed_fwd_tc<T, HD><<<grid, kThreads, Shape<HD>::SMEM, s>>>(a);
     return cudaGetLastError() == cudaSuccess ? kOk : kErrCuda;

@@ -6,6 +6,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 
 #include "attn_ops.h"
@@ -32,6 +33,18 @@ __device__ __forceinline__ void store4(float* p, float4 v) { *reinterpret_cast<f
 template <typename T> __device__ __forceinline__ void store4(T* p, float4 v) {
     T e[4] = {from_f32<T>(v.x), from_f32<T>(v.y), from_f32<T>(v.z), from_f32<T>(v.w)};
     *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(e);
+}
+
+// Raises a kernel's limit of dynamic shared memory, once for each device.
+template <auto* Kernel>
+bool allow_smem(int bytes) {
+    static std::atomic<unsigned long long> done{0};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { cudaGetLastError(); return false; }
+    if (done.load(std::memory_order_relaxed) >> dev & 1) return true;
+    if (cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+    done.fetch_or(1ull << dev, std::memory_order_relaxed);
+    return true;
 }
 
 // ── packed sequences ──────────────────────────────────────────────────────

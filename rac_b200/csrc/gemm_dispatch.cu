@@ -91,10 +91,6 @@ bool encode_tensor(CUtensorMap* map, CUtensorMapDataType type, int rank, const v
                    const uint64_t* strides, const uint32_t* box, int swizzle_bytes) {
     auto enc = tensor_map_encoder();
     if (!enc || rank < 2 || rank > 5 || (reinterpret_cast<uintptr_t>(base) & 15u)) return false;
-    // The encoder needs a current context, which a thread that has made no
-    // runtime call yet (an autograd worker) does not have.
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) { cudaGetLastError(); return false; }
     cuuint64_t d[5], st[4];
     cuuint32_t b[5], es[5];
     for (int i = 0; i < rank; ++i) { d[i] = dims[i]; b[i] = box[i]; es[i] = 1; }

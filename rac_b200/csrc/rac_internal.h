@@ -65,7 +65,9 @@ bool encode_tensor_2d(CUtensorMap* map, const float* base, uint64_t inner, uint6
                       long long ld, uint32_t box_inner, uint32_t box_outer, bool swizzle128);
 
 // A tensor map of any rank up to 5 and type: dims and box innermost first,
-// byte strides of the outer axes, swizzle 128, 64 or 0 bytes.
+// byte strides of the outer axes, swizzle 128, 64 or 0 bytes.  The encoder needs
+// a current context, which a thread that has made no runtime call yet (an
+// autograd worker) does not have: call cudaSetDevice first.
 bool encode_tensor(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* base, const uint64_t* dims,
                    const uint64_t* strides, const uint32_t* box, int swizzle_bytes);
 

@@ -192,5 +192,41 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 
+// The largest (smallest) of 32 values: two a step.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ float min3(float a, float b, float c) {
+    float r;
+    asm("min.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ float largest32(const uint32_t (&v)[32]) {
+    float z[2] = {__uint_as_float(v[0]), __uint_as_float(v[1])};
+#pragma unroll
+    for (int i = 2; i < 30; i += 4) {
+        z[0] = max3(z[0], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+        z[1] = max3(z[1], __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
+    }
+    return fmaxf(max3(z[0], __uint_as_float(v[30]), __uint_as_float(v[31])), z[1]);
+}
+__device__ __forceinline__ float smallest32(const uint32_t (&v)[32]) {
+    float z[2] = {__uint_as_float(v[0]), __uint_as_float(v[1])};
+#pragma unroll
+    for (int i = 2; i < 30; i += 4) {
+        z[0] = min3(z[0], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+        z[1] = min3(z[1], __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
+    }
+    return fminf(min3(z[0], __uint_as_float(v[30]), __uint_as_float(v[31])), z[1]);
+}
+// Two values at a time: one instruction where scalar code takes two, and it is
+// instructions, not the exponential unit, that bound the softmax warps (taking
+// part of the exponentials by polynomial on the FMA pipe made them slower).
+__device__ __forceinline__ float2 pair(uint32_t a, uint32_t b) { return make_float2(__uint_as_float(a), __uint_as_float(b)); }
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+__device__ __forceinline__ float2 exp2_both(float2 x) { return make_float2(exp2_fast(x.x), exp2_fast(x.y)); }
+
 }  // namespace tc
 }  // namespace racb
