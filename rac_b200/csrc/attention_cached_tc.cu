@@ -22,8 +22,13 @@ using namespace tc;
 constexpr int kRowTile = 128, kUnitRows = 256;
 // Warps 0-3, 4-7: softmax of row tile 0, 1; 8-11: loads; 12: matrix instructions; 13-15 fill the warpgroup.
 constexpr int kThreads = 512;
-constexpr int kLaunchRegs = 128, kMathRegs = 160, kLoadRegs = 104, kOtherRegs = 88;
-static_assert(kMathRegs * 256 + kLoadRegs * 128 + kOtherRegs * 128 <= kLaunchRegs * kThreads, "register split");
+// Registers: with more than 64 rows (MANY) a softmax thread holds its row's 128
+// scores, else a half or a quarter of them.
+template <bool MANY>
+struct Regs {
+    static constexpr int LAUNCH = 128, MATH = MANY ? 184 : 160, LOAD = MANY ? 80 : 104, OTHER = MANY ? 64 : 88;
+    static_assert(MATH * 256 + LOAD * 128 + OTHER * 128 <= LAUNCH * kThreads, "register split");
+};
 constexpr int kInfo = 8;                   // tiles of key masks in flight
 
 template <int HD>
@@ -65,16 +70,18 @@ __device__ __forceinline__ bool group_sync(uint64_t* bar, uint32_t& phase, volat
     return __all_sync(0xffffffffu, ok);
 }
 
-// Scores of 32 keys (columns at ts + 32 b of the thread's row); `see`: which are visible.
+// Scores that are not visible (bits of `see`) become the least there are.
+__device__ __forceinline__ void hide_scores(uint32_t (&v)[32], uint32_t see, bool neg) {
+    const uint32_t hide = neg ? 0x7f800000u : 0xff800000u;
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+        if (!(see >> i & 1)) v[i] = hide;
+}
+// Scores of 32 keys (columns at ts + 32 b of the thread's row).
 __device__ __forceinline__ void load_scores(uint32_t (&v)[32], uint32_t ts, int b, bool part, uint32_t see, bool neg) {
     ld32(v, ts + 32 * b);
     wait_ld();
-    if (part) {
-        const uint32_t hide = neg ? 0x7f800000u : 0xff800000u;
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-            if (!(see >> i & 1)) v[i] = hide;
-    }
+    if (part) hide_scores(v, see, neg);
 }
 __device__ __forceinline__ float largest(const uint32_t (&v)[32], bool neg) { return neg ? smallest32(v) : largest32(v); }
 // Weights exp2(c s - ref) of 32 keys, packed to ts + 16 b; returns their sum.
@@ -92,7 +99,7 @@ __device__ __forceinline__ float put_weights(const uint32_t (&v)[32], uint32_t t
     return (add[0].x + add[0].y) + (add[1].x + add[1].y);
 }
 
-template <typename T, int HD>
+template <typename T, int HD, bool MANY>
 __global__ void __launch_bounds__(kThreads, 1) k_cached_tc(const __grid_constant__ Args a) {
     using Sh = Shape<HD>;
     constexpr int ST = Sh::STAGES;
@@ -138,10 +145,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_cached_tc(const __grid_constant
     Segment s;
     // Two row tiles: each has a block of S columns and they take turns.  One: it
     // has both blocks, and tile g's scores lie in block g & 1.
-    const int nw = a.unit_rows > kRowTile ? 2 : 1;
+    const int nw = MANY && a.unit_rows > kRowTile ? 2 : 1;
 
     if (warp >= 12) {
-        fewer_registers<kOtherRegs>();
+        fewer_registers<Regs<MANY>::OTHER>();
         if (warp == 12 && lane == 0) {
             constexpr uint32_t iqk = instruction<T>(kRowTile, kKeys, false), ipv = instruction<T>(kRowTile, HD, true);
             int g = 0, seg = 0;            // tiles and segments so far
@@ -197,7 +204,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_cached_tc(const __grid_constant
         }
         __syncwarp();
     } else if (warp >= 8) {
-        fewer_registers<kLoadRegs>();
+        fewer_registers<Regs<MANY>::LOAD>();
         const int tid = threadIdx.x - 256;
         const char *kp = static_cast<const char*>(p.k.p), *vp = static_cast<const char*>(p.v.p);
         // A thread copies unit c of rows row0, row0 + STEP, ...; STEP is a multiple of 8,
@@ -206,7 +213,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_cached_tc(const __grid_constant
         static_assert(STEP % 8 == 0, "swizzle");
         const int c = tid % Sh::CH, row0 = tid / Sh::CH;
         const uint32_t dst0 = smem(ring) + place<HD>(row0, c);
-        const int group = p.heads / p.kv_heads, span = kRowTile / a.copies;
+        const int group = p.heads / p.kv_heads, span = MANY ? kRowTile : kRowTile / a.copies;
         const float per_group = 1.f / group;
         int e = 0, g = 0, seg = 0;                             // ring entries, tiles, segments so far
         uint32_t syncs = 0;
@@ -286,8 +293,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_cached_tc(const __grid_constant
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
     } else {
-        more_registers<kMathRegs>();
-        const int x = warp >> 2, group = p.heads / p.kv_heads, span = kRowTile / a.copies;
+        more_registers<Regs<MANY>::MATH>();
+        const int x = warp >> 2, group = p.heads / p.kv_heads, span = MANY ? kRowTile : kRowTile / a.copies;
         const int lane_row = (warp & 3) * 32 + lane, copy = lane_row / span, row = lane_row & (span - 1);
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         float* join = reinterpret_cast<float*>(sm + Sh::JOIN + x * Sh::JOIN1);
@@ -362,7 +369,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_cached_tc(const __grid_constant
                         return m == -INFINITY ? 0.f : m;
                     };
                     const uint32_t none[16] = {};
-                    if (a.copies == 4) {               // this copy's 32 keys; the others weigh the rest
+                    if (!MANY && a.copies == 4) {      // this copy's 32 keys; the others weigh the rest
                         uint32_t v[32];
                         load_scores(v, ts, copy, part, visible(copy), neg);
                         const float ref = move(largest(v, neg) * a.c);
@@ -370,7 +377,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_cached_tc(const __grid_constant
                         for (int b = 0; b < 4; ++b)
                             if (b != copy) st16(ts + 16 * b, none);
                         l += put_weights<T>(v, ts, copy, a.c, ref);
-                    } else if (a.copies == 2) {
+                    } else if (!MANY) {
                         uint32_t v[2][32];
                         const int b0 = 2 * copy;
                         load_scores(v[0], ts, b0, part, visible(b0), neg);
@@ -382,22 +389,21 @@ __global__ void __launch_bounds__(kThreads, 1) k_cached_tc(const __grid_constant
                         l += put_weights<T>(v[0], ts, b0, a.c, ref);
                         l += put_weights<T>(v[1], ts, b0 + 1, a.c, ref);
                     } else {
-                        // Read twice rather than held: the registers of 128 would not fit.
-                        float y = neg ? INFINITY : -INFINITY;
-#pragma unroll 1
-                        for (int b = 0; b < 4; ++b) {
-                            uint32_t v[32];
-                            load_scores(v, ts, b, part, visible(b), neg);
-                            const float z = largest(v, neg);
-                            y = neg ? fminf(y, z) : fmaxf(y, z);
+                        uint32_t v[4][32];
+#pragma unroll
+                        for (int b = 0; b < 4; ++b) ld32(v[b], ts + 32 * b);
+                        wait_ld();
+                        if (part) {
+#pragma unroll
+                            for (int b = 0; b < 4; ++b) hide_scores(v[b], visible(b), neg);
                         }
-                        const float ref = move(y * a.c);
-#pragma unroll 1
-                        for (int b = 0; b < 4; ++b) {
-                            uint32_t v[32];
-                            load_scores(v, ts, b, part, visible(b), neg);
-                            l += put_weights<T>(v, ts, b, a.c, ref);     // over scores that have been read
-                        }
+                        float y[4];
+#pragma unroll
+                        for (int b = 0; b < 4; ++b) y[b] = largest(v[b], neg);
+                        const float ref = move((neg ? fminf(fminf(y[0], y[1]), fminf(y[2], y[3]))
+                                                    : fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]))) * a.c);
+#pragma unroll
+                        for (int b = 0; b < 4; ++b) l += put_weights<T>(v[b], ts, b, a.c, ref);
                     }
                     if (!ok) break;
                     wait_st();
@@ -423,7 +429,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_cached_tc(const __grid_constant
                     *reinterpret_cast<float4*>(part + at) = make_float4(f[0], f[1], f[2], f[3]);
                 }
             };
-            if (a.copies > 1) {
+            if (!MANY) {
                 // The copies' sums of a row become one: each with its own reference point.
                 join_ml[lane_row] = make_float2(m, l);
                 ok = group_sync(math_sync + x, syncs, gone);
@@ -491,8 +497,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_cached_tc(const __grid_constant
 
 template <typename T, int HD>
 int launch(const Args& a, int blocks, cudaStream_t s) {
-    if (!allow_smem<&k_cached_tc<T, HD>>(Shape<HD>::SMEM)) return kErrCuda;
-    k_cached_tc<T, HD><<<blocks, kThreads, Shape<HD>::SMEM, s>>>(a);
+    if (a.copies == 1) {
+        if (!allow_smem<&k_cached_tc<T, HD, true>>(Shape<HD>::SMEM)) return kErrCuda;
+        k_cached_tc<T, HD, true><<<blocks, kThreads, Shape<HD>::SMEM, s>>>(a);
+    } else {
+        if (!allow_smem<&k_cached_tc<T, HD, false>>(Shape<HD>::SMEM)) return kErrCuda;
+        k_cached_tc<T, HD, false><<<blocks, kThreads, Shape<HD>::SMEM, s>>>(a);
+    }
     if (cudaGetLastError() != cudaSuccess) return kErrCuda;
     return launch_join<T, HD>(a, blocks, s);
 }

@@ -380,11 +380,12 @@ def _launch(name: str, args: bytes, device: int) -> None:
 
 
 def _elem(t: torch.Tensor, *more: torch.Tensor) -> int:
-    e = _ELEM.get(t.dtype)
+    dt = t.dtype
+    e = _ELEM.get(dt)
     if e is None:
-        raise ValueError(f"float32, float16 or bfloat16 tensors required, got {t.dtype}")
+        raise ValueError(f"float32, float16 or bfloat16 tensors required, got {dt}")
     for x in more:
-        if x.dtype is not t.dtype:
+        if x.dtype is not dt:
             raise ValueError(f"tensors of one type required, got {t.dtype} and {x.dtype}")
     return e
 
@@ -409,19 +410,22 @@ def _fits(t: torch.Tensor) -> bool:
 
 
 def _rows(t: torch.Tensor, width: int) -> tuple:
-    """(t or an aligned copy, its address, strides of its outer axes) for elements of `width` bytes."""
-    s = t.stride()
+    """(t or an aligned copy, its address, strides of its outer axes) for elements of `width` bytes; t has three
+    or four axes."""
     x = t.data_ptr()
-    y = x
-    for v in s[:-1]:
-        y |= v * width
-    if y & 15 or s[-1] != 1 or 0 in s:
-        if not _fits(t):
-            t = t.clone(memory_format=torch.contiguous_format)
-            x = t.data_ptr()
-        # The stride of an axis of one place may be anything.
-        s = tuple(v if n > 1 else 0 for v, n in zip(t.stride(), t.shape))
-    return t, x, s[:-1]
+    s = t.stride()
+    if len(s) == 3:
+        a, b, c = s
+        if not (x | a * width | b * width) & 15 and c == 1 and a and b:
+            return t, x, (a, b)
+    else:
+        a, b, c, e = s
+        if not (x | a * width | b * width | c * width) & 15 and e == 1 and a and b and c:
+            return t, x, (a, b, c)
+    if not _fits(t):
+        t = t.clone(memory_format=torch.contiguous_format)
+    # The stride of an axis of one place may be anything.
+    return t, t.data_ptr(), tuple(v if n > 1 else 0 for v, n in zip(t.stride()[:-1], t.shape))
 
 
 def _index(name: str, t: torch.Tensor, shape: tuple, dtype=torch.int32) -> torch.Tensor:
@@ -439,6 +443,17 @@ def _check_heads(heads: int, kv_heads: int, hd: int) -> None:
         raise ValueError(f"head size 32, 64 or 128 required, got {hd}")
     if kv_heads < 1 or heads < 1 or heads % kv_heads:
         raise ValueError(f"the query heads ({heads}) must be a multiple of the key/value heads ({kv_heads})")
+
+
+def _page_strides(t: torch.Tensor, width: int) -> tuple:
+    """Strides of the outer axes of a page tensor, which the kernels take as it lies."""
+    s = t.stride()
+    y = t.data_ptr()
+    for v in s[:-1]:
+        y |= v * width
+    if (y & 15 or s[-1] != 1 or 0 in s) and not _fits(t):
+        raise ValueError("pages need a contiguous last axis and 16-byte aligned rows")
+    return s[:-1]
 
 
 def _check_out(name: str, out: torch.Tensor, shape: tuple, dtype) -> None:
@@ -529,28 +544,27 @@ def attention_packed_backward(grad_out: torch.Tensor, q: torch.Tensor, k: torch.
     return dq, dk, dv
 
 
-def _check_pages(k_pages, v_pages, layers: bool):
-    """(type, strides [layer,] page, head, row of k, of v, pages, kv_heads, page_size, dim) of two page tensors."""
+def _check_pages(k_pages, v_pages, elem: int, layers: bool):
+    """(strides [layer,] page, head, row of k, of v, pages, kv_heads, page_size, dim) of two page tensors."""
     s = k_pages.shape
-    if len(s) != 4 and not (layers and len(s) == 5) or v_pages.shape != s:
+    n = len(s)
+    if n != 4 and not (layers and n == 5) or v_pages.shape != s:
         raise ValueError("k_pages and v_pages must be alike, " + ("[[layers,] " if layers else "[") +
                          "pages, kv_heads, page_size, dim]")
-    elem = _elem(k_pages, v_pages)
-    row = s[-1] * (2 if elem else 4)
-    if row % 16 or row > 512:
-        raise ValueError(f"pages' rows must be whole 16-byte units and 512 bytes at most, got {row}")
-    if s[-2] < 1 or s[-3] < 1:
+    pages, kv, page, hd = s if n == 4 else s[1:]
+    w = 2 if elem else 4
+    if hd * w % 16 or hd * w > 512:
+        raise ValueError(f"pages' rows must be whole 16-byte units and 512 bytes at most, got {hd * w}")
+    if page < 1 or kv < 1:
         raise ValueError("pages must hold at least one row and one head")
-    if not _fits(k_pages) or not _fits(v_pages):
-        raise ValueError("pages need a contiguous last axis and 16-byte aligned rows")
-    return elem, k_pages.stride()[:-1], v_pages.stride()[:-1], s[-4], s[-3], s[-2], s[-1]
+    return _page_strides(k_pages, w), _page_strides(v_pages, w), pages, kv, page, hd
 
 
 def _check_table(table: torch.Tensor, b: int) -> torch.Tensor:
     s = table.shape
     if len(s) != 2 or s[0] != b:
         raise ValueError(f"page_table must be [{b}, pages of the longest], got {tuple(s)}")
-    return _index("page_table", table, s)
+    return table if table.dtype is torch.int32 and table.is_contiguous() else _index("page_table", table, s)
 
 
 @functools.lru_cache(maxsize=256)
@@ -580,10 +594,13 @@ def attention_cached(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     if n > MAX_NEW_ROWS:
         raise ValueError(f"attention_cached: at most {MAX_NEW_ROWS} new rows a sequence, got {n}")
     ks = k_pages.shape
-    if len(ks) != 4 or ks[3] != hd:
+    if len(ks) != 4:
         raise ValueError(f"attention_cached: pages [pages, kv_heads, page_size, {hd}] required")
     _check_heads(h, ks[1], hd)
-    _elem(q, k_pages)
+    elem = _elem(q, k_pages, v_pages)
+    kst, vst, pages, kv, page, hd_ = _check_pages(k_pages, v_pages, elem, False)
+    if hd_ != hd:
+        raise ValueError(f"attention_cached: pages [pages, kv_heads, page_size, {hd}] required")
     table = _check_table(page_table, b)
     lens = _index("lengths", lengths, (b,))
     cnt = _index("counts", counts, (b,)) if counts is not None else None
@@ -591,7 +608,6 @@ def attention_cached(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
         if tree.dtype is not torch.int64:
             raise ValueError(f"tree must hold int64 masks, got {tree.dtype}")
         tree = _index("tree", tree, (b, n), torch.int64)
-    elem, kst, vst, pages, kv, page, _ = _check_pages(k_pages, v_pages, False)
     if out is not None:
         _check_out("out", out, qs, q.dtype)
     d = _device(q, k_pages, v_pages, table, lens, cnt, tree, out)
@@ -615,11 +631,11 @@ def cache_append_(k_pages: torch.Tensor, v_pages: torch.Tensor, k: torch.Tensor,
     s, ps = k.shape, k_pages.shape
     if len(s) != 3 or v.shape != s or len(ps) != 4 or s[1] != ps[1] or s[2] != ps[3]:
         raise ValueError(f"cache_append_: rows {tuple(s)}, {tuple(v.shape)} do not fit pages {tuple(ps)}")
-    _elem(k_pages, k, v)
+    elem = _elem(k_pages, v_pages, k, v)
     b = starts.numel()
     table, at = _check_table(page_table, b), _index("starts", starts, (b,))
     cu = _index("cu_seqlens", cu_seqlens, (b + 1,))
-    elem, kst, vst, pages, kv, page, hd = _check_pages(k_pages, v_pages, False)
+    kst, vst, pages, kv, page, hd = _check_pages(k_pages, v_pages, elem, False)
     d = _device(k_pages, v_pages, k, v, table, at, cu)
     w = 2 if elem else 4
     k, kp, ks = _rows(k, w)
@@ -640,7 +656,8 @@ def cache_copy_pages_(k_pages: torch.Tensor, v_pages: torch.Tensor, src: torch.T
     if src.dim() != 1 or dst.shape != src.shape:
         raise ValueError(f"src and dst must be 1-D and alike, got {tuple(src.shape)} and {tuple(dst.shape)}")
     s, t = _index("src", src, src.shape), _index("dst", dst, src.shape)
-    elem, kst, vst, pages, kv, page, hd = _check_pages(k_pages, v_pages, True)
+    elem = _elem(k_pages, v_pages)
+    kst, vst, pages, kv, page, hd = _check_pages(k_pages, v_pages, elem, True)
     d = _device(k_pages, v_pages, s, t)
     layers = k_pages.shape[0] if len(kst) == 4 else 1
     _launch("rac_cache_copy_pages_async", _lib.CACHE_ARGS.pack(
@@ -661,7 +678,8 @@ def cache_compact_(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: tor
         raise ValueError(f"accepted must be [{b}, at most {MAX_NEW_ROWS}], got {tuple(s)}")
     table, at = _check_table(page_table, b), _index("starts", starts, (b,))
     acc, n_acc = _index("accepted", accepted, s), _index("n_accepted", n_accepted, (b,))
-    elem, kst, vst, pages, kv, page, hd = _check_pages(k_pages, v_pages, True)
+    elem = _elem(k_pages, v_pages)
+    kst, vst, pages, kv, page, hd = _check_pages(k_pages, v_pages, elem, True)
     d = _device(k_pages, v_pages, table, at, acc, n_acc)
     layers = k_pages.shape[0] if len(kst) == 4 else 1
     _launch("rac_cache_compact_async", _lib.CACHE_ARGS.pack(
