@@ -1,13 +1,13 @@
 // attention_packed_bwd_tc.cu -- gradients of attention over packed prompts on
 // the tensor cores, float16 and bfloat16.
 //
-// Two kernels, each with its sums in tensor memory and no atomics: one keeps a
+// Two kinds of block, each with its sums in tensor memory and no atomics: one keeps a
 // tile of 128 queries and runs over the keys (dq), one keeps a tile of 128 keys
 // and runs over the queries of all heads of its group (dk and dv).  Both
 // compute S and dP anew: seven products where one kernel would do with five,
 // but dq would then be added up by atomics, in an order that changes.
 //
-// In the dk/dv kernel everything is transposed, so that P^T and dS^T have a key
+// In the dk/dv blocks everything is transposed, so that P^T and dS^T have a key
 // a lane and feed dV += P^T dO and dK += dS^T Q from tensor memory.  The order
 //   dV(i), S(i+1), dK(i), dP(i+1), dV(i+1), ...
 // keeps the tensor core at work while the weights P(i+1) are taken from S(i+1)
@@ -138,10 +138,9 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 // ── dk, dv ────────────────────────────────────────────────────────────────
 template <typename T, int HD>
-__global__ void __launch_bounds__(kThreads, 1) k_packed_dkv_tc(const __grid_constant__ BwdArgs a) {
+__device__ __forceinline__ void block_dkv(const BwdArgs& a, uint8_t* sm, unsigned block) {
     using Sh = Shape<HD>;
     constexpr int NA = Sh::A, NB = Sh::B;
-    extern __shared__ __align__(1024) uint8_t sm[];
     uint8_t *ks = sm, *vs = sm + Sh::TILE, *qr = sm + 2 * Sh::TILE, *gr = qr + NA * Sh::TILE;
     float* st_lse = reinterpret_cast<float*>(sm + Sh::STAT);       // negative; [2][128]
     float* st_d = st_lse + 2 * kTile;
@@ -153,8 +152,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_packed_dkv_tc(const __grid_cons
     volatile int* gone = reinterpret_cast<volatile int*>(tmem_base + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-    const int kvh = blockIdx.x % a.kv_heads;
-    const PackedTile t = packed_tile(a.cu, a.n_seqs, a.tokens, kTile, blockIdx.x / a.kv_heads);
+    const int kvh = block % a.kv_heads;
+    const PackedTile t = packed_tile(a.cu, a.n_seqs, a.tokens, kTile, block / a.kv_heads);
     if (t.row0 >= t.len) return;
     const long long out_row = (long long)a.kv_heads * HD;
     T* dk = static_cast<T*>(a.dk) + (t.start * a.kv_heads + kvh) * HD;
@@ -381,10 +380,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_packed_dkv_tc(const __grid_cons
 // S has two blocks of columns, so that S(j+2) can follow dQ(j), whose weights
 // dS(j) lie in S(j)'s; the order is dP(j+1), dQ(j), S(j+2).
 template <typename T, int HD>
-__global__ void __launch_bounds__(kThreads, 1) k_packed_dq_tc(const __grid_constant__ BwdArgs a) {
+__device__ __forceinline__ void block_dq(const BwdArgs& a, uint8_t* sm, unsigned block, unsigned blocks) {
     using Sh = Shape<HD>;
     constexpr int NA = Sh::A, NB = Sh::B;
-    extern __shared__ __align__(1024) uint8_t sm[];
     uint8_t *qs = sm, *gs = sm + Sh::TILE, *kr = sm + 2 * Sh::TILE, *vr = kr + NA * Sh::TILE;
     uint64_t* bars = reinterpret_cast<uint64_t*>(sm + Sh::BARS);
     uint64_t *qg_full = bars, *k_full = bars + 1, *k_empty = k_full + NA, *v_full = k_empty + NA, *v_empty = v_full + NB,
@@ -394,8 +392,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_packed_dq_tc(const __grid_const
     volatile int* gone = reinterpret_cast<volatile int*>(tmem_base + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-    const int head = blockIdx.x % a.heads, kvh = head / a.group;
-    const PackedTile t = packed_tile(a.cu, a.n_seqs, a.tokens, kTile, (gridDim.x - 1 - blockIdx.x) / a.heads);
+    const int head = block % a.heads, kvh = head / a.group;
+    const PackedTile t = packed_tile(a.cu, a.n_seqs, a.tokens, kTile, (blocks - 1 - block) / a.heads);
     if (t.row0 >= t.len) return;
     const long long out_row = (long long)a.heads * HD;
     T* dq = static_cast<T*>(a.dq) + (t.start * a.heads + head) * HD;
@@ -551,36 +549,52 @@ __global__ void __launch_bounds__(kThreads, 1) k_packed_dq_tc(const __grid_const
     if (threadIdx.x == 0 && *gone) atomicOr(a.err, kErrTcWait);
 }
 
+// One launch for both: the blocks of dq, shorter, fill the SMs that run out of dk
+// and dv (two launches one after the other: 1022 against MEASURED us for forward
+// and backward of 8192 tokens).
+template <typename T, int HD>
+__global__ void __launch_bounds__(kThreads, 1) k_packed_bwd_tc(const __grid_constant__ BwdArgs a, unsigned dkv_blocks) {
+    extern __shared__ __align__(1024) uint8_t sm[];
+    if (blockIdx.x < dkv_blocks) block_dkv<T, HD>(a, sm, blockIdx.x);
+    else block_dq<T, HD>(a, sm, blockIdx.x - dkv_blocks, gridDim.x - dkv_blocks);
+}
+
 // D = do . o of each (token, head), HD / 8 lanes a row; float16: the largest |do|
 // and |v| of the sequences' rows (blocks of y = 1 read v).
 template <typename T, int HD>
 __global__ void __launch_bounds__(256) k_packed_delta16(const PackedParams p, float* __restrict__ delta,
                                                         float* __restrict__ top) {
-    constexpr int L = HD / 8;
+    constexpr int L = HD / 8, N = 4;       // lanes of a row; rows of a thread, all read before the first is summed
     const bool is_v = blockIdx.y;
-    const int heads = is_v ? p.kv_heads : p.heads;
-    const long long r = ((long long)blockIdx.x * 256 + threadIdx.x) / L;
-    const int lane = threadIdx.x % L;
-    float m = 0.f, s = 0.f;
-    const long long used = packed_cu(p.cu, p.n_seqs, p.tokens);
-    const bool live = r < used * heads;
-    if (live) {
-        const Rows& x = is_v ? p.v : p.dout;
-        const T* row = static_cast<const T*>(x.p) + (r / heads) * x.row + (r % heads) * x.head;
-        const uint4 gu = *reinterpret_cast<const uint4*>(row + lane * 8);
-        const T* ge = reinterpret_cast<const T*>(&gu);
+    const int heads = is_v ? p.kv_heads : p.heads, lane = threadIdx.x % L;
+    const long long r0 = (long long)blockIdx.x * (N * 256 / L) + threadIdx.x / L;
+    const long long used = packed_cu(p.cu, p.n_seqs, p.tokens) * heads;
+    const Rows& x = is_v ? p.v : p.dout;
+    uint4 g[N], o[N];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(to_f32(ge[i])));
-        if (!is_v) {
-            const uint4 ou = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.out_in) + r * HD + lane * 8);
-            const T* oe = reinterpret_cast<const T*>(&ou);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) s = fmaf(to_f32(ge[i]), to_f32(oe[i]), s);
+    for (int i = 0; i < N; ++i) {
+        const long long r = r0 + i * (256 / L);
+        g[i] = o[i] = make_uint4(0, 0, 0, 0);
+        if (r < used) {
+            g[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(x.p) + (r / heads) * x.row + (r % heads) * x.head + lane * 8);
+            if (!is_v) o[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.out_in) + r * HD + lane * 8);
         }
     }
+    float m = 0.f;
 #pragma unroll
-    for (int off = L / 2; off; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-    if (live && !is_v && lane == 0) delta[(r % heads) * p.tokens + r / heads] = s;
+    for (int i = 0; i < N; ++i) {
+        const long long r = r0 + i * (256 / L);
+        const T *ge = reinterpret_cast<const T*>(&g[i]), *oe = reinterpret_cast<const T*>(&o[i]);
+        float s = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            m = fmaxf(m, fabsf(to_f32(ge[k])));
+            s = fmaf(to_f32(ge[k]), to_f32(oe[k]), s);
+        }
+#pragma unroll
+        for (int off = L / 2; off; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+        if (r < used && !is_v && lane == 0) delta[(r % heads) * p.tokens + r / heads] = s;
+    }
     if (std::is_same<T, __half>::value) {
 #pragma unroll
         for (int off = 16; off; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
@@ -595,14 +609,12 @@ int launch_bwd(const BwdArgs& a, const PackedParams& p, cudaStream_t s) {
     float* top = const_cast<float*>(a.top);
     if (f16 && cudaMemsetAsync(top, 0, 2 * sizeof(float), s) != cudaSuccess) return kErrCuda;
     const long long lanes = a.tokens * a.heads * (HD / 8);
-    k_packed_delta16<T, HD><<<dim3((unsigned)((lanes + 255) / 256), f16 ? 2 : 1), 256, 0, s>>>(
+    k_packed_delta16<T, HD><<<dim3((unsigned)((lanes + 1023) / 1024), f16 ? 2 : 1), 256, 0, s>>>(
         p, const_cast<float*>(a.delta), top);
     if (cudaGetLastError() != cudaSuccess) return kErrCuda;
     const unsigned slots = (unsigned)packed_slots(a.tokens, a.n_seqs, kTile);
-    if (!allow_smem<&k_packed_dkv_tc<T, HD>>(Sh::SMEM) || !allow_smem<&k_packed_dq_tc<T, HD>>(Sh::SMEM)) return kErrCuda;
-    k_packed_dkv_tc<T, HD><<<slots * a.kv_heads, kThreads, Sh::SMEM, s>>>(a);
-    if (cudaGetLastError() != cudaSuccess) return kErrCuda;
-    k_packed_dq_tc<T, HD><<<slots * a.heads, kThreads, Sh::SMEM, s>>>(a);
+    if (!allow_smem<&k_packed_bwd_tc<T, HD>>(Sh::SMEM)) return kErrCuda;
+    k_packed_bwd_tc<T, HD><<<slots * (a.kv_heads + a.heads), kThreads, Sh::SMEM, s>>>(a, slots * a.kv_heads);
     return cudaGetLastError() == cudaSuccess ? kOk : kErrCuda;
 }
 

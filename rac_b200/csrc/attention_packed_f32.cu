@@ -521,11 +521,10 @@ struct BwdShape {
 // dk and dv of 128 keys: query tiles pass by, of all heads of the group.
 // The order is dV(i), S(i+1), dK(i), dP(i+1); P(i) lies in S(i)'s columns, dS(i) in dP(i)'s.
 template <int HD>
-__global__ void __launch_bounds__(kThreads, 1) k_f32_dkv(const __grid_constant__ Args a) {
+__device__ __forceinline__ void block_dkv(const Args& a, uint8_t* sm, unsigned block) {
     using Sh = Shape<HD>;
     using Bs = BwdShape<HD>;
     constexpr int NA = Bs::A, NB = Bs::B, N = Bs::N, TILE = Bs::TILE, C = N / 2;
-    extern __shared__ __align__(1024) uint8_t sm[];
     uint8_t *ks = sm, *vs = sm + Bs::KEPT, *qr = sm + Bs::RING, *gr = qr + NA * TILE;
     float* st_lse = reinterpret_cast<float*>(sm + Bs::STAT);       // negative; [2][64]
     float* st_d = st_lse + 2 * N;
@@ -540,8 +539,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_dkv(const __grid_constant__
 
     // Sums of a group's heads, or of one of them.
     const int outs = a.split ? a.heads : a.kv_heads, each = a.split ? 1 : a.group;
-    const int oh = blockIdx.x % outs, kvh = a.split ? oh / a.group : oh, head0 = oh * each;
-    const PackedTile t = packed_tile(a.cu, a.n_seqs, a.tokens, kWide, blockIdx.x / outs);
+    const int oh = block % outs, kvh = a.split ? oh / a.group : oh, head0 = oh * each;
+    const PackedTile t = packed_tile(a.cu, a.n_seqs, a.tokens, kWide, block / outs);
     if (t.row0 >= t.len) return;
     const long long out_row = (long long)outs * HD;
     float* dk = a.dk + (t.start * outs + oh) * HD;
@@ -787,11 +786,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_dkv(const __grid_constant__
 // dq of 128 queries: key tiles pass by.  S has two blocks of columns, dS(j)
 // lies in S(j)'s; the order is dP(j+1), dQ(j), S(j+2).
 template <int HD>
-__global__ void __launch_bounds__(kThreads, 1) k_f32_dq(const __grid_constant__ Args a) {
+__device__ __forceinline__ void block_dq(const Args& a, uint8_t* sm, unsigned block, unsigned blocks) {
     using Sh = Shape<HD>;
     using Bs = BwdShape<HD>;
     constexpr int NA = Bs::A, NB = Bs::B, N = Bs::N, TILE = Bs::TILE, C = N / 2;
-    extern __shared__ __align__(1024) uint8_t sm[];
     uint8_t *qs = sm, *gs = sm + Bs::KEPT, *kr = sm + Bs::RING, *vr = kr + NA * TILE;
     uint64_t* bars = reinterpret_cast<uint64_t*>(sm + Bs::BARS);
     uint64_t *k_full = bars, *k_empty = k_full + NA, *v_full = k_empty + NA, *v_empty = v_full + NB, *fixed = v_empty + NB,
@@ -801,8 +799,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_dq(const __grid_constant__ 
     volatile int* gone = reinterpret_cast<volatile int*>(tmem_base + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-    const int head = blockIdx.x % a.heads, kvh = head / a.group;
-    const PackedTile t = packed_tile(a.cu, a.n_seqs, a.tokens, kWide, (gridDim.x - 1 - blockIdx.x) / a.heads);
+    const int head = block % a.heads, kvh = head / a.group;
+    const PackedTile t = packed_tile(a.cu, a.n_seqs, a.tokens, kWide, (blocks - 1 - block) / a.heads);
     if (t.row0 >= t.len) return;
     const long long out_row = (long long)a.heads * HD;
     float* dq = a.dq + (t.start * a.heads + head) * HD;
@@ -979,6 +977,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_dq(const __grid_constant__ 
     if (threadIdx.x == 0 && *gone) atomicOr(a.err, kErrTcWait);
 }
 
+// One launch for both: the blocks of dq fill the SMs that run out of dk and dv.
+template <int HD>
+__global__ void __launch_bounds__(kThreads, 1) k_f32_bwd(const __grid_constant__ Args a, unsigned dkv_blocks) {
+    extern __shared__ __align__(1024) uint8_t sm[];
+    if (blockIdx.x < dkv_blocks) block_dkv<HD>(a, sm, blockIdx.x);
+    else block_dq<HD>(a, sm, blockIdx.x - dkv_blocks, gridDim.x - dkv_blocks);
+}
+
 // dk and dv of a key/value head from those of its query heads, in their order.
 __global__ void __launch_bounds__(256) k_add_heads(const float* __restrict__ dk, const float* __restrict__ dv,
                                                    float* __restrict__ ok, float* __restrict__ ov, int group, int hd,
@@ -1048,13 +1054,6 @@ bool parts_map(CUtensorMap* m, const __half* p, long long tokens, int heads, int
     return encode_tensor(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, p, dims, strides, box, sw);
 }
 
-template <auto* Kernel>
-int go(const Args& a, int smem, unsigned grid, cudaStream_t s) {
-    if (!allow_smem<Kernel>(smem)) return kErrCuda;
-    Kernel<<<grid, kThreads, smem, s>>>(a);
-    return cudaGetLastError() == cudaSuccess ? kOk : kErrCuda;
-}
-
 template <int HD>
 int launch(const PackedParams& p, const Room& r, Args& a, bool backward, cudaStream_t s) {
     SplitArgs sp{};
@@ -1069,17 +1068,24 @@ int launch(const PackedParams& p, const Room& r, Args& a, bool backward, cudaStr
     const unsigned slots = (unsigned)packed_slots(p.tokens, p.n_seqs, kSplit);
     k_split<HD><<<slots * sp.first[4], 256, 0, s>>>(sp);
     if (cudaGetLastError() != cudaSuccess) return kErrCuda;
-    if (!backward) return go<&k_f32_fwd<HD>>(a, FwdShape<HD>::SMEM, slots * p.heads, s);
+    if (!backward) {
+        if (!allow_smem<&k_f32_fwd<HD>>(FwdShape<HD>::SMEM)) return kErrCuda;
+        k_f32_fwd<HD><<<slots * p.heads, kThreads, FwdShape<HD>::SMEM, s>>>(a);
+        return cudaGetLastError() == cudaSuccess ? kOk : kErrCuda;
+    }
     a.split = by_head(p.tokens, p.heads, p.kv_heads);
     if (a.split) { a.dk = r.dk; a.dv = r.dv; }
-    if (int st = go<&k_f32_dkv<HD>>(a, BwdShape<HD>::SMEM, slots * (a.split ? p.heads : p.kv_heads), s)) return st;
+    const unsigned dkv_blocks = slots * (a.split ? p.heads : p.kv_heads);
+    if (!allow_smem<&k_f32_bwd<HD>>(BwdShape<HD>::SMEM)) return kErrCuda;
+    k_f32_bwd<HD><<<dkv_blocks + slots * p.heads, kThreads, BwdShape<HD>::SMEM, s>>>(a, dkv_blocks);
+    if (cudaGetLastError() != cudaSuccess) return kErrCuda;
     if (a.split) {
         const long long n = p.tokens * p.kv_heads * (HD / 4);
         k_add_heads<<<(unsigned)((n + 255) / 256), 256, 0, s>>>(r.dk, r.dv, static_cast<float*>(p.dk),
                                                                 static_cast<float*>(p.dv), a.group, HD, n);
         if (cudaGetLastError() != cudaSuccess) return kErrCuda;
     }
-    return go<&k_f32_dq<HD>>(a, BwdShape<HD>::SMEM, slots * p.heads, s);
+    return kOk;
 }
 
 }  // namespace
