@@ -145,7 +145,7 @@ __device__ __forceinline__ void block_dkv(const BwdArgs& a, uint8_t* sm, unsigne
     float* st_lse = reinterpret_cast<float*>(sm + Sh::STAT);       // negative; [2][128]
     float* st_d = st_lse + 2 * kTile;
     uint64_t* bars = reinterpret_cast<uint64_t*>(sm + Sh::BARS);
-    uint64_t *kv_full = bars, *q_full = bars + 1, *q_empty = q_full + NA, *g_full = q_empty + NA, *g_empty = g_full + NB,
+    uint64_t *kv_full = bars, *q_full = bars + 2, *q_empty = q_full + NA, *g_full = q_empty + NA, *g_empty = g_full + NB,
              *stat_full = g_empty + NB, *stat_empty = stat_full + 2, *s_ready = stat_empty + 2, *dp_ready = s_ready + 1,
              *p_ready = dp_ready + 1, *ds_ready = p_ready + 1, *done = ds_ready + 1, *fixed = done + 1;
     uint32_t* tmem_base = reinterpret_cast<uint32_t*>(fixed + NB);
@@ -168,9 +168,12 @@ __device__ __forceinline__ void block_dkv(const BwdArgs& a, uint8_t* sm, unsigne
     const int n = nq * a.group;
     const bool ragged = t.len % kTile != 0;                        // the last query tile of each head
 
-    if (threadIdx.x == 0) {
+    // The loading thread sets up the barriers and sends for the first tiles while
+    // tensor memory is allocated: a block's first product waits for little else.
+    if (threadIdx.x == 32 * 9) {
         *gone = 0;
         bar_init(kv_full, 1);
+        bar_init(kv_full + 1, 1);
         for (int i = 0; i < NA; ++i) { bar_init(q_full + i, 1); bar_init(q_empty + i, 1); }
         for (int i = 0; i < NB; ++i) { bar_init(g_full + i, 1); bar_init(g_empty + i, 1); }
         for (int i = 0; i < 2; ++i) { bar_init(stat_full + i, 1); bar_init(stat_empty + i, 256); }
@@ -178,6 +181,15 @@ __device__ __forceinline__ void block_dkv(const BwdArgs& a, uint8_t* sm, unsigne
         bar_init(done, 1);
         for (int i = 0; i < NB; ++i) bar_init(fixed + i, 1);
         bar_init_done();
+        const int k0 = (int)t.start + t.row0, q0 = (int)t.start + first * kTile;
+        bar_expect(kv_full, Sh::TILE);
+        load_tile<HD>(ks, &a.k, kvh, k0, kv_full);
+        bar_expect(q_full, Sh::TILE);
+        load_tile<HD>(qr, &a.q, kvh * a.group, q0, q_full);
+        bar_expect(kv_full + 1, Sh::TILE);
+        load_tile<HD>(vs, &a.v, kvh, k0, kv_full + 1);
+        bar_expect(g_full, Sh::TILE);
+        load_tile<HD>(gr, &a.g, kvh * a.group, q0, g_full);
     }
     if (warp == 8) tmem_alloc(tmem_base, 512);
     fence_before();
@@ -190,11 +202,6 @@ __device__ __forceinline__ void block_dkv(const BwdArgs& a, uint8_t* sm, unsigne
         if (warp == 9) {
             auto head_of = [&](int i) { return kvh * a.group + i / nq; };
             auto row_of = [&](int i) { return (int)t.start + (first + i % nq) * kTile; };
-            if (lane == 0) {
-                bar_expect(kv_full, 2 * Sh::TILE);
-                load_tile<HD>(ks, &a.k, kvh, (int)t.start + t.row0, kv_full);
-                load_tile<HD>(vs, &a.v, kvh, (int)t.start + t.row0, kv_full);
-            }
             bool ok = true;
             // Entry i is loaded as soon as its places are free; in a sequence's last
             // tile the rows behind it are cleared once they have landed: the weights
@@ -205,7 +212,7 @@ __device__ __forceinline__ void block_dkv(const BwdArgs& a, uint8_t* sm, unsigne
                 if (ok && i >= NB) ok = bar_wait(g_empty + sb, (i / NB - 1) & 1, gone);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
-                if (lane == 0) {
+                if (lane == 0 && i) {
                     bar_expect(q_full + sa, Sh::TILE);
                     load_tile<HD>(qr + sa * Sh::TILE, &a.q, head_of(i), row_of(i), q_full + sa);
                     bar_expect(g_full + sb, Sh::TILE);
@@ -230,7 +237,7 @@ __device__ __forceinline__ void block_dkv(const BwdArgs& a, uint8_t* sm, unsigne
                 if (ok) {
                     mma_rows<T, HD>(tS, ks, qr);
                     commit(s_ready);
-                    ok = bar_wait(g_full, 0, gone);
+                    ok = bar_wait(kv_full + 1, 0, gone) && bar_wait(g_full, 0, gone);
                 }
                 if (ok) {
                     mma_rows<T, HD>(tP, vs, gr);
@@ -385,7 +392,7 @@ __device__ __forceinline__ void block_dq(const BwdArgs& a, uint8_t* sm, unsigned
     constexpr int NA = Sh::A, NB = Sh::B;
     uint8_t *qs = sm, *gs = sm + Sh::TILE, *kr = sm + 2 * Sh::TILE, *vr = kr + NA * Sh::TILE;
     uint64_t* bars = reinterpret_cast<uint64_t*>(sm + Sh::BARS);
-    uint64_t *qg_full = bars, *k_full = bars + 1, *k_empty = k_full + NA, *v_full = k_empty + NA, *v_empty = v_full + NB,
+    uint64_t *qg_full = bars, *k_full = bars + 2, *k_empty = k_full + NA, *v_full = k_empty + NA, *v_empty = v_full + NB,
              *s_ready = v_empty + NB, *dp_ready = s_ready + 2, *ds_ready = dp_ready + 1, *done = ds_ready + 1,
              *fixed = done + 1;
     uint32_t* tmem_base = reinterpret_cast<uint32_t*>(fixed + 1);
@@ -405,14 +412,24 @@ __device__ __forceinline__ void block_dq(const BwdArgs& a, uint8_t* sm, unsigned
     const int n = (last + kTile - 1) / kTile;
     const bool ragged = n * kTile > t.len;
 
-    if (threadIdx.x == 0) {
+    if (threadIdx.x == 32 * 9) {
         *gone = 0;
         bar_init(qg_full, 1);
+        bar_init(qg_full + 1, 1);
         for (int i = 0; i < NA; ++i) { bar_init(k_full + i, 1); bar_init(k_empty + i, 1); }
         for (int i = 0; i < NB; ++i) { bar_init(v_full + i, 1); bar_init(v_empty + i, 1); }
         bar_init(s_ready, 1); bar_init(s_ready + 1, 1); bar_init(dp_ready, 1); bar_init(ds_ready, 256);
         bar_init(done, 1); bar_init(fixed, 1);
         bar_init_done();
+        const int r0 = (int)t.start;
+        bar_expect(qg_full, Sh::TILE);
+        load_tile<HD>(qs, &a.q, head, r0 + t.row0, qg_full);
+        bar_expect(k_full, Sh::TILE);
+        load_tile<HD>(kr, &a.k, kvh, r0, k_full);
+        bar_expect(qg_full + 1, Sh::TILE);
+        load_tile<HD>(gs, &a.g, head, r0 + t.row0, qg_full + 1);
+        bar_expect(v_full, Sh::TILE);
+        load_tile<HD>(vr, &a.v, kvh, r0, v_full);
     }
     if (warp == 8) tmem_alloc(tmem_base, 512);
     fence_before();
@@ -425,10 +442,7 @@ __device__ __forceinline__ void block_dq(const BwdArgs& a, uint8_t* sm, unsigned
         if (warp == 9) {
             if (lane == 0) {
                 const int r0 = (int)t.start;
-                bar_expect(qg_full, 2 * Sh::TILE);
-                load_tile<HD>(qs, &a.q, head, r0 + t.row0, qg_full);
-                load_tile<HD>(gs, &a.g, head, r0 + t.row0, qg_full);
-                for (int j = 0; j < n; ++j) {
+                for (int j = 1; j < n; ++j) {
                     const int sa = j % NA, sb = j % NB;
                     if (j >= NA && !bar_wait(k_empty + sa, (j / NA - 1) & 1, gone)) break;
                     bar_expect(k_full + sa, Sh::TILE);
@@ -464,7 +478,7 @@ __device__ __forceinline__ void block_dq(const BwdArgs& a, uint8_t* sm, unsigned
                     commit(v_empty + j % NB);
                     return true;
                 };
-                bool ok = bar_wait(qg_full, 0, gone) && scores(0) && dps(0);
+                bool ok = bar_wait(qg_full, 0, gone) && scores(0) && bar_wait(qg_full + 1, 0, gone) && dps(0);
                 if (ok && n > 1) ok = scores(1);
                 for (int j = 0; ok && j < n; ++j) {
                     ok = bar_wait(ds_ready, j & 1, gone);

@@ -530,7 +530,7 @@ __device__ __forceinline__ void block_dkv(const Args& a, uint8_t* sm, unsigned b
     float* st_d = st_lse + 2 * N;
     uint64_t* bars = reinterpret_cast<uint64_t*>(sm + Bs::BARS);
     uint64_t *q_full = bars, *q_empty = q_full + NA, *q_fixed = q_empty + NA, *g_full = q_fixed + NA, *g_empty = g_full + NB,
-             *g_fixed = g_empty + NB, *kv_full = g_fixed + NB, *stat_full = kv_full + 1,
+             *g_fixed = g_empty + NB, *kv_full = g_fixed + NB, *stat_full = kv_full + 2,
              *stat_empty = stat_full + 2, *s_ready = stat_empty + 2, *dp_ready = s_ready + 1, *p_ready = dp_ready + 1,
              *ds_ready = p_ready + 1, *dv_done = ds_ready + 1, *dk_done = dv_done + 1;
     uint32_t* tmem_base = reinterpret_cast<uint32_t*>(dk_done + 1);
@@ -555,15 +555,26 @@ __device__ __forceinline__ void block_dkv(const Args& a, uint8_t* sm, unsigned b
     const int n = nq * each;
     const bool ragged = t.len % N != 0;                      // the last query tile of each head
 
-    if (threadIdx.x == 0) {
+    // As in the 16-bit kernels, the first tiles are under way before the block meets.
+    if (threadIdx.x == 32 * 9) {
         *gone = 0;
         for (int i = 0; i < NA; ++i) { bar_init(q_full + i, 1); bar_init(q_empty + i, 1); bar_init(q_fixed + i, 1); }
         for (int i = 0; i < NB; ++i) { bar_init(g_full + i, 1); bar_init(g_empty + i, 1); bar_init(g_fixed + i, 1); }
         bar_init(kv_full, 1);
+        bar_init(kv_full + 1, 1);
         for (int i = 0; i < 2; ++i) { bar_init(stat_full + i, 1); bar_init(stat_empty + i, 256); }
         bar_init(s_ready, 1); bar_init(dp_ready, 1); bar_init(p_ready, 256); bar_init(ds_ready, 256);
         bar_init(dv_done, 1); bar_init(dk_done, 1);
         bar_init_done();
+        const int k0 = (int)t.start + t.row0, q0 = (int)t.start + first * N;
+        bar_expect(kv_full, Bs::KEPT);
+        load_parts<HD, kWide>(ks, &a.k, kvh, a.kv_heads, k0, kv_full);
+        bar_expect(q_full, TILE);
+        load_parts<HD, N>(qr, &a.q, head0, a.heads, q0, q_full);
+        bar_expect(kv_full + 1, Bs::KEPT);
+        load_parts<HD, kWide>(vs, &a.v, kvh, a.kv_heads, k0, kv_full + 1);
+        bar_expect(g_full, TILE);
+        load_parts<HD, N>(gr, &a.g, head0, a.heads, q0, g_full);
     }
     if (warp == 8) tmem_alloc(tmem_base, 512);
     fence_before();
@@ -578,16 +589,11 @@ __device__ __forceinline__ void block_dkv(const Args& a, uint8_t* sm, unsigned b
         if (warp == 9) {
             // `fixed` tells that the rows behind the sequence are cleared (their weights
             // are 0, 0 times another sequence's NaN is not).
-            if (lane == 0) {
-                bar_expect(kv_full, 2 * Bs::KEPT);
-                load_parts<HD, kWide>(ks, &a.k, kvh, a.kv_heads, (int)t.start + t.row0, kv_full);
-                load_parts<HD, kWide>(vs, &a.v, kvh, a.kv_heads, (int)t.start + t.row0, kv_full);
-            }
             auto load = [&](const CUtensorMap* m, int i, uint8_t* r, uint64_t* full, uint64_t* empty, uint64_t* fixed, int n_places) {
                 const int st = i % n_places;
                 uint8_t* dst = r + st * TILE;
                 if (!__all_sync(0xffffffffu, i < n_places || bar_wait(empty + st, (i / n_places - 1) & 1, gone))) return false;
-                if (lane == 0) {
+                if (lane == 0 && i) {
                     bar_expect(full + st, TILE);
                     load_parts<HD, N>(dst, m, head_of(i), a.heads, (int)t.start + row_of(i), full + st);
                 }
@@ -619,7 +625,7 @@ __device__ __forceinline__ void block_dkv(const Args& a, uint8_t* sm, unsigned b
                     commit(dp_ready);
                     return true;
                 };
-                bool ok = bar_wait(kv_full, 0, gone) && scores(0) && dps(0);
+                bool ok = bar_wait(kv_full, 0, gone) && scores(0) && bar_wait(kv_full + 1, 0, gone) && dps(0);
                 for (int i = 0; ok && i < n; ++i) {
                     const bool more = i + 1 < n;
                     ok = bar_wait(p_ready, i & 1, gone);
@@ -793,7 +799,7 @@ __device__ __forceinline__ void block_dq(const Args& a, uint8_t* sm, unsigned bl
     uint8_t *qs = sm, *gs = sm + Bs::KEPT, *kr = sm + Bs::RING, *vr = kr + NA * TILE;
     uint64_t* bars = reinterpret_cast<uint64_t*>(sm + Bs::BARS);
     uint64_t *k_full = bars, *k_empty = k_full + NA, *v_full = k_empty + NA, *v_empty = v_full + NB, *fixed = v_empty + NB,
-             *qg_full = fixed + 1, *s_ready = qg_full + 1,
+             *qg_full = fixed + 1, *s_ready = qg_full + 2,
              *dp_ready = s_ready + 2, *ds_ready = dp_ready + 1, *dq_done = ds_ready + 1;
     uint32_t* tmem_base = reinterpret_cast<uint32_t*>(dq_done + 1);
     volatile int* gone = reinterpret_cast<volatile int*>(tmem_base + 1);
@@ -812,13 +818,22 @@ __device__ __forceinline__ void block_dq(const Args& a, uint8_t* sm, unsigned bl
     const int n = (last + N - 1) / N;
     const bool ragged = n * N > t.len;
 
-    if (threadIdx.x == 0) {
+    if (threadIdx.x == 32 * 9) {
         *gone = 0;
         for (int i = 0; i < NA; ++i) { bar_init(k_full + i, 1); bar_init(k_empty + i, 1); }
         for (int i = 0; i < NB; ++i) { bar_init(v_full + i, 1); bar_init(v_empty + i, 1); }
-        bar_init(fixed, 1); bar_init(qg_full, 1); bar_init(s_ready, 1); bar_init(s_ready + 1, 1);
+        bar_init(fixed, 1); bar_init(qg_full, 1); bar_init(qg_full + 1, 1); bar_init(s_ready, 1); bar_init(s_ready + 1, 1);
         bar_init(dp_ready, 1); bar_init(ds_ready, 256); bar_init(dq_done, 1);
         bar_init_done();
+        const int r0 = (int)t.start;
+        bar_expect(qg_full, Bs::KEPT);
+        load_parts<HD, kWide>(qs, &a.q, head, a.heads, r0 + t.row0, qg_full);
+        bar_expect(k_full, TILE);
+        load_parts<HD, N>(kr, &a.k, kvh, a.kv_heads, r0, k_full);
+        bar_expect(qg_full + 1, Bs::KEPT);
+        load_parts<HD, kWide>(gs, &a.g, head, a.heads, r0 + t.row0, qg_full + 1);
+        bar_expect(v_full, TILE);
+        load_parts<HD, N>(vr, &a.v, kvh, a.kv_heads, r0, v_full);
     }
     if (warp == 8) tmem_alloc(tmem_base, 512);
     fence_before();
@@ -831,10 +846,7 @@ __device__ __forceinline__ void block_dq(const Args& a, uint8_t* sm, unsigned bl
         if (warp == 9) {
             if (lane == 0) {
                 const int r0 = (int)t.start;
-                bar_expect(qg_full, 2 * Bs::KEPT);
-                load_parts<HD, kWide>(qs, &a.q, head, a.heads, r0 + t.row0, qg_full);
-                load_parts<HD, kWide>(gs, &a.g, head, a.heads, r0 + t.row0, qg_full);
-                for (int j = 0; j < n; ++j) {
+                for (int j = 1; j < n; ++j) {
                     const int sa = j % NA, sb = j % NB;
                     if (j >= NA && !bar_wait(k_empty + sa, (j / NA - 1) & 1, gone)) break;
                     bar_expect(k_full + sa, TILE);
@@ -869,7 +881,7 @@ __device__ __forceinline__ void block_dq(const Args& a, uint8_t* sm, unsigned bl
                     commit(v_empty + j % NB);
                     return true;
                 };
-                bool ok = bar_wait(qg_full, 0, gone) && scores(0) && dps(0);
+                bool ok = bar_wait(qg_full, 0, gone) && scores(0) && bar_wait(qg_full + 1, 0, gone) && dps(0);
                 if (ok && n > 1) ok = scores(1);
                 for (int j = 0; ok && j < n; ++j) {
                     ok = bar_wait(ds_ready, j & 1, gone);

@@ -44,7 +44,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_packed_fwd_tc(const __grid_cons
     using Sh = Shape<HD>;
     constexpr int ST = Sh::STAGES;
     extern __shared__ uint8_t raw[];
-    __shared__ uint64_t q_full, full[ST], empty[ST], fixed, s_ready[2], p_ready[2], o_ready[2];
+    __shared__ uint64_t q_full[2], full[ST], empty[ST], fixed, s_ready[2], p_ready[2], o_ready[2];
     __shared__ uint32_t tmem_base;
     __shared__ int gone;
     uint8_t* base = raw + ((1024 - (smem(raw) & 1023)) & 1023);
@@ -76,13 +76,26 @@ __global__ void __launch_bounds__(kThreads, 1) k_packed_fwd_tc(const __grid_cons
     const int n = max(n_tiles[0], n_tiles[1]);
     const bool ragged = n * kKeys > t.len;    // the last key tile runs into the next sequence
 
-    if (threadIdx.x == 0) {
+    // The loading thread sets up the barriers and sends for the first tiles while
+    // tensor memory is allocated: a block's first product waits for little else.
+    if (threadIdx.x == 32 * 9) {
         gone = 0;
-        bar_init(&q_full, 1);
+        bar_init(&q_full[0], 1);
+        bar_init(&q_full[1], 1);
         bar_init(&fixed, 1);
         for (int i = 0; i < ST; ++i) { bar_init(&full[i], 1); bar_init(&empty[i], 1); }
         for (int w = 0; w < 2; ++w) { bar_init(&s_ready[w], 1); bar_init(&p_ready[w], kRows); bar_init(&o_ready[w], 1); }
         bar_init_done();
+        for (int w = 0; w < 2 && n_tiles[w]; ++w) {
+            bar_expect(&q_full[w], Sh::TILE);
+            for (int b = 0; b < Sh::BOXES; ++b)
+                load_3d(qs + w * Sh::TILE + b * Sh::BOX, &a.q, b * (Sh::SW / 2), head, (int)t.start + t.row0 + w * kRows,
+                        &q_full[w]);
+            if (w) break;
+            bar_expect(&full[0], Sh::TILE);
+            for (int b = 0; b < Sh::BOXES; ++b)
+                load_3d(ring + b * Sh::BOX, &a.k, b * (Sh::SW / 2), kvh, (int)t.start, &full[0]);
+        }
     }
     if (warp == 8) tmem_alloc(&tmem_base, 512);
     fence_before();
@@ -95,13 +108,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_packed_fwd_tc(const __grid_cons
     if (warp == 9) {
         // ── loads: K0, V0, K1, V1, ... through the ring ──
         if (lane == 0) {
-            bar_expect(&q_full, (n_tiles[1] ? 2 : 1) * Sh::TILE);
-            for (int w = 0; w < 2; ++w)
-                if (n_tiles[w])
-                    for (int b = 0; b < Sh::BOXES; ++b)
-                        load_3d(qs + w * Sh::TILE + b * Sh::BOX, &a.q, b * (Sh::SW / 2), head,
-                                (int)t.start + t.row0 + w * kRows, &q_full);
-            for (int i = 0; i < 2 * n; ++i) {
+            for (int i = 1; i < 2 * n; ++i) {
                 const int st = i % ST;
                 if (i >= ST && !bar_wait(&empty[st], (i / ST - 1) & 1, &gone)) break;
                 bar_expect(&full[st], Sh::TILE);
@@ -137,12 +144,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_packed_fwd_tc(const __grid_cons
                                             Sh::BOX, iqk);
                 commit(&s_ready[w]);
             };
-            bool ok = bar_wait(&q_full, 0, &gone) && bar_wait(&full[0], 0, &gone);
-            if (ok) {
-                for (int w = 0; w < 2; ++w)
-                    if (n_tiles[w]) scores(w, 0);
-                commit(&empty[0]);
+            bool ok = bar_wait(&full[0], 0, &gone);
+            for (int w = 0; ok && w < 2; ++w) {
+                if (!n_tiles[w]) continue;
+                ok = bar_wait(&q_full[w], 0, &gone);
+                if (ok) scores(w, 0);
             }
+            if (ok) commit(&empty[0]);
             for (int j = 0; ok && j < n; ++j) {
                 const int vi = 2 * j + 1, ki = 2 * j + 2;
                 ok = bar_wait(&full[vi % ST], (vi / ST) & 1, &gone);
