@@ -187,7 +187,13 @@ int rac_check_device_errors(void *stream);
  * behind the last sequence stay as they are, or become zeros where zero_rest
  * is set.
  *
- * The backward call takes the forward's out and lse and the output's gradient
+ * out_low (optional, like out; 16-bit types): what rounding took from out's
+ * first 128 rows of each sequence, where few keys share the weight and the
+ * gradients feel it most.  With it the forward keeps the weights of those
+ * rows' keys to twice the digits, and the backward, given it, takes D = do . o
+ * from both.
+ *
+ * The backward call takes the forward's out, lse and out_low and the output's gradient
  * dout, and writes dq like q, dk and dv like k (contiguous), zeros behind the
  * last sequence.  The same inputs give the same bits.
  *
@@ -198,6 +204,7 @@ typedef struct {
     const int *cu_seqlens;
     void *out;
     float *lse;
+    void *out_low;                        /* optional, 16-bit types, see above */
     const void *dout;                     /* backward */
     void *dq, *dk, *dv;                   /* backward */
     void *workspace;

@@ -36,7 +36,7 @@ class Float2(C.Structure):
 
 
 # The argument structures of rac_b200.h section 4, field for field.
-PACKED_ARGS = struct.Struct("11P8q2q7if")   # rac_attention_packed_args
+PACKED_ARGS = struct.Struct("12P8q2q7if")   # rac_attention_packed_args
 CACHED_ARGS = struct.Struct("9P9qq10if4x")  # rac_attention_cached_args
 CACHE_ARGS = struct.Struct("11P12qq9i4x")   # rac_cache_args
 

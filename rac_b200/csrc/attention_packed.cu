@@ -58,7 +58,7 @@ int attention_packed(const PackedParams& p, cudaStream_t s) {
     if (int st = check(p)) return st;
     if (p.tokens == 0) return kOk;
     if (!p.out) return kErrNullPtr;
-    if (reinterpret_cast<uintptr_t>(p.out) & 15u) return kErrUnsupported;
+    if ((reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.low)) & 15u) return kErrUnsupported;
     if (!room_ok(p, 0)) return kErrAlloc;
     if (int st = bind_device()) return st;
     return p.type == kF32 ? attention_packed_f32(p, 0, s) : attention_packed_tc(p, s);
@@ -70,7 +70,7 @@ int attention_packed_backward(const PackedParams& p, cudaStream_t s) {
     if (!p.dout.p || !p.out_in || !p.lse_in || !p.dq || !p.dk || !p.dv) return kErrNullPtr;
     if (!rows_ok(p.dout, p.type)) return kErrUnsupported;
     if (!room_ok(p, 1)) return kErrAlloc;
-    for (const void* x : {p.out_in, (const void*)p.dq, (const void*)p.dk, (const void*)p.dv})
+    for (const void* x : {p.out_in, (const void*)p.low, (const void*)p.dq, (const void*)p.dk, (const void*)p.dv})
         if (reinterpret_cast<uintptr_t>(x) & 15u) return kErrUnsupported;
     if (int st = bind_device()) return st;
     return p.type == kF32 ? attention_packed_f32(p, 1, s) : attention_packed_backward_tc(p, s);

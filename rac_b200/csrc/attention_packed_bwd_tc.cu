@@ -573,31 +573,37 @@ __global__ void __launch_bounds__(kThreads, 1) k_packed_bwd_tc(const __grid_cons
     else block_dq<T, HD>(a, sm, blockIdx.x - dkv_blocks, gridDim.x - dkv_blocks);
 }
 
-// D = do . o of each (token, head), HD / 8 lanes a row; float16: the largest |do|
-// and |v| of the sequences' rows (blocks of y = 1 read v).
+// D = do . o of the rows of a tile of one head, HD / 8 lanes a row; in a
+// sequence's first tile o is the sum of what was stored and what rounding took
+// from it.  float16: the largest |do| and |v| (blocks of y = 1 read v).  Every
+// row of a thread is read before the first is summed.
 template <typename T, int HD>
 __global__ void __launch_bounds__(256) k_packed_delta16(const PackedParams p, float* __restrict__ delta,
                                                         float* __restrict__ top) {
-    constexpr int L = HD / 8, N = 4;       // lanes of a row; rows of a thread, all read before the first is summed
+    constexpr int L = HD / 8, STEP = 256 / L, N = kTile / STEP;
     const bool is_v = blockIdx.y;
-    const int heads = is_v ? p.kv_heads : p.heads, lane = threadIdx.x % L;
-    const long long r0 = (long long)blockIdx.x * (N * 256 / L) + threadIdx.x / L;
-    const long long used = packed_cu(p.cu, p.n_seqs, p.tokens) * heads;
+    const int heads = is_v ? p.kv_heads : p.heads, head = blockIdx.x % p.heads, lane = threadIdx.x % L;
+    if (head >= heads) return;
+    const PackedTile t = packed_tile(p.cu, p.n_seqs, p.tokens, kTile, blockIdx.x / p.heads);
+    if (t.row0 >= t.len || t.seq == p.n_seqs) return;
     const Rows& x = is_v ? p.v : p.dout;
+    const T* in = static_cast<const T*>(x.p) + t.start * x.row + head * x.head + lane * 8;
+    const long long at = (t.start * p.heads + head) * HD + lane * 8, row = (long long)p.heads * HD;
+    const bool fine = p.low && t.row0 == 0;
     uint4 g[N], o[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        const long long r = r0 + i * (256 / L);
+        const int r = t.row0 + threadIdx.x / L + i * STEP;
         g[i] = o[i] = make_uint4(0, 0, 0, 0);
-        if (r < used) {
-            g[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(x.p) + (r / heads) * x.row + (r % heads) * x.head + lane * 8);
-            if (!is_v) o[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.out_in) + r * HD + lane * 8);
+        if (r < t.len) {
+            g[i] = *reinterpret_cast<const uint4*>(in + r * x.row);
+            if (!is_v) o[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.out_in) + at + r * row);
         }
     }
     float m = 0.f;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        const long long r = r0 + i * (256 / L);
+        const int r = t.row0 + threadIdx.x / L + i * STEP;
         const T *ge = reinterpret_cast<const T*>(&g[i]), *oe = reinterpret_cast<const T*>(&o[i]);
         float s = 0.f;
 #pragma unroll
@@ -605,9 +611,15 @@ __global__ void __launch_bounds__(256) k_packed_delta16(const PackedParams p, fl
             m = fmaxf(m, fabsf(to_f32(ge[k])));
             s = fmaf(to_f32(ge[k]), to_f32(oe[k]), s);
         }
+        if (fine && !is_v && r < t.len) {
+            const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.low) + at + r * row);
+            const T* ue = reinterpret_cast<const T*>(&u);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) s = fmaf(to_f32(ge[k]), to_f32(ue[k]), s);
+        }
 #pragma unroll
         for (int off = L / 2; off; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-        if (r < used && !is_v && lane == 0) delta[(r % heads) * p.tokens + r / heads] = s;
+        if (r < t.len && !is_v && lane == 0) delta[head * p.tokens + t.start + r] = s;
     }
     if (std::is_same<T, __half>::value) {
 #pragma unroll
@@ -622,11 +634,9 @@ int launch_bwd(const BwdArgs& a, const PackedParams& p, cudaStream_t s) {
     const bool f16 = std::is_same<T, __half>::value;
     float* top = const_cast<float*>(a.top);
     if (f16 && cudaMemsetAsync(top, 0, 2 * sizeof(float), s) != cudaSuccess) return kErrCuda;
-    const long long lanes = a.tokens * a.heads * (HD / 8);
-    k_packed_delta16<T, HD><<<dim3((unsigned)((lanes + 1023) / 1024), f16 ? 2 : 1), 256, 0, s>>>(
-        p, const_cast<float*>(a.delta), top);
-    if (cudaGetLastError() != cudaSuccess) return kErrCuda;
     const unsigned slots = (unsigned)packed_slots(a.tokens, a.n_seqs, kTile);
+    k_packed_delta16<T, HD><<<dim3(slots * a.heads, f16 ? 2 : 1), 256, 0, s>>>(p, const_cast<float*>(a.delta), top);
+    if (cudaGetLastError() != cudaSuccess) return kErrCuda;
     if (!allow_smem<&k_packed_bwd_tc<T, HD>>(Sh::SMEM)) return kErrCuda;
     k_packed_bwd_tc<T, HD><<<slots * (a.kv_heads + a.heads), kThreads, Sh::SMEM, s>>>(a, slots * a.kv_heads);
     return cudaGetLastError() == cudaSuccess ? kOk : kErrCuda;

@@ -34,7 +34,7 @@ PackedParams packed(const rac_attention_packed_args& a) {
     p.cu = a.cu_seqlens; p.n_seqs = a.n_seqs; p.tokens = a.tokens;
     p.heads = a.heads; p.kv_heads = a.kv_heads; p.head_dim = a.head_dim;
     p.type = a.dtype; p.causal = a.is_causal; p.scale = a.scale;
-    p.out = a.out; p.lse = a.lse; p.zero_rest = a.zero_rest;
+    p.out = a.out; p.lse = a.lse; p.low = a.out_low; p.zero_rest = a.zero_rest;
     p.out_in = a.out; p.lse_in = a.lse;
     p.dq = a.dq; p.dk = a.dk; p.dv = a.dv;
     p.ws = a.workspace; p.ws_bytes = a.ws_bytes > 0 ? (size_t)a.ws_bytes : 0;

@@ -25,6 +25,7 @@ struct PackedParams {
     float scale;
     void* out;            // [tokens, heads, head_dim]
     float* lse;           // [heads, tokens], natural log; may be null forward
+    void* low;            // like out: what rounding took from each sequence's first 128 rows; may be null
     int zero_rest;        // write zeros to the rows behind the last sequence
     // backward
     Rows dout;

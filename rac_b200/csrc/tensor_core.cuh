@@ -186,6 +186,12 @@ template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
+template <typename T> __device__ __forceinline__ float low_of(uint32_t p) {
+    return std::is_same<T, __half>::value ? __low2float(*reinterpret_cast<const __half2*>(&p)) : __uint_as_float(p << 16);
+}
+template <typename T> __device__ __forceinline__ float high_of(uint32_t p) {
+    return std::is_same<T, __half>::value ? __high2float(*reinterpret_cast<const __half2*>(&p)) : __uint_as_float(p & 0xffff0000u);
+}
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -486,7 +486,7 @@ def _packed_workspace(like, *sizes):
 
 def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,
                      is_causal: bool = True, scale: float | None = None, out: torch.Tensor | None = None,
-                     lse: torch.Tensor | None = None) -> torch.Tensor:
+                     lse: torch.Tensor | None = None, out_low: torch.Tensor | None = None) -> torch.Tensor:
     """softmax(scale q k^T) v within each sequence of a packed batch, on q [tokens, heads, dim] and
     k, v [tokens, kv_heads, dim] (float32, float16 or bfloat16; dim 32, 64 or 128; head h reads key/value
     head h // (heads // kv_heads)).  Sequence i holds rows cu_seqlens[i] .. cu_seqlens[i + 1] - 1; cu_seqlens
@@ -495,14 +495,20 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
 
     Rows behind the last sequence keep what `out` holds; without `out` they are zeros.  What lies in another
     sequence, NaN included, reaches no row.  (Within a sequence a NaN or an infinity in v reaches every row of
-    the 128 whose keys it stands among, hidden or not.)  `lse`, a float32 [heads, tokens], receives the
-    logarithm of each row's sum, which attention_packed_backward needs."""
+    the 128 whose keys it stands among, hidden or not.)
+
+    For attention_packed_backward: `lse`, a float32 [heads, tokens], receives the logarithm of each row's sum.
+    `out_low`, like out and of use in 16 bits, receives what rounding took from the first 128 rows of each
+    sequence, where few keys share the weight: with it the gradients are rounded about as much as the output,
+    without it short sequences' are up to twice as far off."""
     elem, cu, t, h, kv, hd = _check_packed(q, k, v, cu_seqlens)
     if out is not None:
         _check_out("out", out, q.shape, q.dtype)
     if lse is not None:
         _check_out("lse", lse, (h, t), torch.float32)
-    d = _device(q, k, v, cu, out, lse)
+    if out_low is not None:
+        _check_out("out_low", out_low, q.shape, q.dtype)
+    d = _device(q, k, v, cu, out, lse, out_low)
     w = 2 if elem else 4
     q, qp, qs = _rows(q, w)
     k, kp, ks = _rows(k, w)
@@ -511,7 +517,8 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     n = cu.shape[0] - 1
     ws, ws_n = _packed_workspace(q, t, n, h, kv, hd, elem, 0)
     _launch("rac_attention_packed_async", _lib.PACKED_ARGS.pack(
-        qp, kp, vp, cu.data_ptr(), o.data_ptr(), 0 if lse is None else lse.data_ptr(), 0, 0, 0, 0,
+        qp, kp, vp, cu.data_ptr(), o.data_ptr(), 0 if lse is None else lse.data_ptr(),
+        0 if out_low is None else out_low.data_ptr(), 0, 0, 0, 0,
         ws.data_ptr() if ws_n else 0, *qs, *ks, *vs, 0, 0, t, ws_n, n, h, kv, hd, elem, bool(is_causal), out is None,
         hd ** -0.5 if scale is None else scale), d)
     return o
@@ -519,8 +526,9 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
 
 def attention_packed_backward(grad_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                               out: torch.Tensor, lse: torch.Tensor, cu_seqlens: torch.Tensor,
-                              is_causal: bool = True, scale: float | None = None):
-    """Gradients (dq, dk, dv) of attention_packed from its out and lse; the key/value heads' sum over the
+                              is_causal: bool = True, scale: float | None = None,
+                              out_low: torch.Tensor | None = None):
+    """Gradients (dq, dk, dv) of attention_packed from its out, lse and out_low; the key/value heads' sum over the
     query heads that read them.  Rows behind the last sequence get zeros.  The same inputs give the same bits."""
     elem, cu, t, h, kv, hd = _check_packed(q, k, v, cu_seqlens)
     if grad_out.shape != q.shape:
@@ -528,7 +536,9 @@ def attention_packed_backward(grad_out: torch.Tensor, q: torch.Tensor, k: torch.
     _elem(q, grad_out)
     _check_out("out", out, q.shape, q.dtype)
     _check_out("lse", lse, (h, t), torch.float32)
-    d = _device(q, k, v, cu, grad_out, out, lse)
+    if out_low is not None:
+        _check_out("out_low", out_low, q.shape, q.dtype)
+    d = _device(q, k, v, cu, grad_out, out, lse, out_low)
     w = 2 if elem else 4
     q, qp, qs = _rows(q, w)
     k, kp, ks = _rows(k, w)
@@ -538,7 +548,7 @@ def attention_packed_backward(grad_out: torch.Tensor, q: torch.Tensor, k: torch.
     n = cu.shape[0] - 1
     ws, ws_n = _packed_workspace(q, t, n, h, kv, hd, elem, 1)
     _launch("rac_attention_packed_backward_async", _lib.PACKED_ARGS.pack(
-        qp, kp, vp, cu.data_ptr(), out.data_ptr(), lse.data_ptr(), gp, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+        qp, kp, vp, cu.data_ptr(), out.data_ptr(), lse.data_ptr(), 0 if out_low is None else out_low.data_ptr(), gp, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
         ws.data_ptr() if ws_n else 0, *qs, *ks, *vs, *gs, t, ws_n, n, h, kv, hd, elem, bool(is_causal), 1,
         hd ** -0.5 if scale is None else scale), d)
     return dq, dk, dv

@@ -170,18 +170,21 @@ class RACAttentionPackedFunction(Function):
 
     @staticmethod
     def forward(ctx, q, k, v, cu_seqlens, is_causal, scale):
-        lse = torch.empty((q.shape[1], q.shape[0]), device=q.device, dtype=torch.float32) \
-            if any(ctx.needs_input_grad[:3]) else None
-        out = ext.attention_packed(q, k, v, cu_seqlens, is_causal, scale, lse=lse)
-        ctx.save_for_backward(q, k, v, out, lse, cu_seqlens)
+        lse = low = None
+        if any(ctx.needs_input_grad[:3]):
+            lse = torch.empty((q.shape[1], q.shape[0]), device=q.device, dtype=torch.float32)
+            if q.dtype != torch.float32:
+                low = torch.empty_like(q, memory_format=torch.contiguous_format)
+        out = ext.attention_packed(q, k, v, cu_seqlens, is_causal, scale, lse=lse, out_low=low)
+        ctx.save_for_backward(q, k, v, out, lse, low, cu_seqlens)
         ctx.is_causal, ctx.scale = is_causal, scale
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_out):
-        q, k, v, out, lse, cu_seqlens = ctx.saved_tensors
-        return (*ext.attention_packed_backward(grad_out, q, k, v, out, lse, cu_seqlens, ctx.is_causal, ctx.scale),
+        q, k, v, out, lse, low, cu_seqlens = ctx.saved_tensors
+        return (*ext.attention_packed_backward(grad_out, q, k, v, out, lse, cu_seqlens, ctx.is_causal, ctx.scale, low),
                 None, None, None)
 
 
