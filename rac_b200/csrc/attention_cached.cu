@@ -89,8 +89,8 @@ __global__ void __launch_bounds__(kThreadsF32, kBlocksPerSm) k_cached_f32(const 
                 const long long x = __shfl_sync(0xffffffffu, pg, key), y = __shfl_sync(0xffffffffu, sl, key);
                 k[i] = v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
                 if (x >= 0) {
-                    k[i] = __ldcs(reinterpret_cast<const float4*>(kp + x * p.k.page + y * p.k.row));
-                    v[i] = __ldcs(reinterpret_cast<const float4*>(vp + x * p.v.page + y * p.v.row));
+                    k[i] = __ldg(reinterpret_cast<const float4*>(kp + x * p.k.page + y * p.k.row));
+                    v[i] = __ldg(reinterpret_cast<const float4*>(vp + x * p.v.page + y * p.v.row));
                 }
             }
         };

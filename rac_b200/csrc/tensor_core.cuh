@@ -35,16 +35,22 @@ __device__ __forceinline__ bool bar_try(uint64_t* bar, uint32_t parity) {
     return ok != 0;
 }
 
-// Every wait ends: after kWaitLimit polls, or when another thread of the CTA
-// gave up, `gone` is set and the wait returns false.  The kernel then skips
-// the rest of its work, frees its tensor memory and returns.
-constexpr uint32_t kWaitLimit = 1u << 22;
+// Every wait ends: after kWaitNs, or when another thread of the block gave up,
+// `gone` is set and the wait returns false.  The kernel then skips the rest of
+// its work, frees its tensor memory and returns.
+constexpr uint64_t kWaitNs = 4000000000ull;
+__device__ __forceinline__ uint64_t now_ns() {
+    uint64_t t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    return t;
+}
 __device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, volatile int* gone) {
     if (bar_try(bar, parity)) return true;
+    const uint64_t t0 = now_ns();
 #pragma unroll 1
-    for (uint32_t i = 0; i < kWaitLimit; ++i) {
+    for (uint32_t i = 0; i < (1u << 30); ++i) {
         if (bar_try(bar, parity)) return true;
-        if ((i & 63) == 63 && *gone) return false;
+        if ((i & 63) == 63 && (*gone || now_ns() - t0 > kWaitNs)) break;
     }
     *gone = 1;
     return false;

@@ -221,6 +221,52 @@ def test_backward_from_autograd(cuda, dt):
 
 
 @gpu
+@pytest.mark.parametrize("dt", [F32, BF16])
+def test_gradient_of_a_sum(cuda, dt):
+    """out.sum() hands down one expanded value: strides of zero."""
+    q, k, v, go, cu = make([70, 20], 4, 2, 64, dt, cuda, seed=10)
+    leaves = [x.detach().requires_grad_(True) for x in (q, k, v)]
+    out = R.rac_attention_packed(*leaves, cu)
+    got = torch.autograd.grad(out.sum(), leaves, retain_graph=True)
+    want = torch.autograd.grad(out, leaves, torch.ones_like(out))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@gpu
+@pytest.mark.parametrize("dt", [F32, F16, BF16])
+def test_two_streams_at_once(cuda, dt):
+    """Calls that overlap on the GPU keep apart: each has its own workspace, barriers and tensor memory."""
+    sets = [make([900, 300, 77], 8, 2, 64, dt, cuda, seed=s) for s in (12, 13)]
+    want = [run_all(*s[:3], s[3], s[4], True, 0.125) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [None, None]
+    for _ in range(5):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i] = run_all(*sets[i][:3], sets[i][3], sets[i][4], True, 0.125)
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert all(torch.equal(a[n], b[n]) for n in a)
+
+
+@gpu
+def test_rows_past_32_bits(cuda):
+    """The last of 280000 rows of 64 heads of 128, elements past 2^31; the sequences before are short ones, so that
+    the work is small."""
+    t, h, n = 280000, 64, 40
+    q = torch.zeros(t, h, 128, dtype=BF16, device=cuda)
+    k, v = (torch.zeros(t, 1, 128, dtype=BF16, device=cuda) for _ in range(2))
+    g = torch.Generator(device=cuda).manual_seed(14)
+    for x in (q, k, v):
+        x[-n:] = torch.randn(x[-n:].shape, device=cuda, generator=g).to(BF16)
+    cu = torch.cat([torch.arange(0, t - n, n), torch.tensor([t - n, t])]).to(device=cuda, dtype=torch.int32)
+    out = ext.attention_packed(q, k, v, cu)
+    val, tol = plain.packed(q[-n:], k[-n:], v[-n:], [n], True, 128 ** -0.5)
+    plain.close(out[-n:], val["out"], tol["out"])
+
+
+@gpu
 def test_capture_and_another_stream(cuda):
     """Captured forward and backward replay on new inputs, two graphs that were captured one after the other
     do not disturb each other; a side stream gives the same bits."""
