@@ -31,18 +31,18 @@ __global__ void __launch_bounds__(kThreadsF32, kBlocksPerSm) k_cached_f32(const 
     constexpr int STEPS = 8 / G;           // steps of a warp's 32 keys
     __shared__ float4 so[4][kRowsF32][L];
     __shared__ float2 sml[4][kRowsF32];
-    __shared__ Walk walk;
+    __shared__ Walk ends[2];
     const CachedParams& p = a.p;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, dim = (lane % L) * 4, group = p.heads / p.kv_heads;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    if (warp == 0) {
-        const Walk w = piece(a, blockIdx.x, gridDim.x);
-        if (lane == 0) walk = w;
+    if (warp < 2) {
+        const Walk w = place(a, blockIdx.x + warp, gridDim.x);
+        if (lane == 0) ends[warp] = w;
     }
     __syncthreads();
-    Walk w = walk;
+    Walk w = between(ends);
     Segment s;
-    while (next(a, w, s)) {
+    for (bool first = true; next(a, w, s); first = false) {
         const int len = rows_in_cache(p, s.b), cnt = new_rows(p, s.b), prefix = max(0, len - cnt);
         const float* kp = static_cast<const float*>(p.k.p) + s.kvh * p.k.head + dim;
         const float* vp = static_cast<const float*>(p.v.p) + s.kvh * p.v.head + dim;
@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(kThreadsF32, kBlocksPerSm) k_cached_f32(const 
         if (lane < kRowsF32) sml[warp][lane] = make_float2(m, l);
         __syncthreads();
         const bool whole = s.j1 - s.j0 == s.tiles;
-        const long long piece_at = 2LL * blockIdx.x + (s.pos == walk.pos ? 0 : 1);
+        const long long piece_at = 2LL * blockIdx.x + (first ? 0 : 1);
         for (int e = threadIdx.x; e < kRowsF32 * L; e += kThreadsF32) {
             const int ur = e / L, c = e % L, row = s.unit * kRowsF32 + ur, nd = row / group;
             if (ur >= a.unit_rows || row >= a.rows) continue;

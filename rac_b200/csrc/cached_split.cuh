@@ -23,6 +23,7 @@ struct Args {
     float c;                               // scale * log2(e)
     int rows;                              // rows of a (sequence, kv head): new rows x heads of the group
     int unit_span, row_units, unit_rows;   // rows from unit to unit; units of a head; rows of a unit
+    int start;                             // what a unit's start costs, in tiles: its places on the line before them
     int copies;                            // of the rows in a tile (tensor-core kernel)
     float *part, *part_lse;                // [2 * blocks, unit_rows, dim], [2 * blocks, unit_rows]
     unsigned int* err;
@@ -41,33 +42,37 @@ __device__ __forceinline__ int tiles_of(const CachedParams& p, int b) {
     return max(1, (rows_in_cache(p, b) + kKeys - 1) / kKeys);
 }
 
-// The piece of the line of tiles that a block works on, as segments of one unit each.
+// The piece of the line of tiles that a block works on: where it has got to and
+// the tiles to go; and the piece's segments, of one unit each.
 struct Walk {
-    long long pos, end, at;                // at: position of sequence b's first tile
-    int b;
+    long long left;
+    int b, kvh, unit, j;
 };
 struct Segment {
     int b, kvh, unit, tiles, j0, j1;       // key tiles [j0, j1) of `tiles`
-    long long pos;
 };
+// By counting: every role of the kernels steps through the segments, and a 64-bit
+// division there is a call that costs the roles' loops their registers.
 __device__ __forceinline__ bool next(const Args& a, Walk& w, Segment& s) {
-    if (w.pos >= w.end) return false;
-    const long long per = (long long)a.p.kv_heads * a.row_units;
-    int n = tiles_of(a.p, w.b);
-    while (w.pos >= w.at + n * per) {
-        w.at += n * per;
-        ++w.b;
-        n = tiles_of(a.p, w.b);
-    }
-    const long long rel = w.pos - w.at, u = rel / n;
+    if (w.left <= 0) return false;
     s.b = w.b;
-    s.kvh = (int)(u / a.row_units);
-    s.unit = (int)(u % a.row_units);
-    s.tiles = n;
-    s.j0 = (int)(rel % n);
-    s.j1 = (int)min((long long)n, s.j0 + w.end - w.pos);
-    s.pos = w.pos;
-    w.pos += s.j1 - s.j0;
+    s.kvh = w.kvh;
+    s.unit = w.unit;
+    s.tiles = tiles_of(a.p, w.b);
+    s.j0 = w.j;
+    s.j1 = (int)min((long long)s.tiles, s.j0 + w.left);
+    w.left -= s.j1 - s.j0;
+    w.j = s.j1;
+    if (w.j == s.tiles) {
+        w.j = 0;
+        if (++w.unit == a.row_units) {
+            w.unit = 0;
+            if (++w.kvh == a.p.kv_heads) {
+                w.kvh = 0;
+                ++w.b;
+            }
+        }
+    }
     return true;
 }
 
@@ -80,35 +85,47 @@ __device__ __forceinline__ long long tiles_before(const CachedParams& p, int lim
     return n;
 }
 
-// Block `blk` of n works on positions [total blk / n, total (blk + 1) / n), n the
-// blocks launched or, where that is less, the tiles there are: no piece is empty.
-__device__ __forceinline__ Walk piece(const Args& a, int blk, int blocks) {
-    const long long per = (long long)a.p.kv_heads * a.row_units, total = tiles_before(a.p, a.p.batch) * per;
+// The beginning of piece i of n, at position total i / n of the line; `left` counts
+// the tiles before it.  n: the blocks launched or, where that is less, the positions
+// there are.  By one warp: two of them look for a block's two ends at the same time.
+__device__ __forceinline__ Walk place(const Args& a, int i, int blocks) {
+    const long long per = (long long)a.p.kv_heads * a.row_units;
+    const long long total = (tiles_before(a.p, a.p.batch) + (long long)a.p.batch * a.start) * per;
     const long long n_pieces = min((long long)blocks, total);
-    Walk w;
-    w.pos = blk < n_pieces ? total * blk / n_pieces : total;
-    w.end = blk < n_pieces ? total * (blk + 1) / n_pieces : total;
-    w.at = 0;
-    w.b = 0;
+    const long long pos = i < n_pieces ? total * i / n_pieces : total;
+    Walk w{};
     const int lane = threadIdx.x & 31;
-    for (int b0 = 0; b0 < a.p.batch && w.pos < w.end; b0 += 32) {
-        long long n = b0 + lane < a.p.batch ? tiles_of(a.p, b0 + lane) * per : 0;
+    long long at = 0;                      // of sequence w.b: its first position
+    w.b = a.p.batch;
+    for (int b0 = 0; b0 < a.p.batch; b0 += 32) {
+        const bool live = b0 + lane < a.p.batch;
+        long long n = live ? tiles_of(a.p, b0 + lane) : 0;
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
             const long long x = __shfl_up_sync(0xffffffffu, n, off);
             if (lane >= off) n += x;
         }
-        // n: end of sequence b0 + lane, counted from w.at
-        const unsigned past = __ballot_sync(0xffffffffu, w.at + n > w.pos);
-        if (past) {
-            const int l = __ffs(past) - 1;
-            const long long before = __shfl_sync(0xffffffffu, n, l ? l - 1 : 0);
-            w.at += l ? before : 0;
-            w.b = b0 + l;
-            break;
-        }
-        w.at += __shfl_sync(0xffffffffu, n, 31);
+        // Tiles and positions up to the end of sequence b0 + lane, counted from b0.
+        const long long m = n + (long long)a.start * min(lane + 1, a.p.batch - b0);
+        const unsigned past = __ballot_sync(0xffffffffu, at + m * per > pos);
+        const int l = past ? __ffs(past) - 1 : 32;
+        const long long x = __shfl_sync(0xffffffffu, n, l ? l - 1 : 0), y = __shfl_sync(0xffffffffu, m, l ? l - 1 : 0);
+        if (l) { w.left += x * per; at += y * per; }
+        if (past) { w.b = b0 + l; break; }
     }
+    if (w.b == a.p.batch) return w;
+    const int n = tiles_of(a.p, w.b);
+    const long long u = (pos - at) / (n + a.start);
+    w.kvh = (int)u / a.row_units;          // u < per
+    w.unit = (int)u % a.row_units;
+    w.j = (int)max(0LL, pos - at - u * (n + a.start) - a.start);
+    w.left += u * n + w.j;
+    return w;
+}
+// The walk of a block between two such places.
+__device__ __forceinline__ Walk between(const Walk (&ends)[2]) {
+    Walk w = ends[0];
+    w.left = ends[1].left - w.left;
     return w;
 }
 
@@ -121,13 +138,14 @@ __global__ void __launch_bounds__(256) k_cached_join(const __grid_constant__ Arg
     const long long bu = blockIdx.x / parts;
     const int b = (int)(bu / per), u = (int)(bu % per);
     const int kvh = u / a.row_units, unit = u % a.row_units, group = p.heads / p.kv_heads;
-    const long long total = tiles_before(p, p.batch) * per;
+    const long long total = (tiles_before(p, p.batch) + (long long)p.batch * a.start) * per;
     const int n = tiles_of(p, b);
     const long long blocks = min((long long)launched, total);
-    const long long t0 = tiles_before(p, b) * per + (long long)u * n;
-    const long long c0 = ((t0 + 1) * blocks - 1) / total, c1 = ((t0 + n) * blocks - 1) / total;
+    // The unit's places: from t0, its tiles from t1; the blocks of its first and last tile.
+    const long long t0 = (tiles_before(p, b) + (long long)b * a.start) * per + (long long)u * (n + a.start), t1 = t0 + a.start;
+    const long long c0 = ((t1 + 1) * blocks - 1) / total, c1 = ((t1 + n) * blocks - 1) / total;
     const int cnt = new_rows(p, b), lane = threadIdx.x & 31;
-    const long long s0 = 2 * c0 + (total * c0 / blocks == t0 ? 0 : 1);     // the first piece's place
+    const long long s0 = 2 * c0 + (total * c0 / blocks >= t0 ? 0 : 1);     // the first piece's place
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (c0 == c1) return;
     const int r = unit * a.unit_span + ur, node = r / group;
