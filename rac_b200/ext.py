@@ -496,6 +496,8 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     Rows behind the last sequence keep what `out` holds; without `out` they are zeros.  What lies in another
     sequence, NaN included, reaches no row.  (Within a sequence a NaN or an infinity in v reaches every row of
     the 128 whose keys it stands among, hidden or not.)
+    float32: values are taken to 22 bits or, where that is more, 2^-39 of the largest finite one among 128 rows of
+    a sequence's head, hidden ones included.
 
     For attention_packed_backward: `lse`, a float32 [heads, tokens], receives the logarithm of each row's sum.
     `out_low`, like out and of use in 16 bits, receives what rounding took from the first 128 rows of each

@@ -70,6 +70,19 @@ def test_values(cuda, lengths, nodes, h, kv, d, page, dt):
 
 
 @gpu
+@pytest.mark.parametrize("nodes,dt", [(48, BF16), (32, F16), (16, BF16), (3, F32)])
+def test_many_sequences_of_unlike_lengths(cuda, nodes, dt):
+    """Blocks whose piece of the work ends anywhere: in a unit's tiles, between units, among empty sequences."""
+    lengths = [(0, 1, 2500, 130, 640, 48, 127, 129)[(i * 5) % 8] + (i % 3) for i in range(70)]
+    q, kp, vp, table, lens = make(lengths, nodes, 8, 2, 64, 32, dt, cuda, seed=9, fill=math.nan)
+    counts = [min(nodes, n) for n in lengths]
+    got = ext.attention_cached(q, kp, vp, table, lens, torch.tensor(counts, dtype=torch.int32, device=cuda), None, 0.2)
+    want, tol = plain.cached(q, kp, vp, table.cpu(), lengths, counts, None, 0.2)
+    plain.close(got, want, tol)
+    ext.check_device_errors(cuda)
+
+
+@gpu
 @pytest.mark.parametrize("dt", [F32, BF16])
 def test_masks(cuda, dt):
     """Rows that see nothing (an empty mask on an empty prefix), a mask that skips the row itself, bits of rows
