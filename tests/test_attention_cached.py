@@ -83,6 +83,23 @@ def test_many_sequences_of_unlike_lengths(cuda, nodes, dt):
 
 
 @gpu
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("nodes,h,dt", [(16, 4, F16), (17, 4, BF16), (32, 8, F16), (64, 8, BF16), (43, 12, F16),
+                                        (64, 24, BF16), (33, 24, F32)])
+def test_row_counts(cuda, nodes, h, dt, d):
+    """Rows of a key/value head (two of them) that fill a half, one, two or more row tiles, or pass them by a few."""
+    lengths = [700, nodes, 129, 1]
+    q, kp, vp, table, lens = make(lengths, nodes, h, 2, d, 24, dt, cuda, seed=3, fill=math.nan)
+    counts = [nodes, nodes, nodes - 1, 1]
+    tree = tree_masks(len(lengths), nodes, 7)
+    got = ext.attention_cached(q, kp, vp, table, lens, torch.tensor(counts, dtype=torch.int32, device=cuda),
+                               tree.to(cuda), 0.1)
+    want, tol = plain.cached(q, kp, vp, table.cpu(), lengths, counts, tree, 0.1)
+    plain.close(got, want, tol)
+    ext.check_device_errors(cuda)
+
+
+@gpu
 @pytest.mark.parametrize("dt", [F32, BF16])
 def test_masks(cuda, dt):
     """Rows that see nothing (an empty mask on an empty prefix), a mask that skips the row itself, bits of rows
