@@ -18,7 +18,7 @@
 // Measured, bf16, dim 128, 32 heads on 8: one token for each of 64 sequences of 500
 // to 8100 rows 214 to 243 us, 5.3 to 4.7 TB/s of the cache's bytes, bound by them
 // and by each block's way to its first tile; 48 tree nodes for each of 8 sequences
-// of 777 to 16384 rows 119 to 122 us, bound by the exponentials of both row tiles
+// of 777 to 16384 rows 115 to 121 us, bound by the exponentials of both row tiles
 // and, 16 us, the join.
 #include "cached_split.cuh"
 
@@ -40,6 +40,7 @@ struct Regs {
     static constexpr int LAUNCH = 128, MATH = MANY ? 184 : 160, LOAD = MANY ? 80 : 104, OTHER = MANY ? 64 : 88;
     static_assert(MATH * 256 + LOAD * 128 + OTHER * 128 <= LAUNCH * kThreads, "register split");
 };
+constexpr int kTurnCycles = 4000;          // that the second row tile's softmax lets the first go ahead, at most
 constexpr int kInfo = 8;                   // tiles of key masks in flight
 
 template <int HD>
@@ -127,7 +128,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_cached_tc(const __grid_constant
              *s_ready = q_empty + 2, *p_ready = s_ready + 2, *o_ready = p_ready + 2, *pv_done = o_ready + 2,
              *load_sync = pv_done + 1, *math_sync = load_sync + 1;   // math_sync: two
     uint32_t* tmem_base = reinterpret_cast<uint32_t*>(math_sync + 2);
-    volatile int* gone = reinterpret_cast<volatile int*>(tmem_base + 1);
+    volatile int *gone = reinterpret_cast<volatile int*>(tmem_base + 1), *weighed = gone + 1;
     Walk(&ends)[2] = *reinterpret_cast<Walk(*)[2]>(sm + Sh::WALK);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const CachedParams& p = a.p;
@@ -135,6 +136,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_cached_tc(const __grid_constant
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (threadIdx.x == 0) {
         *gone = 0;
+        *weighed = 0;
         for (int i = 0; i < ST; ++i) { bar_init(full + i, 128); bar_init(empty + i, NW); }
         for (int i = 0; i < kInfo; ++i) bar_init(info + i, 4);
         for (int i = 0; i < 2; ++i) {
@@ -342,6 +344,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_cached_tc(const __grid_constant
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 fence_after();
+                if (NW == 2 && x == 1 && busy) {
+                    // After the first row tile's weights, so that one's products run under the
+                    // other's exponentials; in step both take 2900 cycles instead of 2000 (119.4
+                    // us for the trees, 115.5 in turn).  Only a matter of pace: nothing depends on it.
+                    for (const long long t0 = clock64(); *weighed <= t && clock64() - t0 < kTurnCycles;) {}
+                    __syncwarp();
+                }
                 if (busy) {
                     const uint32_t ts = tm + lanes + buf * kKeys;
                     const uint32_t* in = oks + (t % kInfo) * 4;
@@ -422,6 +431,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_cached_tc(const __grid_constant
                 }
                 fence_before();
                 bar_arrive(p_ready + buf);
+                if (NW == 2 && threadIdx.x == 0) *weighed = t + 1;
             }
             if (ok) ok = __all_sync(0xffffffffu, bar_wait(o_ready + x, (NW == 2 ? seg : seg >> 1) & 1, gone));
             if (!ok) break;
