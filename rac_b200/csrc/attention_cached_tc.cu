@@ -32,6 +32,8 @@ constexpr int kRowTile = 128, kUnitRows = 256;
 // 14, 15 fill the warpgroup.
 constexpr int kThreads = 512;
 // Up to 64 rows, which stand in the one tile several times; up to 128; up to 256 in two tiles.
+// One kernel for the first and the others took 235 us for 64 single tokens and 154 for
+// trees, where kernels apart took 220 and 136: the registers of one are not those of the other.
 enum Rows { kCopies, kOneTile, kTwoTiles };
 // Registers: a softmax thread holds its row's 128 scores, with copies a half or a quarter of them.
 template <Rows ROWS>

@@ -55,7 +55,8 @@ struct Shape {
 };
 
 // FINE: the first key tile's weights, which the first rows have no others beside,
-// in two parts, and what rounding takes from those rows' output.
+// in two parts, and what rounding takes from those rows' output.  A kernel of its
+// own: decided at run time it cost the calls without it 810 us for 650 (13 k tokens).
 template <typename T, int HD, bool FINE>
 __global__ void __launch_bounds__(kThreads, 1) k_packed_fwd_tc(const __grid_constant__ FwdArgs a) {
     using Sh = Shape<HD>;
