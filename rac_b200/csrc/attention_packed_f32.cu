@@ -44,8 +44,9 @@ struct SplitArgs {
     int heads[4], first[5];                // heads of each; prefix sums
     __half* parts[4];                      // [tokens, 2 heads, dim]: hi of each head, then lo
     float* factors[4];                     // [slots, heads]: 1 / f
+    float *vnorm, *gnorm;                  // with dout: like v's and dout's factors, the largest |v f| and |do f| of a row
     const float* out;                      // with dout: the forward's output, for D = do . o
-    float* delta;                          // [heads, tokens]
+    float *delta, *dtop;                   // [heads, tokens]; like dout's factors, the largest |D|
     const int* cu;
     int n_seqs;
     int negate;                            // q's parts are those of -q (a negative scale: the kernels take its size)
@@ -55,7 +56,7 @@ struct SplitArgs {
 template <int HD>
 __global__ void __launch_bounds__(256) k_split(const SplitArgs a) {
     constexpr int L = HD / 4, STEP = 256 / L, N = kSplit / STEP;
-    __shared__ float red[8];
+    __shared__ float red[8], red2[2][8];
     int h = blockIdx.x % a.first[4], w = 0;
     const int slot = blockIdx.x / a.first[4];
     while (h >= a.first[w + 1]) ++w;
@@ -74,6 +75,7 @@ __global__ void __launch_bounds__(256) k_split(const SplitArgs a) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) m = y[k] < INFINITY ? fmaxf(m, y[k]) : m;    // infinities and NaN keep to themselves
     }
+    float dtop = 0.f;
     if (w == 3) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
@@ -86,6 +88,7 @@ __global__ void __launch_bounds__(256) k_split(const SplitArgs a) {
 #pragma unroll
             for (int off = L / 2; off; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
             if (lane == 0 && r < t.len) a.delta[h * a.tokens + t.start + r] = s;
+            if (fabsf(s) < INFINITY) dtop = fmaxf(dtop, fabsf(s));
         }
     }
 #pragma unroll
@@ -117,6 +120,38 @@ __global__ void __launch_bounds__(256) k_split(const SplitArgs a) {
         *reinterpret_cast<uint2*>(row) = *reinterpret_cast<uint2*>(hi);
         *reinterpret_cast<uint2*>(row + (long long)a.heads[w] * HD) = *reinterpret_cast<uint2*>(lo);
     }
+    if (w < 2 || !a.delta) return;
+    // What bounds do . v and D, for the factors of dS.
+    float norm = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float y[4] = {x[i].x * f, x[i].y * f, x[i].z * f, x[i].w * f};
+        float s = 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) s = fabsf(y[k]) < INFINITY ? fmaf(y[k], y[k], s) : s;
+#pragma unroll
+        for (int off = L / 2; off; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+        norm = fmaxf(norm, s);
+    }
+#pragma unroll
+    for (int off = 16; off; off >>= 1) {
+        norm = fmaxf(norm, __shfl_xor_sync(0xffffffffu, norm, off));
+        dtop = fmaxf(dtop, __shfl_xor_sync(0xffffffffu, dtop, off));
+    }
+    if ((threadIdx.x & 31) == 0) {
+        red2[0][threadIdx.x >> 5] = norm;
+        red2[1][threadIdx.x >> 5] = dtop;
+    }
+    __syncthreads();
+    if (threadIdx.x) return;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        norm = fmaxf(norm, red2[0][i]);
+        dtop = fmaxf(dtop, red2[1][i]);
+    }
+    const long long at = (long long)slot * a.heads[w] + h;
+    (w == 2 ? a.vnorm : a.gnorm)[at] = sqrtf(norm);
+    if (w == 3) a.dtop[at] = dtop;
 }
 
 // ── tiles and products ────────────────────────────────────────────────────
@@ -128,6 +163,7 @@ struct Args {
     float c, scale;                        // |scale| log2(e), scale
     int split;                             // dk, dv: one query head a block, to be added up
     const float *fq, *fk, *fv, *fg;        // factors
+    const float *vnorm, *gnorm, *dtop;     // what bounds dS, see SplitArgs
     const __half *pq, *pk, *pv, *pg;       // parts
     const float *lse_in, *delta;
     float *out, *lse, *dq, *dk, *dv;
@@ -507,12 +543,22 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_fwd(const __grid_constant__
 }
 
 // ── backward ──────────────────────────────────────────────────────────────
-// Parts of a tile's largest value reach 2^14, so that with the factors f of dO
-// and V  |dS| <= 2 dim 2^28 f f'.  dS goes into parts times g = 2^15 / that, and
-// P times 2^12: dS' = P' (acc 2^-26 / dim - D g 2^-12), acc the sum of dO V^T's parts.
+// For a tile of queries and one of keys  |dS| = P |do . v - D| <= B = max |do| max |v| +
+// max |D|: rows of these two tiles bound do . v, and D, which holds the values of all the
+// keys that a query sees, is bounded by itself.  dS goes into parts times a power of two g
+// <= 2^15 / B (finite also where B is 0 or infinite) and P times 2^12:
+// dS' = P' (acc f f' g 2^-12 - D g 2^-12), acc the sum of the parts of dO V^T and f, f'
+// their factors.  B lies some 2^4 above a dO . V of independent values, so that dS of weights
+// around 1 / n keeps 22 bits up to some 2^14 keys; a smaller one keeps 2^-40 of B.
 constexpr float kPUp = 12.f, kPDown = 1.f / 4096.f;
-template <int HD> constexpr float acc_factor() { return 1.f / (67108864.f * HD); }
-template <int HD> __device__ __forceinline__ float ds_up(float fg, float fv) { return 1.f / (16384.f * HD) / fg / fv; }
+struct DsFactors { float up, acc, down; };  // g; f f' g 2^-12; 1 / g
+__device__ __forceinline__ DsFactors ds_factors(float fg, float gnorm, float dtop, float fv, float vnorm) {
+    // The products' factors are powers of two: no rounding, and no overflow unless dS itself overflows.
+    const float b = (gnorm * fg) * (vnorm * fv) + dtop;
+    const int e = min(max((int)(__float_as_uint(b) >> 23) - 126, -111), 128);       // B < 2^e
+    const float up = __uint_as_float((uint32_t)(142 - e) << 23);                     // 2^(15 - e)
+    return {up, fminf(fg * up * fv, 3e38f) * kPDown, __uint_as_float((uint32_t)(112 + e) << 23)};
+}
 
 template <int HD>
 struct BwdShape {
@@ -652,12 +698,14 @@ __device__ __forceinline__ void block_dkv(const Args& a, uint8_t* sm, unsigned b
             }
             __syncwarp();
         } else if (warp == 10) {
-            const float fv = a.fv[slot_of(t, t.row0) * a.kv_heads + kvh];
+            const long long ks = slot_of(t, t.row0) * a.kv_heads + kvh;
+            const float fv = a.fv[ks], vnorm = a.vnorm[ks];
             for (int i = 0; i < n; ++i) {
                 const int sl = i & 1, h = head_of(i);
                 const bool ok = i < 2 || bar_wait(stat_empty + sl, (i / 2 - 1) & 1, gone);
                 if (!__all_sync(0xffffffffu, ok)) break;
-                const float up = ds_up<HD>(a.fg[slot_of(t, row_of(i)) * a.heads + h], fv) * kPDown;
+                const long long qs = slot_of(t, row_of(i)) * a.heads + h;
+                const float up = ds_factors(a.fg[qs], a.gnorm[qs], a.dtop[qs], fv, vnorm).up * kPDown;
                 for (int r = lane; r < N; r += 32) {
                     const int row = row_of(i) + r;
                     float x = INFINITY, d = 0.f;
@@ -682,7 +730,7 @@ __device__ __forceinline__ void block_dkv(const Args& a, uint8_t* sm, unsigned b
         constexpr int W = HD == 32 ? 32 : HD / 2;
         const uint32_t v0 = tV + lanes + (HD == 32 ? 0 : W * half), k0 = tK + lanes + (HD == 32 ? 0 : W * half);
         const long long ks = slot_of(t, t.row0) * a.kv_heads + kvh;
-        const float fk = a.fk[ks], fv = a.fv[ks];
+        const float fk = a.fk[ks], fv = a.fv[ks], vnorm = a.vnorm[ks];
         float2 av[W / 2], ak[W / 2];
 #pragma unroll
         for (int i = 0; i < W / 2; ++i) av[i] = ak[i] = both(0.f);
@@ -704,6 +752,7 @@ __device__ __forceinline__ void block_dkv(const Args& a, uint8_t* sm, unsigned b
             const int sl = i & 1, q0 = row_of(i);
             const long long qs = slot_of(t, q0) * a.heads + head_of(i);
             const float fq = a.fq[qs], fg = a.fg[qs], c = a.c * fq * fk;
+            const DsFactors ds = ds_factors(fg, a.gnorm[qs], a.dtop[qs], fv, vnorm);
             ok = bar_wait(stat_full + sl, (i / 2) & 1, gone) && bar_wait(s_ready, i & 1, gone);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
@@ -738,7 +787,7 @@ __device__ __forceinline__ void block_dkv(const Args& a, uint8_t* sm, unsigned b
             bar_arrive(p_ready);
             if (i) add_k(i - 1);
             if (!ok) break;
-            take_k = fq / ds_up<HD>(fg, fv);
+            take_k = fminf(fq * ds.down, 3e38f);
             ok = __all_sync(0xffffffffu, bar_wait(dp_ready, i & 1, gone));
             if (!ok) break;
             fence_after();
@@ -750,7 +799,7 @@ __device__ __forceinline__ void block_dkv(const Args& a, uint8_t* sm, unsigned b
 #pragma unroll
                 for (int x = 0; x < 16; x += 2) {
                     const float4 z = *reinterpret_cast<const float4*>(dd + 2 * (b + x));       // -D
-                    const float2 f = both(acc_factor<HD>());
+                    const float2 f = both(ds.acc);
                     p[b + x] = __fmul2_rn(p[b + x], __ffma2_rn(pair(s[2 * x], s[2 * x + 1]), f, make_float2(z.x, z.y)));
                     p[b + x + 1] = __fmul2_rn(p[b + x + 1], __ffma2_rn(pair(s[2 * x + 2], s[2 * x + 3]), f, make_float2(z.z, z.w)));
                 }
@@ -912,7 +961,7 @@ __device__ __forceinline__ void block_dq(const Args& a, uint8_t* sm, unsigned bl
         constexpr int W = HD == 32 ? 32 : HD / 2;
         const uint32_t q0 = tQ + lanes + (HD == 32 ? 0 : W * half), p0 = tP + lanes + C * half;
         const long long qslot = slot_of(t, t.row0) * a.heads + head;
-        const float fq = a.fq[qslot], fg = a.fg[qslot];
+        const float fq = a.fq[qslot], fg = a.fg[qslot], gnorm = a.gnorm[qslot], dtop = a.dtop[qslot];
         float lse = INFINITY, d = 0.f;
         float2 acc[W / 2];
 #pragma unroll
@@ -955,8 +1004,9 @@ __device__ __forceinline__ void block_dq(const Args& a, uint8_t* sm, unsigned bl
             }
             if (j) add_q(j - 1);
             if (!ok) break;
-            const float up = ds_up<HD>(fg, fv), du = d * up * kPDown;
-            take_f = fk / up;
+            const DsFactors ds = ds_factors(fg, gnorm, dtop, fv, a.vnorm[ks]);
+            const float du = d * (ds.up * kPDown);
+            take_f = fminf(fk * ds.down, 3e38f);
             ok = __all_sync(0xffffffffu, bar_wait(dp_ready, j & 1, gone));
             if (!ok) break;
             fence_after();
@@ -968,7 +1018,7 @@ __device__ __forceinline__ void block_dq(const Args& a, uint8_t* sm, unsigned bl
                 wait_ld();
 #pragma unroll
                 for (int x = 0; x < 16; ++x)
-                    p[b + x] = __fmul2_rn(p[b + x], __ffma2_rn(pair(s[2 * x], s[2 * x + 1]), both(acc_factor<HD>()), both(-du)));
+                    p[b + x] = __fmul2_rn(p[b + x], __ffma2_rn(pair(s[2 * x], s[2 * x + 1]), both(ds.acc), both(-du)));
                 if (part) {
 #pragma unroll
                     for (int x = 0; x < 16; ++x) {
@@ -1032,11 +1082,11 @@ bool by_head(long long tokens, int heads, int kv_heads) {
     return heads > kv_heads && tokens / kWide * kv_heads < 2 * 148;
 }
 
-// Workspace: parts of q, k, v (and dO), their factors, D, and dk and dv by query head.
+// Workspace: parts of q, k, v (and dO), their factors, what bounds dS, D, and dk and dv by query head.
 struct Room {
     __half* parts[4];
     float* factors[4];
-    float *delta, *dk, *dv;
+    float *vnorm, *gnorm, *dtop, *delta, *dk, *dv;
     size_t bytes;
 };
 Room room(void* ws, long long tokens, int n_seqs, int heads, int kv_heads, int hd, int backward) {
@@ -1053,8 +1103,16 @@ Room room(void* ws, long long tokens, int n_seqs, int heads, int kv_heads, int h
         r.factors[i] = reinterpret_cast<float*>(p + at);
         at += up256((size_t)slots * h[i] * sizeof(float));
     }
-    r.delta = reinterpret_cast<float*>(p + at);
-    if (backward) at += up256((size_t)tokens * heads * sizeof(float));
+    if (backward) {
+        r.vnorm = reinterpret_cast<float*>(p + at);
+        at += up256((size_t)slots * kv_heads * sizeof(float));
+        r.gnorm = reinterpret_cast<float*>(p + at);
+        at += up256((size_t)slots * heads * sizeof(float));
+        r.dtop = reinterpret_cast<float*>(p + at);
+        at += up256((size_t)slots * heads * sizeof(float));
+        r.delta = reinterpret_cast<float*>(p + at);
+        at += up256((size_t)tokens * heads * sizeof(float));
+    }
     if (backward && by_head(tokens, heads, kv_heads)) {
         r.dk = reinterpret_cast<float*>(p + at);
         at += up256((size_t)tokens * heads * hd * sizeof(float));
@@ -1083,6 +1141,7 @@ int launch(const PackedParams& p, const Room& r, Args& a, bool backward, cudaStr
         sp.parts[i] = r.parts[i]; sp.factors[i] = r.factors[i];
     }
     sp.out = static_cast<const float*>(p.out_in); sp.delta = r.delta;
+    sp.vnorm = r.vnorm; sp.gnorm = r.gnorm; sp.dtop = r.dtop;
     sp.negate = p.scale < 0.f; sp.cu = p.cu; sp.n_seqs = p.n_seqs; sp.tokens = p.tokens;
     const unsigned slots = (unsigned)packed_slots(p.tokens, p.n_seqs, kSplit);
     k_split<HD><<<slots * sp.first[4], 256, 0, s>>>(sp);
@@ -1130,6 +1189,7 @@ int attention_packed_f32(const PackedParams& p, int backward, cudaStream_t s) {
     a.scale = p.scale;
     a.pq = r.parts[0]; a.pk = r.parts[1]; a.pv = r.parts[2]; a.pg = r.parts[3];
     a.fq = r.factors[0]; a.fk = r.factors[1]; a.fv = r.factors[2]; a.fg = r.factors[3];
+    a.vnorm = r.vnorm; a.gnorm = r.gnorm; a.dtop = r.dtop;
     a.lse_in = p.lse_in; a.delta = r.delta;
     a.out = static_cast<float*>(p.out); a.lse = p.lse;
     a.dq = static_cast<float*>(p.dq); a.dk = static_cast<float*>(p.dk); a.dv = static_cast<float*>(p.dv);
