@@ -300,6 +300,11 @@ static_assert(kMathRegs * 256 + kOtherRegs * 128 <= kLaunchRegs * kThreads, "reg
 // Slot (of 128 rows) of a row of a sequence.
 __device__ __forceinline__ long long slot_of(const PackedTile& t, int row) { return t.start / kSplit + t.seq + row / kSplit; }
 
+// |scale| log2(e) times both tiles' factors: what a score of their parts is multiplied by.
+// Neither 0, which would turn a hidden score's infinity into NaN, nor infinite, which would
+// do so to a score of 0: a score of parts is below 2^36, and 1e-37 leaves it without weight.
+__device__ __forceinline__ float score_factor(float cq, float fk) { return fminf(fmaxf(cq * fk, 1e-37f), 3e38f); }
+
 constexpr int kKeysF32 = 128;              // keys of a tile, forward
 
 // ── forward ───────────────────────────────────────────────────────────────
@@ -437,7 +442,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_fwd(const __grid_constant__
         bool ok = true;
         for (int j = w; j < n; j += 2) {
             const long long ks = slot_of(t, j * kKeysF32) * a.kv_heads + kvh;
-            const float c = cq * a.fk[ks], fv = a.fv[ks];
+            const float c = score_factor(cq, a.fk[ks]), fv = a.fv[ks];
             ok = __all_sync(0xffffffffu, bar_wait(s_ready + w, (j >> 1) & 1, gone));
             if (!ok) break;
             fence_after();
@@ -751,7 +756,7 @@ __device__ __forceinline__ void block_dkv(const Args& a, uint8_t* sm, unsigned b
         for (int i = 0; i < n; ++i) {
             const int sl = i & 1, q0 = row_of(i);
             const long long qs = slot_of(t, q0) * a.heads + head_of(i);
-            const float fq = a.fq[qs], fg = a.fg[qs], c = a.c * fq * fk;
+            const float fq = a.fq[qs], fg = a.fg[qs], c = score_factor(a.c * fq, fk);
             const DsFactors ds = ds_factors(fg, a.gnorm[qs], a.dtop[qs], fv, vnorm);
             ok = bar_wait(stat_full + sl, (i / 2) & 1, gone) && bar_wait(s_ready, i & 1, gone);
             ok = __all_sync(0xffffffffu, ok);
@@ -987,7 +992,7 @@ __device__ __forceinline__ void block_dq(const Args& a, uint8_t* sm, unsigned bl
         for (int j = 0; j < n; ++j) {
             const uint32_t s0 = tS + lanes + N * (j & 1) + C * half;
             const long long ks = slot_of(t, j * N) * a.kv_heads + kvh;
-            const float fk = a.fk[ks], fv = a.fv[ks], c = a.c * fq * fk;
+            const float fk = a.fk[ks], fv = a.fv[ks], c = score_factor(a.c * fq, fk);
             ok = __all_sync(0xffffffffu, bar_wait(s_ready + (j & 1), (j >> 1) & 1, gone));
             if (!ok) break;
             fence_after();
@@ -1184,8 +1189,7 @@ int attention_packed_f32(const PackedParams& p, int backward, cudaStream_t s) {
     if (cudaGetDevice(&dev) != cudaSuccess) { cudaGetLastError(); return kErrCuda; }
     a.cu = p.cu; a.n_seqs = p.n_seqs; a.heads = p.heads; a.kv_heads = p.kv_heads; a.group = p.heads / p.kv_heads;
     a.causal = p.causal; a.zero_rest = p.zero_rest; a.tokens = p.tokens;
-    // 0 would turn a hidden score's infinity into NaN; 1e-30 weighs the rest alike.
-    a.c = p.scale == 0.f ? 1e-30f : fabsf(p.scale) * kLog2e;
+    a.c = fabsf(p.scale) * kLog2e;
     a.scale = p.scale;
     a.pq = r.parts[0]; a.pk = r.parts[1]; a.pv = r.parts[2]; a.pg = r.parts[3];
     a.fq = r.factors[0]; a.fk = r.factors[1]; a.fv = r.factors[2]; a.fg = r.factors[3];

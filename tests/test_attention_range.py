@@ -68,3 +68,19 @@ def test_gradients_of_long_sequences_keep_their_digits(cuda, d):
     for name, want in (("dq", dq), ("dk", dk)):
         off = ((got[name][:, 0].double() - want).norm() / want.norm()).item()
         assert off <= bound, (name, off, bound)
+
+
+@gpu
+@pytest.mark.parametrize("size,scale", [(1e-5, 0.0), (1e-20, 0.125), (1e-30, 0.125), (1e-30, -0.125), (1.0, 0.0),
+                                        (1e6, 0.0)])
+@pytest.mark.parametrize("causal,lens", [(True, [190, 70]), (False, [190, 70])])
+def test_scores_of_no_size(cuda, size, scale, causal, lens):
+    """float32 queries and keys whose scores vanish: each row is the mean of the values that it sees."""
+    q, k, v, go, cu = make(lens, 4, 2, 64, F32, cuda, seed=24)
+    q, k = q * size, k * size
+    got = run_all(q, k, v, go, cu, causal, scale)
+    val, tol = plain.packed(-q if scale < 0 else q, k, v, lens, causal, abs(scale), go)
+    if scale < 0:
+        val["dq"] = -val["dq"]
+    for name in ("out", "dq", "dk", "dv"):
+        plain.close(got[name], val[name], tol[name], name)
