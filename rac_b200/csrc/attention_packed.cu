@@ -34,11 +34,11 @@ int check(const PackedParams& p) {
 
 }  // namespace
 
-// 16-bit types, backward: D, [heads, tokens], and two largest values.
+// 16-bit types, backward: D, [heads, tokens], and two largest values of each sequence and key/value head.
 size_t attention_packed_workspace(long long tokens, int n_seqs, int heads, int kv_heads, int head_dim, int type,
                                   int backward) {
     if (type == kF32) return attention_packed_f32_workspace(tokens, n_seqs, heads, kv_heads, head_dim, backward);
-    return backward ? sizeof(float) * ((size_t)tokens * heads + 2) : 0;
+    return backward ? sizeof(float) * ((size_t)tokens * heads + 2 * (size_t)n_seqs * kv_heads) : 0;
 }
 
 static bool room_ok(const PackedParams& p, int backward) {

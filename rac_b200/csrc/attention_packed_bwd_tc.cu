@@ -16,8 +16,9 @@
 //
 // float16: weights below 2^-14 and dS of small gradients would fall among the
 // subnormal numbers and lose their digits.  P carries a factor 2^10, and dS a
-// power of two taken from the largest |do| and |v| that keeps it below the
-// type's largest value: |dS| <= 2 head_dim max|do| max|v|.
+// power of two that keeps it below the type's largest value, taken from the largest
+// |do| and |v| of the sequence and key/value head: |dS| <= 2 head_dim max|do| max|v|.
+// (Of all sequences together, one of large gradients took the digits of the others.)
 //
 // Bound: the seven products (the tensor pipe is busy half of the time) and the
 // way of P and dS through registers between them.  8192 causal tokens in three
@@ -45,15 +46,16 @@ struct BwdArgs {
     long long tokens;
     float c, scale;                        // scale * log2(e), scale
     const float *lse, *delta;              // [heads, tokens]
-    const float* top;                      // float16: max |do|, max |v|
+    const float* top;                      // float16: max |do|, max |v| of each sequence and key/value head
     void *dq, *dk, *dv;
     unsigned int* err;
 };
 
-// Power of two on dS and exponent on P.
+// Power of two on dS of a sequence's key/value head, and exponent on P.
 template <typename T>
-__device__ __forceinline__ float ds_factor(const float* top, int hd) {
+__device__ __forceinline__ float ds_factor(const BwdArgs& a, int seq, int kvh, int hd) {
     if (!std::is_same<T, __half>::value) return 1.f;
+    const float* top = a.top + 2 * ((long long)seq * a.kv_heads + kvh);
     const float b = 2.f * hd * top[0] * top[1];
     if (!(b > 0.f) || b > 1e30f) return 1.f;
     int e;
@@ -279,7 +281,7 @@ __device__ __forceinline__ void block_dkv(const BwdArgs& a, uint8_t* sm, unsigne
             __syncwarp();
         } else if (warp == 10) {
             // Row statistics of each query tile; a row behind the sequence has weight exp2(-inf).
-            const float gf = ds_factor<T>(a.top, HD) * (1.f / (1 << p_shift<T>()));
+            const float gf = ds_factor<T>(a, t.seq, kvh, HD) * (1.f / (1 << p_shift<T>()));
             for (int i = 0; i < n; ++i) {
                 const int sl = i & 1;
                 const bool ok = i < 2 || bar_wait(stat_empty + sl, (i / 2 - 1) & 1, gone);
@@ -305,7 +307,7 @@ __device__ __forceinline__ void block_dkv(const BwdArgs& a, uint8_t* sm, unsigne
         const int half = warp >> 2, row = t.row0 + (warp & 3) * 32 + lane;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t s0 = tS + lanes + 64 * half, p0 = tP + lanes + 64 * half;
-        const float gf = ds_factor<T>(a.top, HD) * (1.f / (1 << p_shift<T>()));
+        const float gf = ds_factor<T>(a, t.seq, kvh, HD) * (1.f / (1 << p_shift<T>()));
         bool ok = true;
         for (int i = 0; i < n; ++i) {
             const int sl = i & 1;
@@ -378,7 +380,7 @@ __device__ __forceinline__ void block_dkv(const BwdArgs& a, uint8_t* sm, unsigne
             fence_after();
             const bool live = row < t.len;
             if (half == 0) store_row<T, HD>(tV + lanes, 1.f / (1 << p_shift<T>()), dv + row * out_row, live);
-            else store_row<T, HD>(tK + lanes, a.scale / ds_factor<T>(a.top, HD), dk + row * out_row, live);
+            else store_row<T, HD>(tK + lanes, a.scale / ds_factor<T>(a, t.seq, kvh, HD), dk + row * out_row, live);
         }
     }
     fence_before();
@@ -504,7 +506,7 @@ __device__ __forceinline__ void block_dq(const BwdArgs& a, uint8_t* sm, unsigned
         const int half = warp >> 2, row = t.row0 + (warp & 3) * 32 + lane;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t p0 = tP + lanes + 64 * half;
-        const float gf = ds_factor<T>(a.top, HD);
+        const float gf = ds_factor<T>(a, t.seq, kvh, HD);
         float lse = INFINITY, d = 0.f;
         if (row < t.len) {
             const long long at = (long long)head * a.tokens + t.start + row;
@@ -580,7 +582,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_packed_bwd_tc(const __grid_cons
 
 // D = do . o of the rows of a tile of one head, HD / 8 lanes a row; in a
 // sequence's first tile o is the sum of what was stored and what rounding took
-// from it.  float16: the largest |do| and |v| (blocks of y = 1 read v).  Every
+// from it.  float16: the largest |do| and |v| of its key/value head (blocks of y = 1 read v).  Every
 // row of a thread is read before the first is summed.
 template <typename T, int HD>
 __global__ void __launch_bounds__(256) k_packed_delta16(const PackedParams p, float* __restrict__ delta,
@@ -627,9 +629,11 @@ __global__ void __launch_bounds__(256) k_packed_delta16(const PackedParams p, fl
         if (r < t.len && !is_v && lane == 0) delta[head * p.tokens + t.start + r] = s;
     }
     if (std::is_same<T, __half>::value) {
+        const int kvh = is_v ? head : head / (p.heads / p.kv_heads);
+        int* at = reinterpret_cast<int*>(top + 2 * ((long long)t.seq * p.kv_heads + kvh) + is_v);
 #pragma unroll
         for (int off = 16; off; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
-        if ((threadIdx.x & 31) == 0 && m > 0.f) atomicMax(reinterpret_cast<int*>(top + is_v), __float_as_int(m));
+        if ((threadIdx.x & 31) == 0 && m > 0.f) atomicMax(at, __float_as_int(m));      // a maximum: any order gives it
     }
 }
 
@@ -638,7 +642,7 @@ int launch_bwd(const BwdArgs& a, const PackedParams& p, cudaStream_t s) {
     using Sh = Shape<HD>;
     const bool f16 = std::is_same<T, __half>::value;
     float* top = const_cast<float*>(a.top);
-    if (f16 && cudaMemsetAsync(top, 0, 2 * sizeof(float), s) != cudaSuccess) return kErrCuda;
+    if (f16 && cudaMemsetAsync(top, 0, sizeof(float) * 2 * p.n_seqs * p.kv_heads, s) != cudaSuccess) return kErrCuda;
     const unsigned slots = (unsigned)packed_slots(a.tokens, a.n_seqs, kTile);
     k_packed_delta16<T, HD><<<dim3(slots * a.heads, f16 ? 2 : 1), 256, 0, s>>>(p, const_cast<float*>(a.delta), top);
     if (cudaGetLastError() != cudaSuccess) return kErrCuda;
@@ -658,7 +662,7 @@ int bwd_by_dim(const BwdArgs& a, const PackedParams& p, cudaStream_t s) {
 
 }  // namespace
 
-// Workspace: D [heads, tokens], then the two largest values.
+// Workspace: D [heads, tokens], then the largest values [n_seqs, kv_heads, 2].
 int attention_packed_backward_tc(const PackedParams& p, cudaStream_t s) {
     BwdArgs a{};
     if (!rows_map(&a.q, p.q, p.type, p.tokens, p.heads, p.head_dim) ||

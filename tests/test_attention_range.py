@@ -1,12 +1,15 @@
 """Packed attention over the whole range of its types: rows of very different sizes in different tiles and sequences,
 values near the ends of the range, gradients of long sequences."""
+import math
+
 import pytest
 import torch
 
 import attention_plain as plain
+from rac_b200 import ext
 from test_attention_packed import check, make, run_all
 
-F32 = torch.float32
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
 gpu = pytest.mark.gpu
 
 
@@ -84,3 +87,22 @@ def test_scores_of_no_size(cuda, size, scale, causal, lens):
         val["dq"] = -val["dq"]
     for name in ("out", "dq", "dk", "dv"):
         plain.close(got[name], val[name], tol[name], name)
+
+
+@gpu
+@pytest.mark.parametrize("dt", [F32, F16, BF16])
+@pytest.mark.parametrize("other", [2.0 ** 12, math.inf, math.nan])
+def test_a_sequence_does_not_feel_the_size_of_another(cuda, dt, other):
+    """Gradients of a sequence are the same bits whatever the others hold."""
+    lens = [70, 100, 31]
+    q, k, v, go, cu = make(lens, 4, 2, 64, dt, cuda, seed=25)
+    go = go * 2.0 ** -6
+    clean = run_all(q, k, v, go, cu, True, 0.125)
+    v, go = v.clone(), go.clone()
+    for x in (v, go):
+        x[70:170] *= other
+    got = run_all(q, k, v, go, cu, True, 0.125)
+    for name in ("out", "dq", "dk", "dv"):
+        for sl in (slice(0, 70), slice(170, 201)):
+            assert torch.equal(got[name][sl], clean[name][sl]), name
+    ext.check_device_errors(cuda)
