@@ -158,12 +158,19 @@ int rac_rope_cache_async(float *cos_out, float *sin_out, int max_seq, int head_d
 int rac_rope_apply_async(float *x, const float *cos_tab, const float *sin_tab,
                          const int *pos, long long batch_heads, int seq, int head_dim,
                          int form, void *stream);
+/* Row positions[i] of the tables [table_rows, half] (dtype as in section 4) for
+ * i < n, as floats: tables for rac_rope_apply_async over rows of any positions
+ * (int32 or int64: pos_bytes 4 or 8).  A position outside the tables gives a row of
+ * NaN, and rac_check_device_errors() reports RAC_ERR_DEVICE. */
+int rac_rope_rows_async(const void *cos_tab, const void *sin_tab, int dtype, const void *positions, int pos_bytes,
+                        long long n, long long table_rows, int half, float *cos_out, float *sin_out, void *stream);
 /* Fused attention on `stream` (device pointers): rac_attention without the
  * [seq, seq] score tensor (lib/c/rac_cpu.c:637-703 semantics). */
 int rac_attention_async(const float *q, const float *k, const float *v, const float *mask,
                         int is_causal, float *out, int batch, int n_heads, int seq,
                         int head_dim, void *stream);
-/* Reads and clears the device's error word (bounded-loop overruns) after
+/* Reads and clears the device's error word (bounded-loop overruns, pages and
+ * positions that do not exist) after
  * synchronising `stream`; returns RAC_OK or RAC_ERR_DEVICE. */
 int rac_check_device_errors(void *stream);
 

@@ -285,6 +285,12 @@ RAC_API int rac_rope_apply_async(float* x, const float* cos_tab, const float* si
     return set_status(rope_apply(x, cos_tab, sin_tab, pos, batch_heads, seq, head_dim, form,
                                  as_stream(stream)), "rac_rope_apply_async");
 }
+RAC_API int rac_rope_rows_async(const void* cos_tab, const void* sin_tab, int dtype, const void* pos, int pos_bytes,
+                                long long n, long long table_rows, int half, float* cos_out, float* sin_out,
+                                void* stream) {
+    return set_status(rope_rows(cos_tab, sin_tab, dtype, pos, pos_bytes, n, table_rows, half, cos_out, sin_out,
+                                as_stream(stream)), "rac_rope_rows_async");
+}
 RAC_API int rac_check_device_errors(void* stream) {
     int dev = 0;
     int st = device_ready(&dev);

@@ -5,8 +5,12 @@
 // and a grid-stride loop over a grid sized to the SM count.  The arithmetic
 // follows lib/c/rac_cpu.c rounding step by rounding step (see
 // rac_device.cuh), so results are bit-identical to the reference library.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
 #include <atomic>
 
+#include "attn_ops.h"
 #include "rac_device.cuh"
 #include "rac_internal.h"
 #include "stream_ops.h"
@@ -350,6 +354,52 @@ int rope_apply(float* x, const float* cos_tab, const float* sin_tab, const int* 
     k_rope_apply<<<grid_for(work, 256), 256, 0, s>>>(x, cos_tab, sin_tab, pos, rows, seq,
                                                      head_dim, form, vec ? 1 : 0);
     return cudaGetLastError() == cudaSuccess ? kOk : kErrCuda;
+}
+
+constexpr unsigned int kErrBadPosition = 32u;   // bit 5 of the device error word
+
+// Rows of the tables at given positions, as floats.  A position that the tables
+// do not hold gives NaN and sets the error word.
+template <typename T, typename P>
+__global__ void __launch_bounds__(256) k_rope_rows(const T* __restrict__ cos_tab, const T* __restrict__ sin_tab,
+                                                   const P* __restrict__ pos, long long n, long long table_rows,
+                                                   int half, float* __restrict__ cos_out,
+                                                   float* __restrict__ sin_out) {
+    const long long total = n * half, stride = (long long)gridDim.x * blockDim.x;
+    for (long long e = (long long)blockIdx.x * blockDim.x + threadIdx.x; e < total; e += stride) {
+        const long long p = (long long)pos[e / half];
+        if (p < 0 || p >= table_rows) {
+            cos_out[e] = sin_out[e] = __int_as_float(0x7fffffff);
+            atomicOr(&g_err_word, kErrBadPosition);
+            continue;
+        }
+        const long long at = p * half + e % half;
+        cos_out[e] = static_cast<float>(cos_tab[at]);
+        sin_out[e] = static_cast<float>(sin_tab[at]);
+    }
+}
+
+template <typename T>
+static int rope_rows_of(const void* ct, const void* st, const void* pos, int pos_bytes, long long n,
+                        long long table_rows, int half, float* c, float* sn, cudaStream_t s) {
+    const T *a = static_cast<const T*>(ct), *b = static_cast<const T*>(st);
+    const int grid = grid_for(n * half, 256);
+    if (pos_bytes == 8)
+        k_rope_rows<<<grid, 256, 0, s>>>(a, b, static_cast<const long long*>(pos), n, table_rows, half, c, sn);
+    else
+        k_rope_rows<<<grid, 256, 0, s>>>(a, b, static_cast<const int*>(pos), n, table_rows, half, c, sn);
+    return cudaGetLastError() == cudaSuccess ? kOk : kErrCuda;
+}
+
+int rope_rows(const void* cos_tab, const void* sin_tab, int type, const void* pos, int pos_bytes, long long n,
+              long long table_rows, int half, float* cos_out, float* sin_out, cudaStream_t s) {
+    if (n < 0 || table_rows < 0 || half <= 0 || (pos_bytes != 4 && pos_bytes != 8)) return kErrInvalidDim;
+    if (type < kF32 || type > kBF16) return kErrUnsupported;
+    if (n == 0) return kOk;
+    if (!pos || !cos_out || !sin_out || (table_rows && (!cos_tab || !sin_tab))) return kErrNullPtr;
+    if (type == kF32) return rope_rows_of<float>(cos_tab, sin_tab, pos, pos_bytes, n, table_rows, half, cos_out, sin_out, s);
+    if (type == kF16) return rope_rows_of<__half>(cos_tab, sin_tab, pos, pos_bytes, n, table_rows, half, cos_out, sin_out, s);
+    return rope_rows_of<__nv_bfloat16>(cos_tab, sin_tab, pos, pos_bytes, n, table_rows, half, cos_out, sin_out, s);
 }
 
 }  // namespace racb

@@ -18,6 +18,9 @@ int rope_cache(float* cos_out, float* sin_out, int max_seq, int head_dim, float 
                cudaStream_t s);
 int rope_apply(float* x, const float* cos_tab, const float* sin_tab, const int* pos,
                long long batch_heads, int seq, int head_dim, int form, cudaStream_t s);
+// type: ElemType of the tables [table_rows, half]; pos: n integers of pos_bytes (4 or 8).
+int rope_rows(const void* cos_tab, const void* sin_tab, int type, const void* pos, int pos_bytes, long long n,
+              long long table_rows, int half, float* cos_out, float* sin_out, cudaStream_t s);
 
 // Row-wise (rows x d, row-major, leading dimension d).
 int softmax_rows(const float* x, float* y, long long rows, int d, cudaStream_t s);

@@ -657,6 +657,26 @@ def cache_append_(k_pages: torch.Tensor, v_pages: torch.Tensor, k: torch.Tensor,
         0, *kst, 0, *vst, *ks, *vs, s[0], table.shape[1], pages, page, b, 0, 1, kv, hd, elem), d)
 
 
+def rope_rows(cos_tab: torch.Tensor, sin_tab: torch.Tensor, positions: torch.Tensor):
+    """Rows `positions` ([n], int32 or int64) of RoPE tables [rows, dim / 2], as float32: (cos, sin) [n, dim / 2] for
+    rope_apply_.  A position outside the tables gives a row of NaN, and check_device_errors() raises."""
+    if cos_tab.dim() != 2 or sin_tab.shape != cos_tab.shape:
+        raise ValueError(f"rope_rows: tables must be [rows, dim / 2] and alike, got {tuple(cos_tab.shape)} and "
+                         f"{tuple(sin_tab.shape)}")
+    if positions.dim() != 1 or positions.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"rope_rows: positions must be 1-D and int32 or int64, got {tuple(positions.shape)} of "
+                         f"{positions.dtype}")
+    elem = _elem(cos_tab, sin_tab)
+    d = _device(cos_tab, sin_tab, positions)
+    c, s, pos = cos_tab.contiguous(), sin_tab.contiguous(), positions.contiguous()
+    out = c.new_empty((2, pos.shape[0], c.shape[1]), dtype=torch.float32)
+    args = (c.data_ptr(), s.data_ptr(), elem, pos.data_ptr(), pos.element_size(), pos.shape[0], c.shape[0], c.shape[1],
+            out[0].data_ptr(), out[1].data_ptr())
+    with torch.cuda.device(d):
+        _lib.call("rac_rope_rows_async", *args, _raw_stream(d))
+    return out[0], out[1]
+
+
 def _layered(st: tuple) -> tuple:
     return st if len(st) == 4 else (0, *st)
 

@@ -483,7 +483,9 @@ class RACRoPEAttention(nn.Module):
     * forward(x, cu_seqlens=...): x holds sequences of different lengths laid
       end to end ([tokens, d] or [1, tokens, d]).  RoPE positions count from each
       sequence's start.  Their tables hold max_seq_len rows: where x has more
-      rows than that, pass max_seqlen (the longest sequence) or positions;
+      rows than that, pass max_seqlen (the longest sequence) or positions.  A
+      position past the tables is refused where the host knows it; where only the
+      device does, the row turns into NaN and ext.check_device_errors() raises;
     * forward(x, cache=step, layer=i): x holds the new tokens of the sequences of
       a RACCacheStep (cache.py) in its order; they join the cache and attend
       over it.  No gradients."""
@@ -540,9 +542,7 @@ class RACRoPEAttention(nn.Module):
 
     def _rotate_rows(self, q, k, positions):
         """RoPE of q [T, H, hd] and k [T, Hkv, hd] at positions [T]."""
-        pos = positions.to(torch.long).clamp(0, self.rope.max_seq_len - 1)
-        c = self.rope.cos_cache[pos].float().contiguous()
-        s = self.rope.sin_cache[pos].float().contiguous()
+        c, s = ext.rope_rows(self.rope.cos_cache, self.rope.sin_cache, positions)
         return tuple(_RoPEFunction.apply(t.transpose(0, 1), c, s).transpose(0, 1) for t in (q, k))
 
     def _packed_positions(self, cu, tokens, max_seqlen):
@@ -552,7 +552,17 @@ class RACRoPEAttention(nn.Module):
                              "pass max_seqlen or positions")
         tok = torch.arange(tokens, device=cu.device, dtype=torch.int32)
         seq = torch.searchsorted(cu, tok, right=True) - 1
-        return tok - cu[seq]
+        # Rows behind the last sequence have no position of their own.
+        return torch.where(tok < cu[-1], tok - cu[seq], 0)
+
+    def _check_positions(self, positions, tokens):
+        if tuple(positions.shape) != (tokens,):
+            raise ValueError(f"positions must be [{tokens}], got {tuple(positions.shape)}")
+        rows = self.rope.max_seq_len
+        # On the device they are checked there.
+        if not positions.is_cuda and tokens and not 0 <= int(positions.min()) <= int(positions.max()) < rows:
+            raise ValueError(f"positions from {int(positions.min())} to {int(positions.max())}, RoPE tables of {rows}")
+        return positions if positions.dtype in (torch.int32, torch.int64) else positions.long()
 
     def _rows_context(self, x, is_causal=False, positions=None, cu_seqlens=None, cache=None, layer=0,
                       max_seqlen=None):
@@ -576,20 +586,24 @@ class RACRoPEAttention(nn.Module):
         elif cu_seqlens is None:
             if x.dim() != 3:
                 raise ValueError("x must be [batch, seq, d_model]")
-            cu = torch.arange(0, T + 1, max(1, x.shape[1]), device=x.device, dtype=torch.int32)
+            n = x.shape[1]
+            cu = torch.arange(0, T + 1, max(1, n), device=x.device, dtype=torch.int32)
             if positions is not None:
-                positions = positions.to(x.device).repeat(x.shape[0])
+                positions = self._check_positions(positions, n).to(x.device)
+            elif n > self.rope.max_seq_len:
+                raise ValueError(f"sequences of {n} rows, RoPE tables of {self.rope.max_seq_len}: pass positions")
             else:
-                positions = torch.arange(x.shape[1], device=x.device).repeat(x.shape[0])
-            max_seqlen = x.shape[1]
+                positions = torch.arange(n, device=x.device)
+            positions = positions.repeat(x.shape[0])
         else:
             if x.dim() == 3 and x.shape[0] != 1:
                 raise ValueError("packed x must be [tokens, d_model] or [1, tokens, d_model]")
             cu = cu_seqlens.to(torch.int32)
-        if positions is None:
-            positions = self._packed_positions(cu, T, max_seqlen)
-        elif tuple(positions.shape) != (T,):
-            raise ValueError(f"positions must be [{T}], got {tuple(positions.shape)}")
+            if positions is None:
+                positions = self._packed_positions(cu, T, max_seqlen)
+            else:
+                positions = self._check_positions(positions, T).to(x.device)
+                positions = torch.where(torch.arange(T, device=x.device) < cu[-1], positions, 0)
         qkv = self.qkv(x).reshape(T, H + 2 * Hk, hd)
         q, k, v = qkv[:, :H], qkv[:, H:H + Hk], qkv[:, H + Hk:]
         q, k = self._rotate_rows(q, k, positions)
