@@ -30,6 +30,7 @@ class RACCacheStep:
     def __init__(self, cache, ids, starts, counts, parents, table):
         self.cache, self.ids, self.starts_host, self.counts_host = cache, ids, starts, counts
         self.parents = parents
+        self._turns = [cache._turns[i] for i in ids]
         self.tokens = sum(counts)
         self.width = max(counts)
         self.longest = max(s + n for s, n in zip(starts, counts))
@@ -85,8 +86,8 @@ class RACCacheStep:
         return (o if self.uniform else o[self._pad]).to(q.dtype)
 
     def stale(self) -> bool:
-        return any(self.cache.length(i) != s + n if i in self.cache._seqs else True
-                   for i, s, n in zip(self.ids, self.starts_host, self.counts_host))
+        """Whether one of the sequences has taken another step, been cut back or freed since."""
+        return any(self.cache._turns.get(i) != t for i, t in zip(self.ids, self._turns))
 
 
 def _depths(parents: list[int]) -> list[int]:
@@ -121,6 +122,7 @@ class RACPagedCache:
         self._free = list(range(n_pages - 1, -1, -1))
         self._uses = [0] * n_pages                 # sequences that hold the page
         self._seqs: dict[int, tuple[list[int], int]] = {}
+        self._turns: dict[int, int] = {}           # of each sequence, how often its rows have changed
         self._next = 0
 
     # ── sequences ──
@@ -128,6 +130,7 @@ class RACPagedCache:
         """A new, empty sequence."""
         self._next += 1
         self._seqs[self._next - 1] = ([], 0)
+        self._turns[self._next - 1] = 0
         return self._next - 1
 
     def length(self, seq: int) -> int:
@@ -179,7 +182,7 @@ class RACPagedCache:
     def free(self, seq: int) -> None:
         """Gives up a sequence; pages that nobody else holds are free again."""
         pages, _ = self._get(seq)
-        del self._seqs[seq]
+        del self._seqs[seq], self._turns[seq]
         self._drop(pages)
 
     def truncate(self, seq: int, length: int) -> None:
@@ -187,6 +190,9 @@ class RACPagedCache:
         pages, n = self._get(seq)
         if not 0 <= length <= n:
             raise ValueError(f"length must be between 0 and {n}, got {length}")
+        if length == n:
+            return
+        self._turns[seq] += 1
         keep = -(-length // self.page_size)
         self._seqs[seq] = (pages[:keep], length)
         self._drop(pages[keep:])
@@ -237,6 +243,7 @@ class RACPagedCache:
         starts = [n for _, n in have]
         for s, p, n, c in zip(seqs, lists, starts, counts):
             self._seqs[s] = (p, n + c)
+            self._turns[s] += 1
         return RACCacheStep(self, seqs, starts, counts, parents, lists)
 
     def accept(self, step: RACCacheStep, accepted: list[list[int]]) -> None:
