@@ -167,6 +167,23 @@ class RACPagedCache:
             at = torch.tensor([src, dst], dtype=torch.int32).to(self.k.device)
             ext.cache_copy_pages_(self.k, self.v, at[0], at[1])
 
+    def _shared(self, places: list[tuple[list[int], int]]) -> list[tuple[list[int], int]]:
+        """Of places (a sequence's pages, index) that are to be written to, those whose page another sequence keeps."""
+        uses, got = list(self._uses), []
+        for pages, at in places:
+            if uses[pages[at]] > 1:
+                uses[pages[at]] -= 1
+                got.append((pages, at))
+        return got
+
+    def _replace(self, places: list[tuple[list[int], int]], new: list[int]) -> None:
+        """Puts copies, on the pages `new`, in these places."""
+        src = [pages[at] for pages, at in places]
+        for (pages, at), p in zip(places, new):
+            pages[at] = p
+        self._drop(src)
+        self._copy(src, new)
+
     def fork(self, seq: int) -> int:
         """A new sequence with seq's rows.  Full pages are shared; a page that is partly filled is copied."""
         pages, n = self._get(seq)
@@ -221,22 +238,12 @@ class RACPagedCache:
         ps = self.page_size
         # A page that new rows are written to and that others hold too is copied first.  Counted before
         # anything is taken: a step that does not fit changes nothing.
-        uses, shared, grow = list(self._uses), [], []
-        for i, ((pages, n), c) in enumerate(zip(have, counts)):
-            at = n // ps
-            if n % ps and uses[pages[at]] > 1:
-                uses[pages[at]] -= 1
-                shared.append((i, at))
-            grow.append(-(-(n + c) // ps) - len(pages))
-        new = self._take(len(shared) + sum(grow))
         lists = [list(pages) for pages, _ in have]
-        src = [lists[i][at] for i, at in shared]
-        dst = new[:len(shared)]
-        for (i, at), p in zip(shared, dst):
-            lists[i][at] = p
-        self._drop(src)
-        self._copy(src, dst)
+        shared = self._shared([(p, n // ps) for p, (_, n) in zip(lists, have) if n % ps])
+        grow = [-(-(n + c) // ps) - len(p) for p, (_, n), c in zip(lists, have, counts)]
+        new = self._take(len(shared) + sum(grow))
         at = len(shared)
+        self._replace(shared, new[:at])
         for i, g in enumerate(grow):
             lists[i] += new[at:at + g]
             at += g
@@ -248,7 +255,8 @@ class RACPagedCache:
 
     def accept(self, step: RACCacheStep, accepted: list[list[int]]) -> None:
         """Keeps the given new rows of a step (rising node numbers, one list a sequence) and forgets the
-        others: the kept rows move together in every layer, the sequences shorten to them."""
+        others: the kept rows move together in every layer, the sequences shorten to them.  Pages that others
+        hold too, forks of these sequences, are copied before a row moves into them."""
         if step.cache is not self or step.stale():
             raise ValueError("not the latest step of these sequences")
         if len(accepted) != len(step.ids):
@@ -259,9 +267,20 @@ class RACPagedCache:
         if any(a != list(range(len(a))) for a in accepted):
             if step.width > ext.MAX_NEW_ROWS:
                 raise ValueError(f"at most {ext.MAX_NEW_ROWS} new rows can be moved together")
-            w, b = step.width, len(accepted)
+            w, b, ps = step.width, len(accepted), self.page_size
+            lists = [list(self._get(i)[0]) for i in step.ids]
+            into = [sorted({(s + i) // ps for i, x in enumerate(a) if x != i})
+                    for s, a in zip(step.starts_host, accepted)]
+            shared = self._shared([(p, at) for p, ats in zip(lists, into) for at in ats])
+            table = step.page_table
+            if shared:
+                self._replace(shared, self._take(len(shared)))
+                for i, p in zip(step.ids, lists):
+                    self._seqs[i] = (p, self.length(i))
+                flat = [x for p in lists for x in p + [0] * (table.shape[1] - len(p))]
+                table = torch.tensor(flat, dtype=torch.int32).view(table.shape).to(self.k.device)
             flat = [x for a in accepted for x in list(a) + [0] * (w - len(a))] + [len(a) for a in accepted]
             t = torch.tensor(flat, dtype=torch.int32).to(self.k.device)
-            ext.cache_compact_(self.k, self.v, step.page_table, step.starts, t[:b * w].view(b, w), t[b * w:])
+            ext.cache_compact_(self.k, self.v, table, step.starts, t[:b * w].view(b, w), t[b * w:])
         for i, s, a in zip(step.ids, step.starts_host, accepted):
             self.truncate(i, s + len(a))

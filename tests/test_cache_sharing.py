@@ -41,3 +41,41 @@ def test_a_step_of_the_same_length_is_another_step(quiet):  # noqa: F811
     c.free(b)
     out_of_date(c, both)
     _consistent(c)
+
+
+@pytest.mark.parametrize("drafted,kept", [(8, [0, 3]), (8, [1, 2, 6]), (9, [8]), (6, [0, 1, 5])])
+def test_accepted_rows_leave_a_fork_as_it_was(quiet, drafted, kept):  # noqa: F811
+    """A fork of a sequence that holds drafted rows shares its full pages: those that receive a moved row are copied."""
+    c = cache(12, layers=2)
+    a = c.add()
+    _write(c, c.step([a], 2), 10)
+    step = c.step([a], drafted, parents=[-1] * drafted)
+    _write(c, step, 100)
+    f = c.fork(a)
+    before = _rows(c, a)
+    c.accept(step, [kept])
+    _consistent(c)
+    assert _rows(c, f) == before
+    assert _rows(c, a) == before[:2] + [100 + x for x in kept]
+    # What neither holds any longer is free, what both hold is still shared.
+    assert c.pages(a)[0] != c.pages(f)[0] or kept[:2] == [0, 1]
+    c.free(f)
+    assert _rows(c, a) == before[:2] + [100 + x for x in kept]
+    c.free(a)
+    assert c.free_pages == 12
+
+
+def test_accept_that_does_not_fit_changes_nothing(quiet):  # noqa: F811
+    c = cache(4)
+    a, b = c.add(), c.add()
+    step = c.step([a, b], 4, parents=[-1, 0, 0, 0])
+    _write(c, step, 50)
+    f, g = c.fork(a), c.fork(b)
+    c.step([f], 5)                                              # two pages more: none is left
+    pages, rows = c.pages(a), [_rows(c, s) for s in (a, b, g)]
+    with pytest.raises(RuntimeError, match="free"):
+        c.accept(step, [[1], [2]])
+    _consistent(c)
+    assert c.pages(a) == pages and [_rows(c, s) for s in (a, b, g)] == rows and not step.stale()
+    c.accept(step, [[0], [0, 1]])                               # nothing moves: no page is needed
+    assert _rows(c, a) == rows[0][:1] and _rows(c, b) == rows[1][:2] and _rows(c, g) == rows[2]
