@@ -68,6 +68,8 @@ class RACCacheStep:
         c = self.cache
         if self.stale():
             raise ValueError("the sequences of this step have moved on: take a new step")
+        if any(c._forked.get(i) == t for i, t in zip(self.ids, self._turns)):
+            raise ValueError("a sequence of this step was forked before all layers had run: take a new step")
         kp, vp = c.k[layer], c.v[layer]
         k, v = k.to(c.dtype), v.to(c.dtype)
         ext.cache_append_(kp, vp, k, v, self.page_table, self.starts, self.cu_seqlens)
@@ -123,6 +125,7 @@ class RACPagedCache:
         self._uses = [0] * n_pages                 # sequences that hold the page
         self._seqs: dict[int, tuple[list[int], int]] = {}
         self._turns: dict[int, int] = {}           # of each sequence, how often its rows have changed
+        self._forked: dict[int, int] = {}          # the count at which it was last forked
         self._next = 0
 
     # ── sequences ──
@@ -185,7 +188,8 @@ class RACPagedCache:
         self._copy(src, new)
 
     def fork(self, seq: int) -> int:
-        """A new sequence with seq's rows.  Full pages are shared; a page that is partly filled is copied."""
+        """A new sequence with seq's rows.  Full pages are shared; a page that is partly filled is copied.  The rows
+        of seq's last step have to be there, in every layer: none of its layers runs after the fork."""
         pages, n = self._get(seq)
         whole = n // self.page_size
         last = self._take(len(pages) - whole)
@@ -194,12 +198,14 @@ class RACPagedCache:
             self._uses[p] += 1
         new = self.add()
         self._seqs[new] = (pages[:whole] + last, n)
+        self._forked[seq] = self._turns[seq]
         return new
 
     def free(self, seq: int) -> None:
         """Gives up a sequence; pages that nobody else holds are free again."""
         pages, _ = self._get(seq)
         del self._seqs[seq], self._turns[seq]
+        self._forked.pop(seq, None)
         self._drop(pages)
 
     def truncate(self, seq: int, length: int) -> None:

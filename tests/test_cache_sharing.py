@@ -79,3 +79,25 @@ def test_accept_that_does_not_fit_changes_nothing(quiet):  # noqa: F811
     assert c.pages(a) == pages and [_rows(c, s) for s in (a, b, g)] == rows and not step.stale()
     c.accept(step, [[0], [0, 1]])                               # nothing moves: no page is needed
     assert _rows(c, a) == rows[0][:1] and _rows(c, b) == rows[1][:2] and _rows(c, g) == rows[2]
+
+
+@pytest.mark.parametrize("rows", [3, 4, 6])
+def test_no_layer_writes_after_a_fork(quiet, monkeypatch, rows):  # noqa: F811
+    """The rows of a layer that is run after a fork would be missing in the fork's copied page, and would be
+    written into pages that it shares: the step is refused.  Its rows may still be accepted."""
+    ran = []
+    monkeypatch.setattr("rac_b200.ext.cache_append_", lambda *a: ran.append(a))
+    c = cache(12, layers=2)
+    a, b = c.add(), c.add()
+    step = c.step([a, b], rows, parents=[-1] * rows)
+    _write(c, step, 7)
+    c.fork(b)
+    with pytest.raises(ValueError, match="forked"):
+        step.attend(1, *[c.k.new_zeros(2 * rows, 1, 32)] * 3)
+    assert not ran and not step.stale()
+    c.accept(step, [[rows - 1], [0]])
+    step = c.step([a, b], 1)
+    with pytest.raises(ValueError, match="CUDA"):               # runs, as far as it can here
+        step.attend(1, *[c.k.new_zeros(2, 1, 32)] * 3)
+    assert len(ran) == 1
+    _consistent(c)
