@@ -514,6 +514,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_cached_tc(const __grid_constant
     }
     fence_before();
     __syncthreads();
+    settle(gone);
     fence_after();
     if (warp == 12) tmem_free(tm, 512);
     if (threadIdx.x == 0 && *gone) atomicOr(a.err, kErrTcWait);

@@ -385,6 +385,7 @@ __device__ __forceinline__ void block_dkv(const BwdArgs& a, uint8_t* sm, unsigne
     }
     fence_before();
     __syncthreads();
+    settle(gone);
     fence_after();
     if (warp == 8) tmem_free(tm, 512);
     if (threadIdx.x == 0 && *gone) atomicOr(a.err, kErrTcWait);
@@ -565,6 +566,7 @@ __device__ __forceinline__ void block_dq(const BwdArgs& a, uint8_t* sm, unsigned
     }
     fence_before();
     __syncthreads();
+    settle(gone);
     fence_after();
     if (warp == 8) tmem_free(tm, 512);
     if (threadIdx.x == 0 && *gone) atomicOr(a.err, kErrTcWait);

@@ -542,6 +542,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_f32_fwd(const __grid_constant__
     }
     fence_before();
     __syncthreads();
+    settle(gone);
     fence_after();
     if (warp == 8) tmem_free(tm, 512);
     if (threadIdx.x == 0 && *gone) atomicOr(a.err, kErrTcWait);
@@ -845,6 +846,7 @@ __device__ __forceinline__ void block_dkv(const Args& a, uint8_t* sm, unsigned b
     }
     fence_before();
     __syncthreads();
+    settle(gone);
     fence_after();
     if (warp == 8) tmem_free(tm, 512);
     if (threadIdx.x == 0 && *gone) atomicOr(a.err, kErrTcWait);
@@ -1046,6 +1048,7 @@ __device__ __forceinline__ void block_dq(const Args& a, uint8_t* sm, unsigned bl
     }
     fence_before();
     __syncthreads();
+    settle(gone);
     fence_after();
     if (warp == 8) tmem_free(tm, 512);
     if (threadIdx.x == 0 && *gone) atomicOr(a.err, kErrTcWait);

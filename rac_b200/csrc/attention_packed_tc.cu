@@ -325,6 +325,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_packed_fwd_tc(const __grid_cons
     }
     fence_before();
     __syncthreads();
+    settle(&gone);
     fence_after();
     if (warp == 8) tmem_free(tm, 512);
     if (threadIdx.x == 0 && gone) atomicOr(a.err, kErrTcWait);

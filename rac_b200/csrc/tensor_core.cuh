@@ -37,7 +37,7 @@ __device__ __forceinline__ bool bar_try(uint64_t* bar, uint32_t parity) {
 
 // Every wait ends: after kWaitNs, or when another thread of the block gave up,
 // `gone` is set and the wait returns false.  The kernel then skips the rest of
-// its work, frees its tensor memory and returns.
+// its work, settles, frees its tensor memory and returns.
 constexpr uint64_t kWaitNs = 4000000000ull;
 __device__ __forceinline__ uint64_t now_ns() {
     uint64_t t;
@@ -56,6 +56,16 @@ __device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, volatil
     return false;
 }
 constexpr unsigned int kErrTcWait = 16u;      // bit 4 of the device error word
+// Before such a block leaves: its copies and products under way, which end by
+// themselves within microseconds, must not land in memory that another block has
+// got by then.  No barrier tells (one that would have is what the block gave up
+// on), so it waits a millisecond; by every thread, after the block has met.
+__device__ __forceinline__ void settle(volatile int* gone) {
+    if (!*gone) return;
+    const uint64_t t0 = now_ns();
+#pragma unroll 1
+    for (int i = 0; i < 4096 && now_ns() - t0 < 1000000ull; ++i) __nanosleep(1000);
+}
 
 // ── TMA ───────────────────────────────────────────────────────────────────
 __device__ __forceinline__ void load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
