@@ -204,8 +204,8 @@ int rac_check_device_errors(void *stream);
  * dout, and writes dq like q, dk and dv like k (contiguous), zeros behind the
  * last sequence.  The same inputs give the same bits.
  *
- * workspace: rac_attention_packed_workspace() bytes, 256-byte aligned (may be
- * NULL where that is 0), free again when the call's kernels are done. */
+ * workspace: rac_attention_packed_workspace() bytes on the current device, 256-byte
+ * aligned (may be NULL where that is 0), free again when the call's kernels are done. */
 typedef struct {
     const void *q, *k, *v;
     const int *cu_seqlens;

@@ -230,18 +230,6 @@ int cached_f32(const CachedParams& p, int blocks, cudaStream_t s) {
 
 }  // namespace
 
-static int sm_count() {
-    static int per_dev[64] = {};
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { cudaGetLastError(); return 0; }
-    if (per_dev[dev] == 0) {
-        int n = 0;
-        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) { cudaGetLastError(); return 0; }
-        per_dev[dev] = n;
-    }
-    return per_dev[dev];
-}
-
 // Two pieces a block, of the kernel that needs more.
 size_t attention_cached_workspace(int, int nodes, int heads, int kv_heads, int head_dim) {
     const int sms = sm_count();
@@ -267,7 +255,6 @@ int attention_cached(const CachedParams& p, cudaStream_t s) {
         p.heads / p.kv_heads > 4096)
         return kErrInvalidDim;
     const int sms = sm_count();
-    if (sms == 0) return kErrCuda;
     if (!p.ws || (reinterpret_cast<uintptr_t>(p.ws) & 15u) ||
         p.ws_bytes < attention_cached_workspace(p.batch, p.nodes, p.heads, p.kv_heads, p.head_dim))
         return kErrAlloc;

@@ -1084,10 +1084,11 @@ __global__ void __launch_bounds__(256) k_add_heads(const float* __restrict__ dk,
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
 // Fewer blocks than twice the SMs leave some idle while others go through a whole
-// group: then each query head has a block of its own.  2048 tokens of 16 heads (4
-// key/value heads): 64 busy blocks 181 us, 256 of them 77 us with the sums.
+// group: then each query head has a block of its own, for two more tensors of q's
+// size.  2048 tokens of 16 heads (4 key/value heads): 64 busy blocks 181 us, 256 of
+// them 77 us with the sums.
 bool by_head(long long tokens, int heads, int kv_heads) {
-    return heads > kv_heads && tokens / kWide * kv_heads < 2 * 148;
+    return heads > kv_heads && tokens / kWide * kv_heads < 2 * sm_count();
 }
 
 // Workspace: parts of q, k, v (and dO), their factors, what bounds dS, D, and dk and dv by query head.

@@ -161,7 +161,7 @@ static int pick_fixed(const GemmParams& p, int layout, int v, cudaStream_t s) {
 
 static bool aligned16(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0; }
 
-static int sm_count() {
+int sm_count() {
     static std::atomic<int> cached[64] = {};
     int dev = 0;
     cudaGetDevice(&dev);
@@ -188,8 +188,6 @@ void keep_device_pool() {
         cudaGetLastError();
     });
 }
-
-static int sm_count();
 
 // 3 for M <= 32.  Otherwise the 64x64 or 32x64 tile that minimises the work
 // of the most loaded SM, ceil(tiles / SMs) x tile area -- the GEMM is

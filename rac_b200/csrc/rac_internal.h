@@ -97,4 +97,7 @@ int record_status(int st, const char* msg);
 // Per-device error word that bounded device loops set (see rac_device.cuh).
 unsigned int* device_error_word(int device);
 
+// SMs of the current device.
+int sm_count();
+
 }  // namespace racb

@@ -17,6 +17,7 @@ Every call needs CUDA tensors: there is no CPU path, and a CPU tensor is a
 """
 from __future__ import annotations
 
+import contextlib
 import functools
 
 import torch
@@ -479,8 +480,12 @@ def _check_packed(q, k, v, cu_seqlens):
     return _elem(q, k, v), _index("cu_seqlens", cu_seqlens, cu_seqlens.shape), t, h, ks[1], hd
 
 
-def _packed_workspace(like, *sizes):
-    n = _lib.lib().rac_attention_packed_workspace(*sizes) if sizes[-2] == 0 or sizes[-1] else 0
+def _packed_workspace(like, device, *sizes):
+    n = 0
+    if sizes[-2] == 0 or sizes[-1]:
+        # Its size goes by the device's SMs.
+        with contextlib.nullcontext() if torch.cuda.current_device() == device else torch.cuda.device(device):
+            n = _lib.lib().rac_attention_packed_workspace(*sizes)
     return (like.new_empty(n, dtype=torch.uint8), n) if n else (None, 0)
 
 
@@ -517,7 +522,7 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     v, vp, vs = _rows(v, w)
     o = _like(q) if out is None else out
     n = cu.shape[0] - 1
-    ws, ws_n = _packed_workspace(q, t, n, h, kv, hd, elem, 0)
+    ws, ws_n = _packed_workspace(q, d, t, n, h, kv, hd, elem, 0)
     _launch("rac_attention_packed_async", _lib.PACKED_ARGS.pack(
         qp, kp, vp, cu.data_ptr(), o.data_ptr(), 0 if lse is None else lse.data_ptr(),
         0 if out_low is None else out_low.data_ptr(), 0, 0, 0, 0,
@@ -548,7 +553,7 @@ def attention_packed_backward(grad_out: torch.Tensor, q: torch.Tensor, k: torch.
     g, gp, gs = _rows(grad_out, w)
     dq, dk, dv = _like(q), _like(k), _like(v)
     n = cu.shape[0] - 1
-    ws, ws_n = _packed_workspace(q, t, n, h, kv, hd, elem, 1)
+    ws, ws_n = _packed_workspace(q, d, t, n, h, kv, hd, elem, 1)
     _launch("rac_attention_packed_backward_async", _lib.PACKED_ARGS.pack(
         qp, kp, vp, cu.data_ptr(), out.data_ptr(), lse.data_ptr(), 0 if out_low is None else out_low.data_ptr(), gp, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
         ws.data_ptr() if ws_n else 0, *qs, *ks, *vs, *gs, t, ws_n, n, h, kv, hd, elem, bool(is_causal), 1,
