@@ -496,7 +496,7 @@ class RACRoPEAttention(nn.Module):
         super().__init__()
         assert d_model % n_heads == 0
         self.d_model, self.n_heads = d_model, n_heads
-        self.n_kv_heads = n_heads if n_kv_heads is None else n_kv_heads
+        self._kv_heads = n_kv_heads
         if self.n_kv_heads < 1 or n_heads % self.n_kv_heads:
             raise ValueError(f"n_heads={n_heads} must be a multiple of n_kv_heads={self.n_kv_heads}")
         self.d_head = d_model // n_heads
@@ -507,6 +507,14 @@ class RACRoPEAttention(nn.Module):
         self.rope = RACRoPE(self.d_head, max_seq_len=max_seq_len, base=rope_base,
                             device=device, dtype=dtype or torch.float32)
         self.dropout = nn.Dropout(dropout) if dropout > 0 else nn.Identity()
+
+    # Without heads of their own, keys and values have as many as the queries: also where n_heads
+    # is set later (a shard's), and in a module that was saved before this attribute was there.
+    _kv_heads: Optional[int] = None
+
+    @property
+    def n_kv_heads(self) -> int:
+        return self.n_heads if self._kv_heads is None else self._kv_heads
 
     def _context(self, x, mask=None, is_causal=False, positions=None, n_heads=None):
         """Attention output before out_proj, [B, T, heads*d_head]."""
