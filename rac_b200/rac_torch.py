@@ -206,7 +206,8 @@ class _RoPEFunction(Function):
 
 def _rope(x, cos, sin):
     out = x.to(torch.float32, memory_format=torch.contiguous_format, copy=True)
-    ext.rope_apply_(out, cos, sin, form=1)
+    if out.numel():
+        ext.rope_apply_(out, cos, sin, form=1)
     return out if x.dtype == torch.float32 else out.to(x.dtype)
 
 
