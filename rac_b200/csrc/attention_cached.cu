@@ -143,7 +143,8 @@ __global__ void __launch_bounds__(kThreadsF32, kBlocksPerSm) k_cached_f32(const 
                             o[i].x *= y; o[i].y *= y; o[i].z *= y; o[i].w *= y;
                         }
                     }
-                    const float wgt = see && m != -INFINITY ? exp2f(x - m) : 0.f;
+                    // No maximum yet: the score is minus infinity, or NaN, which maxima pass over.
+                    const float wgt = !see ? 0.f : m != -INFINITY ? exp2f(x - m) : x == -INFINITY ? 0.f : x;
                     l += wgt;
 #pragma unroll
                     for (int i = 0; i < NB; ++i)

@@ -461,7 +461,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_cached_tc(const __grid_constant
                 for (int i = row; i < kRowTile; i += span) M = fmaxf(M, join_ml[i].x);
                 for (int i = row; i < kRowTile; i += span) {
                     const float2 y = join_ml[i];
-                    L += y.x == -INFINITY ? 0.f : y.y * exp2_fast(y.x - M);
+                    L += y.x == -INFINITY ? y.y : y.y * exp2_fast(y.x - M);      // without a maximum: 0, or NaN
                 }
                 const float f = m == -INFINITY ? 0.f : exp2_fast(m - M), inv = L == 0.f ? 0.f : 1.f / L;
                 const int most = 16 / a.copies;        // columns that a thread adds up: 4 or 8
