@@ -1,6 +1,9 @@
-"""RACPagedCache: steps that are out of date, and pages that forks share.  The accounts are the host's and need no GPU."""
+"""RACPagedCache: steps that are out of date, and pages that forks share."""
 import pytest
+import torch
 
+from rac_b200 import ext
+from rac_b200 import rac_torch as R
 from rac_b200.cache import RACPagedCache
 from test_cache_pages import _consistent, _rows, _write, quiet  # noqa: F401
 
@@ -100,4 +103,38 @@ def test_no_layer_writes_after_a_fork(quiet, monkeypatch, rows):  # noqa: F811
     with pytest.raises(ValueError, match="CUDA"):               # runs, as far as it can here
         step.attend(1, *[c.k.new_zeros(2, 1, 32)] * 3)
     assert len(ran) == 1
+    _consistent(c)
+
+
+@pytest.mark.gpu
+def test_forks_of_drafted_rows_answer_on(cuda):
+    """A fork taken between a drafted tree and its acceptance goes on with the whole tree's rows, its sequence with the
+    accepted ones: each as in a packed pass over them.  32-bit sums of at most 256 terms: 1e-5 of the largest value."""
+    torch.manual_seed(0)
+    blk = R.RACLlamaBlock(128, 4, ff_dim=192, max_seq_len=64, n_kv_heads=2).to(cuda)
+    x = torch.randn(26, 128, device=cuda)
+
+    def whole(rows):
+        t = x[rows]
+        return blk(t, is_causal=True, cu_seqlens=torch.tensor([0, len(rows)], dtype=torch.int32, device=cuda))
+
+    with torch.no_grad():
+        c = RACPagedCache(1, 20, 2, 32, page_size=4, device=cuda)
+        a = c.add()
+        blk(x[:7], is_causal=True, cache=c.step([a], 7))
+        step = c.step([a], 12, parents=[-1, 0, 0] + list(range(2, 11)))       # 0, 1 and 0, 2, 3, ... 11
+        blk(x[7:19], is_causal=True, cache=step)
+        f = c.fork(a)
+        held = [c.k[:, c.pages(f)].clone(), c.v[:, c.pages(f)].clone()]
+        c.accept(step, [[0, 2, 3, 4, 5, 6]])
+        assert torch.equal(c.k[:, c.pages(f)], held[0]) and torch.equal(c.v[:, c.pages(f)], held[1])
+        got = blk(x[19:21], is_causal=True, cache=c.step([a], 2))
+        want = whole(list(range(8)) + list(range(9, 14)) + [19, 20])[-2:]
+        assert (got - want).abs().max() <= 1e-5 * want.abs().max()
+        c.free(a)
+        c.truncate(f, 8)
+        got = blk(x[8:26], is_causal=True, cache=c.step([f], 18))
+        want = whole(list(range(26)))[8:]
+        assert (got - want).abs().max() <= 1e-5 * want.abs().max()
+    ext.check_device_errors(cuda)
     _consistent(c)
