@@ -572,7 +572,7 @@ struct BwdShape {
     // Places of Q (dk/dv) or K (dq), which a later product reads again, and of dO or V.
     static constexpr int A = HD == 32 ? 3 : 2, B = HD == 128 ? 1 : 2;
     static constexpr int N = narrow<HD>(), TILE = Sh::tile(N), KEPT = Sh::tile(kWide);
-    static constexpr int RING = 2 * KEPT, STAT = RING + (A + B) * TILE, BARS = STAT + 2 * 2 * N * 4;
+    static constexpr int RING = 2 * KEPT, STAT = RING + (A + B) * TILE, BARS = STAT + 2 * 2 * N * 4 + 2 * 8;
     static constexpr int SMEM = BARS + 512;
     static_assert(SMEM <= 227 * 1024, "shared memory");
 };
@@ -587,6 +587,7 @@ __device__ __forceinline__ void block_dkv(const Args& a, uint8_t* sm, unsigned b
     uint8_t *ks = sm, *vs = sm + Bs::KEPT, *qr = sm + Bs::RING, *gr = qr + NA * TILE;
     float* st_lse = reinterpret_cast<float*>(sm + Bs::STAT);       // negative; [2][64]
     float* st_d = st_lse + 2 * N;
+    float2* st_ds = reinterpret_cast<float2*>(st_d + 2 * N);       // factors of dS: of acc, and back; [2]
     uint64_t* bars = reinterpret_cast<uint64_t*>(sm + Bs::BARS);
     uint64_t *q_full = bars, *q_empty = q_full + NA, *q_fixed = q_empty + NA, *g_full = q_fixed + NA, *g_empty = g_full + NB,
              *g_fixed = g_empty + NB, *kv_full = g_fixed + NB, *stat_full = kv_full + 2,
@@ -711,7 +712,9 @@ __device__ __forceinline__ void block_dkv(const Args& a, uint8_t* sm, unsigned b
                 const bool ok = i < 2 || bar_wait(stat_empty + sl, (i / 2 - 1) & 1, gone);
                 if (!__all_sync(0xffffffffu, ok)) break;
                 const long long qs = slot_of(t, row_of(i)) * a.heads + h;
-                const float up = ds_factors(a.fg[qs], a.gnorm[qs], a.dtop[qs], fv, vnorm).up * kPDown;
+                const DsFactors ds = ds_factors(a.fg[qs], a.gnorm[qs], a.dtop[qs], fv, vnorm);
+                const float up = ds.up * kPDown;
+                if (lane == 0) st_ds[sl] = make_float2(ds.acc, ds.down);
                 for (int r = lane; r < N; r += 32) {
                     const int row = row_of(i) + r;
                     float x = INFINITY, d = 0.f;
@@ -736,7 +739,7 @@ __device__ __forceinline__ void block_dkv(const Args& a, uint8_t* sm, unsigned b
         constexpr int W = HD == 32 ? 32 : HD / 2;
         const uint32_t v0 = tV + lanes + (HD == 32 ? 0 : W * half), k0 = tK + lanes + (HD == 32 ? 0 : W * half);
         const long long ks = slot_of(t, t.row0) * a.kv_heads + kvh;
-        const float fk = a.fk[ks], fv = a.fv[ks], vnorm = a.vnorm[ks];
+        const float fk = a.fk[ks];
         float2 av[W / 2], ak[W / 2];
 #pragma unroll
         for (int i = 0; i < W / 2; ++i) av[i] = ak[i] = both(0.f);
@@ -758,7 +761,6 @@ __device__ __forceinline__ void block_dkv(const Args& a, uint8_t* sm, unsigned b
             const int sl = i & 1, q0 = row_of(i);
             const long long qs = slot_of(t, q0) * a.heads + head_of(i);
             const float fq = a.fq[qs], fg = a.fg[qs], c = score_factor(a.c * fq, fk);
-            const DsFactors ds = ds_factors(fg, a.gnorm[qs], a.dtop[qs], fv, vnorm);
             ok = bar_wait(stat_full + sl, (i / 2) & 1, gone) && bar_wait(s_ready, i & 1, gone);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
@@ -793,7 +795,7 @@ __device__ __forceinline__ void block_dkv(const Args& a, uint8_t* sm, unsigned b
             bar_arrive(p_ready);
             if (i) add_k(i - 1);
             if (!ok) break;
-            take_k = fminf(fq * ds.down, 3e38f);
+            take_k = fminf(fq * st_ds[sl].y, 3e38f);
             ok = __all_sync(0xffffffffu, bar_wait(dp_ready, i & 1, gone));
             if (!ok) break;
             fence_after();
@@ -805,7 +807,7 @@ __device__ __forceinline__ void block_dkv(const Args& a, uint8_t* sm, unsigned b
 #pragma unroll
                 for (int x = 0; x < 16; x += 2) {
                     const float4 z = *reinterpret_cast<const float4*>(dd + 2 * (b + x));       // -D
-                    const float2 f = both(ds.acc);
+                    const float2 f = both(st_ds[sl].x);
                     p[b + x] = __fmul2_rn(p[b + x], __ffma2_rn(pair(s[2 * x], s[2 * x + 1]), f, make_float2(z.x, z.y)));
                     p[b + x + 1] = __fmul2_rn(p[b + x + 1], __ffma2_rn(pair(s[2 * x + 2], s[2 * x + 3]), f, make_float2(z.z, z.w)));
                 }
@@ -968,7 +970,7 @@ __device__ __forceinline__ void block_dq(const Args& a, uint8_t* sm, unsigned bl
         constexpr int W = HD == 32 ? 32 : HD / 2;
         const uint32_t q0 = tQ + lanes + (HD == 32 ? 0 : W * half), p0 = tP + lanes + C * half;
         const long long qslot = slot_of(t, t.row0) * a.heads + head;
-        const float fq = a.fq[qslot], fg = a.fg[qslot], gnorm = a.gnorm[qslot], dtop = a.dtop[qslot];
+        const float fq = a.fq[qslot];
         float lse = INFINITY, d = 0.f;
         float2 acc[W / 2];
 #pragma unroll
@@ -994,7 +996,7 @@ __device__ __forceinline__ void block_dq(const Args& a, uint8_t* sm, unsigned bl
         for (int j = 0; j < n; ++j) {
             const uint32_t s0 = tS + lanes + N * (j & 1) + C * half;
             const long long ks = slot_of(t, j * N) * a.kv_heads + kvh;
-            const float fk = a.fk[ks], fv = a.fv[ks], c = score_factor(a.c * fq, fk);
+            const float c = score_factor(a.c * fq, a.fk[ks]);
             ok = __all_sync(0xffffffffu, bar_wait(s_ready + (j & 1), (j >> 1) & 1, gone));
             if (!ok) break;
             fence_after();
@@ -1011,9 +1013,10 @@ __device__ __forceinline__ void block_dq(const Args& a, uint8_t* sm, unsigned bl
             }
             if (j) add_q(j - 1);
             if (!ok) break;
-            const DsFactors ds = ds_factors(fg, gnorm, dtop, fv, a.vnorm[ks]);
+            // Read here, not before the weights: registers are what this kernel lacks.
+            const DsFactors ds = ds_factors(a.fg[qslot], a.gnorm[qslot], a.dtop[qslot], a.fv[ks], a.vnorm[ks]);
             const float du = d * (ds.up * kPDown);
-            take_f = fminf(fk * ds.down, 3e38f);
+            take_f = fminf(a.fk[ks] * ds.down, 3e38f);
             ok = __all_sync(0xffffffffu, bar_wait(dp_ready, j & 1, gone));
             if (!ok) break;
             fence_after();
