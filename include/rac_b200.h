@@ -232,7 +232,8 @@ int rac_attention_packed_backward_async(const rac_attention_packed_args *args, v
  * or `nodes` where counts is NULL; at most 64) included: they are in the
  * cache already.  New row i sees every row before the new ones and the new
  * rows j whose bit is set in tree[b, i] (int64 [batch, nodes]), j <= i where
- * tree is NULL; a row that sees nothing gives zeros.  q [batch, nodes, heads,
+ * tree is NULL; a row that sees nothing gives zeros (the values of new rows
+ * must be finite, seen or not).  q [batch, nodes, heads,
  * head_dim]; out contiguous, rows from counts[b] on as they were or zeros
  * (zero_rest).  Pages outside [0, n_pages) are not read: their rows count as
  * hidden and rac_check_device_errors() reports RAC_ERR_DEVICE.  workspace:

@@ -16,10 +16,9 @@
 // With two row tiles each has its own issuing thread; one thread for both spent
 // 2 x 500 cycles a tile on the way between them.
 // Measured, bf16, dim 128, 32 heads on 8: one token for each of 64 sequences of 500
-// to 8100 rows 214 to 243 us, 5.3 to 4.7 TB/s of the cache's bytes, bound by them
-// and by each block's way to its first tile; 48 tree nodes for each of 8 sequences
-// of 777 to 16384 rows 115 to 121 us, bound by the exponentials of both row tiles
-// and, 16 us, the join.
+// to 8100 rows 243 us, 4.7 TB/s of the cache's bytes, bound by them and by each
+// block's way to its first tile; 48 tree nodes for each of 8 sequences of 777 to
+// 16384 rows 121 us, bound by the exponentials of both row tiles and, 16 us, the join.
 #include "cached_split.cuh"
 
 namespace racb {

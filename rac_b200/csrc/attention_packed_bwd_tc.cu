@@ -22,8 +22,8 @@
 //
 // Bound: the seven products (the tensor pipe is busy half of the time) and the
 // way of P and dS through registers between them.  8192 causal tokens in three
-// sequences, 32 heads of 128 on 8, bf16, forward and backward: 0.99 ms, and up to
-// 1.07 where the power limit lowers the clock.
+// sequences, 32 heads of 128 on 8, bf16, forward and backward: 1.11 ms, of which
+// these kernels take 0.76 and D 0.03.
 #include "attn_common.cuh"
 #include "tensor_core.cuh"
 

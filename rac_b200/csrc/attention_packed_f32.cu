@@ -18,10 +18,10 @@
 //
 // Bound: the three products of each pair of tiles, and between them the way of
 // every partial sum through registers.  4096 tokens in ragged causal prompts, 32
-// heads of 128 with keys of their own: 261 us, of them 61 for the parts (87 us is
+// heads of 128 with keys of their own: 288 us, of them 68 for the parts (87 us is
 // what the products alone need); 2048 tokens, 16 heads of 64 on 4, both ways, forward and backward:
-// 174 to 187 us, of which splitting takes 23, the forward 43, dk and dv 70, the
-// heads' sums 6, dq 51 when they run one by one.
+// 180 us; one by one splitting takes 9 and 17, the forward 44, dq, dk and dv 118, the
+// heads' sums 7.
 #include "attn_common.cuh"
 #include "tensor_core.cuh"
 

@@ -4,8 +4,8 @@
 // Nothing is computed: each moved byte is read once and written once, in
 // 16-byte units whatever the element type, and HBM bandwidth (launch latency
 // for a few rows) bounds them.  96 pages of 256 KiB (k and v, 64 rows of 8 heads of
-// 128, bf16) copied in each of 16 layers: 138 us, 5.9 TB/s read and written, 0.90
-// of the copy peak.  4072 rows of them appended in one layer: 10.8 us; accepted
+// 128, bf16) copied in each of 16 layers: 140 us, 5.8 TB/s read and written, 0.88
+// of the copy peak.  4072 rows of them appended in one layer: 12 us; accepted
 // rows of trees moved together: 10 us, the launch's time.  Page and row numbers come from device memory;
 // one outside its range is skipped and sets the device error word.
 #include "attn_common.cuh"

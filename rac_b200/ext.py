@@ -602,8 +602,9 @@ def attention_cached(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     New row i sees every row before the new ones and, of those, row j where bit j of tree[b, i] (int64
     [batch, nodes]) is set, or j <= i without a tree.  nodes == 1 is the step of a single token.  A row that
     sees nothing gives zeros.  Rows from counts[b] on keep what `out` holds; without `out` they are zeros.
-    Cache rows behind lengths[b] may hold anything.  A page number outside the cache is not followed: its rows
-    count as hidden, and check_device_errors() raises."""
+    Cache rows behind lengths[b] may hold anything, and so may a new row's key where a row does not see it; its
+    value must be finite (0 times a NaN or an infinity is NaN), or it reaches the other rows of its sequence.  A page
+    number outside the cache is not followed: its rows count as hidden, and check_device_errors() raises."""
     qs = q.shape
     if len(qs) != 4:
         raise ValueError("attention_cached: q [batch, nodes, heads, dim] required")
