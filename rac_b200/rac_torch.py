@@ -517,6 +517,10 @@ class RACRoPEAttention(nn.Module):
     def n_kv_heads(self) -> int:
         return self.n_heads if self._kv_heads is None else self._kv_heads
 
+    @n_kv_heads.setter
+    def n_kv_heads(self, n: int) -> None:
+        self._kv_heads = n
+
     def _context(self, x, mask=None, is_causal=False, positions=None, n_heads=None):
         """Attention output before out_proj, [B, T, heads*d_head]."""
         B, T, _ = x.shape

@@ -31,6 +31,8 @@ def test_modules_without_grouped_heads_stay_as_they_were():
     assert not shard._needs_rows(None, None, None)
     kept = copy.deepcopy(R.RACRoPEAttention(64, 4, n_kv_heads=2))
     assert kept.n_kv_heads == 2 and kept._needs_rows(None, None, None)
+    kept.n_heads, kept.n_kv_heads = 2, 1                        # a shard of grouped heads
+    assert kept.n_kv_heads == 1 and kept._needs_rows(None, None, None)
 
 
 @gpu
