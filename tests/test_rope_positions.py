@@ -79,3 +79,12 @@ def test_table_rows(cuda, dt):
                        ((c.double(), s.double(), pos), "float32"), ((c, s, pos.cpu()), "CUDA")]:
         with pytest.raises(ValueError, match=word):
             ext.rope_rows(*call)
+
+
+def test_c_entry_refuses():
+    def call(cos=256, dtype=0, pos=256, width=4, n=3, rows=8, half=16, out=256):
+        return _lib.lib().rac_rope_rows_async(cos, 256, dtype, pos, width, n, rows, half, out, 256, None)
+
+    assert call(n=-1) == -2 and call(rows=-1) == -2 and call(half=0) == -2 and call(width=2) == -2
+    assert call(dtype=3) == -5 and call(cos=0) == -1 and call(pos=0) == -1 and call(out=0) == -1
+    assert call(n=0) == 0
